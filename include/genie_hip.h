@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define GENIE_ABI_VERSION 13
+#define GENIE_ABI_VERSION 14
 
 #define GENIE_F32 0
 #define GENIE_BF16 1
@@ -508,6 +508,50 @@ int genie_attention_lean_mode(int mask);
 /* Resident blocks per CU of a lean kernel at its launch configuration (which: 0 forward, 1 backward dQ, 2 backward dK / dV), as the HIP
  * runtime computes it; -1 on error.  Budget: 4 / 3 / 3. */
 int genie_attention_lean_occupancy(int which);
+
+/* ---------------------------------------------------------------------------------------------
+ * Sequence operators (ABI 14; packed_attention.hip, cached_attention.hip, decay_attention.hip).  Not in the reference, whose attention knows clips of
+ * one length: token streams of different lengths packed one behind the other, and their forms for single tokens.
+ *   - bf16 activations (rows, heads, width); *_strides = {row, head} in elements, multiples of 8, rows 16-byte aligned, row stride from the head width to
+ *     2^21; width a multiple of 8 up to 128.  Outputs and gradients are contiguous.
+ *   - cu: int32 DEVICE pointer, nseq + 1 entries from 0 on; sequence s owns rows cu[s] .. cu[s + 1].  Read on the device only, entries clamped to the rows that
+ *     exist.  Rows behind cu[nseq] are never read and zero in every output.
+ *   - all sums in a fixed order (no atomics); every workspace is the caller's, nothing is kept between calls.
+ * ------------------------------------------------------------------------------------------- */
+/* Causal softmax attention with hq query heads over hkv key / value heads (hq % hkv == 0): query i of a sequence sees keys 0 .. i + n_k - n_q; a query that sees
+ * none gives zeros.  lse [hq][rows_q] fp32 (optional in the forward): natural-log sum of the scaled scores' exponentials, -inf where nothing is seen. */
+int genie_packed_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int32_t* cu_q, const int32_t* cu_k, int nseq,
+                               int rows_q, int rows_k, int hq, int hkv, int dim, const int64_t* q_strides, const int64_t* k_strides,
+                               const int64_t* v_strides, float scale, void* stream);
+/* Its gradients; out, lse from the forward, delta_ws fp32 [hq][rows_q] scratch. */
+int genie_packed_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse, float* delta_ws, void* dq,
+                               void* dk, void* dv, const int32_t* cu_q, const int32_t* cu_k, int nseq, int rows_q, int rows_k, int hq, int hkv, int dim,
+                               const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int64_t* dout_strides, float scale,
+                               void* stream);
+/* One token per sequence against its cache.  q (batch, hq, dim); caches (batch, capacity, hkv, dim) with *c_strides = {batch, token, head}; lengths int32 [batch] on the
+ * device.  k_new / v_new (batch, hkv, dim), both or neither: written to place lengths[b] of the caches and attended to.  A negative length (without a new
+ * token: or zero) gives zeros and writes nothing, one without room in the cache NaN.  ws: genie_cached_attention_ws_floats. */
+int64_t genie_cached_attention_ws_floats(int batch, int hq, int hkv, int dim, int capacity);
+int genie_cached_attention_step(const void* q, const void* k_new, const void* v_new, void* k_cache, void* v_cache, const int32_t* lengths, void* out,
+                                float* ws, int64_t ws_floats, int batch, int hq, int hkv, int dim, int capacity, const int64_t* q_strides,
+                                const int64_t* kn_strides, const int64_t* vn_strides, const int64_t* kc_strides, const int64_t* vc_strides, float scale,
+                                void* stream);
+/* Linear attention with a decay per head: S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T, o_t = scale q_t S_t; log_decay fp32 [heads] on the device, <= 0.
+ * initial_state / final_state fp32 [nseq][heads][dk][dv], optional.  seg_ws (genie_decay_attention_ws_floats; may be 0): the states in front of the segments
+ * that long sequences are cut into -- the backward call reads the forward's. */
+int64_t genie_decay_attention_ws_floats(int nseq, int rows, int heads, int dk, int dv);
+int genie_decay_attention_fwd(const void* q, const void* k, const void* v, const float* log_decay, const int32_t* cu, const float* initial_state, void* out,
+                              float* final_state, float* seg_ws, int64_t seg_ws_floats, int nseq, int rows, int heads, int dk, int dv,
+                              const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, float scale, void* stream);
+/* Its gradients (rev_ws: a second workspace of the same size). */
+int genie_decay_attention_bwd(const void* q, const void* k, const void* v, const void* dout, const float* log_decay, const int32_t* cu,
+                              const float* initial_state, float* seg_ws, float* rev_ws, int64_t ws_floats, void* dq, void* dk_out, void* dv_out, int nseq,
+                              int rows, int heads, int dk, int dv, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                              const int64_t* dout_strides, float scale, void* stream);
+/* The recurrence for one token: state / new_state fp32 [batch][heads][dk][dv], the same buffer or disjoint ones. */
+int genie_decay_attention_step(const void* q, const void* k, const void* v, const float* log_decay, const float* state, float* new_state, void* out, int batch,
+                               int heads, int dk, int dv, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, float scale,
+                               void* stream);
 
 /* Debug / bring-up probes (used by tests only). */
 int genie_probe_ds_read_tr16(const void* lds_image_u16_2048, const int32_t* lane_byte_addr_64, void* out_u16_64x4,

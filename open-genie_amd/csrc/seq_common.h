@@ -1,0 +1,93 @@
+// Device helpers shared by the kernels that walk PACKED sequences (packed_attention.hip, decay_attention.hip) or a cache (cached_attention.hip):
+// the slot -> (sequence, tile) search, range-checked loads, the transposing LDS read as a builtin.
+#pragma once
+#include "attn_common.h"
+
+// ------------------------------------------------------------------------------------------------------------------------------
+// Work list of packed sequences without a host round trip.  Sequence s owns the slots from f(s) = cu[s] / TILE + s on: f is strictly
+// increasing and f(s + 1) - f(s) >= ceil(len_s / TILE), so every tile has a slot, at most nseq + 1 slots stay empty, and the number of slots
+// is known from the sizes alone: rows / TILE + nseq + 1.  The last, virtual sequence (index nseq) holds the rows behind the last real one.
+// cu is device memory nobody has checked: entries are clamped to [0, rows], so that wrong ones cost wrong results, never an access out of bounds.
+// ------------------------------------------------------------------------------------------------------------------------------
+struct SeqSlot { int seq, start, len, tile; };
+
+__device__ __forceinline__ int seq_cu(const int32_t* cu, int s, int rows) { return s <= 0 ? 0 : min(max(cu[s], 0), rows); }
+
+// The search is 64-way: one load and one ballot per level (one level up to 63 sequences), the same in every wave of the block.
+template <int TILE>
+__device__ __forceinline__ SeqSlot seq_find(const int32_t* cu, int nseq, int rows, int slot) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = nseq + 1;
+    while (n > 1) {
+        const int step = (n + 63) >> 6;
+        const int i = lane * step;
+        const bool ok = i < n && seq_cu(cu, lo + i, rows) / TILE + lo + i <= slot;
+        const int cnt = max(1, (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(ok)));
+        lo += (cnt - 1) * step;
+        n = min(step, n - (cnt - 1) * step);
+    }
+    SeqSlot r;
+    r.seq = __builtin_amdgcn_readfirstlane(lo);
+    r.start = __builtin_amdgcn_readfirstlane(seq_cu(cu, r.seq, rows));
+    const int end = r.seq < nseq ? __builtin_amdgcn_readfirstlane(seq_cu(cu, r.seq + 1, rows)) : rows;
+    r.len = max(0, end - r.start);
+    r.tile = slot - (r.start / TILE + r.seq);
+    return r;
+}
+
+// The same closed form with TILE a launch argument (the decay kernels' segment length).
+__device__ __forceinline__ SeqSlot seq_find_n(const int32_t* cu, int nseq, int rows, int tile_rows, int slot) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = nseq + 1;
+    while (n > 1) {
+        const int step = (n + 63) >> 6;
+        const int i = lane * step;
+        const bool ok = i < n && seq_cu(cu, lo + i, rows) / tile_rows + lo + i <= slot;
+        const int cnt = max(1, (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(ok)));
+        lo += (cnt - 1) * step;
+        n = min(step, n - (cnt - 1) * step);
+    }
+    SeqSlot r;
+    r.seq = __builtin_amdgcn_readfirstlane(lo);
+    r.start = __builtin_amdgcn_readfirstlane(seq_cu(cu, r.seq, rows));
+    const int end = r.seq < nseq ? __builtin_amdgcn_readfirstlane(seq_cu(cu, r.seq + 1, rows)) : rows;
+    r.len = max(0, end - r.start);
+    r.tile = slot - (r.start / tile_rows + r.seq);
+    return r;
+}
+
+// ------------------------------------------------------------------------------------------------------------------------------
+// Range-checked 16-B load: lanes whose offset reaches past `bytes_left` get zeros.  Offsets are inside one tile (the base moves in 64 bits), and the
+// host refuses row strides whose tile does not fit 2^28 bytes.  SEQ_OOB marks a lane that never has data (columns behind the head's width).
+// ------------------------------------------------------------------------------------------------------------------------------
+#define SEQ_OOB 0x7ff00000u
+__device__ __forceinline__ u32x4_t seq_load16(const void* base, int bytes_left, uint32_t voff) {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, bytes_left, 0x00020000);
+    return __builtin_amdgcn_raw_buffer_load_b128(r, voff, 0, 0);
+}
+// bytes a tile may read from its first row on, when `rows` rows remain
+__device__ __forceinline__ int seq_bytes_left(long long rows, long long stride_bytes, int dim) {
+    if (rows <= 0) return 0;
+    const long long b = (rows - 1) * stride_bytes + dim * 2;
+    return (int)(b < 0x3fff0000ll ? b : 0x3fff0000ll);
+}
+
+// ds_read_b64_tr_b16: in each group of 16 lanes, lane i names 4 consecutive 16-bit values of row i / 4 (columns 4 (i % 4) ...) and receives column i of the
+// four rows.  The builtin: the compiler tracks the wait itself (tiles here are staged through registers, no LDS-DMA is in flight beside it).
+typedef __attribute__((address_space(3))) bf16x4_t seq_lds_b16x4;
+__device__ __forceinline__ bf16x4_t seq_tr16(const char* p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((seq_lds_b16x4*)p); }
+
+__device__ __forceinline__ bf16x8_t seq_pack8(const float a0, const float a1, const float a2, const float a3, const float a4, const float a5, const float a6,
+                                              const float a7) {
+    const u32x4_t v = {pack_bf16x2(a0, a1), pack_bf16x2(a2, a3), pack_bf16x2(a4, a5), pack_bf16x2(a6, a7)};
+    return __builtin_bit_cast(bf16x8_t, v);
+}
+
+// value of the partner lane (lane ^ 32) combined with this lane's.  Inline asm as in the other attention kernels: given two copies of one value the
+// builtin is folded as if the swap were the identity; no memory is involved, `s_nop 1` covers the VALU-write -> permlane-read hazard.
+__device__ __forceinline__ void seq_swap32(float& a, float& b) { asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b)); }
+__device__ __forceinline__ float seq_xmax32(float x) { float a = x, b = x; seq_swap32(a, b); return fmaxf(a, b); }
+__device__ __forceinline__ float seq_xsum32(float x) { float a = x, b = x; seq_swap32(a, b); return a + b; }
+
+// row of accumulator register r in the 32 x 32 MFMA result layout (column = lane & 31), h = lane >> 5
+__device__ __forceinline__ constexpr int seq_crow(int r) { return (r & 3) + 8 * (r >> 2); }

@@ -15,7 +15,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get('GENIE_HIP_LIB', os.path.join(os.path.dirname(_HERE), 'lib', 'libgenie_hip.so'))
 
 GENIE_F32, GENIE_BF16 = 0, 1
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 
 class GenieTap(C.Structure):
@@ -136,6 +136,14 @@ SIGNATURES = {
     'genie_attention_dropout_mask': (C.c_int, [_P, _I, _I, _I, _I, _F, C.c_uint64, _P]),
     'genie_attention_lean_mode': (C.c_int, [_I]),
     'genie_attention_lean_occupancy': (C.c_int, [_I]),
+    'genie_packed_attention_fwd': (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _PL, _PL, _PL, _F, _P]),
+    'genie_packed_attention_bwd': (C.c_int, [_P] * 12 + [_I] * 6 + [_PL] * 4 + [_F, _P]),
+    'genie_cached_attention_ws_floats': (C.c_int64, [_I, _I, _I, _I, _I]),
+    'genie_cached_attention_step': (C.c_int, [_P] * 8 + [_L] + [_I] * 5 + [_PL] * 5 + [_F, _P]),
+    'genie_decay_attention_ws_floats': (C.c_int64, [_I, _I, _I, _I, _I]),
+    'genie_decay_attention_fwd': (C.c_int, [_P] * 9 + [_L] + [_I] * 5 + [_PL] * 3 + [_F, _P]),
+    'genie_decay_attention_bwd': (C.c_int, [_P] * 9 + [_L] + [_P] * 3 + [_I] * 5 + [_PL] * 4 + [_F, _P]),
+    'genie_decay_attention_step': (C.c_int, [_P] * 7 + [_I] * 4 + [_PL] * 3 + [_F, _P]),
     'genie_probe_ds_read_tr16': (C.c_int, [_P, _P, _P, _P]),
 }
 

@@ -25,6 +25,7 @@ from . import _hip
 from .cl import empty_like_cl, is_cl, pitch_of, to_cl
 from . import conv as _conv
 from .conv import ConvSpec, conv_dgrad, conv_forward, conv_wgrad, pack_weight_bwd, pack_weight_fwd
+from .sequence import cached_attention_step, decay_attention, decay_attention_step, packed_attention      # noqa: F401  (public operators of this module)
 
 DIRECT_PARAM_GRADS = __import__('os').environ.get('GENIE_DIRECT_PARAM_GRADS', 'arena')
 
