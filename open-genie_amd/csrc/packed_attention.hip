@@ -525,10 +525,12 @@ template <typename K>
 static int packed_launch(K kernel, const PackedArgs& a, int64_t blocks, int threads, int lds, void* stream) {
     GENIE_CHECK_ARG(blocks < (1ll << 31), "packed attention: too many blocks");
     if (blocks <= 0) return GENIE_OK;
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (e != hipSuccess) {
-        genie_set_error("packed attention: %s", hipGetErrorString(e));
-        return GENIE_ERR_HIP;
+    if (lds > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) {
+            genie_set_error("packed attention: %s", hipGetErrorString(e));
+            return GENIE_ERR_HIP;
+        }
     }
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), lds, (hipStream_t)stream, a);
     GENIE_CHECK_LAUNCH();
