@@ -523,8 +523,9 @@ int genie_attention_lean_occupancy(int which);
 int genie_packed_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int32_t* cu_q, const int32_t* cu_k, int nseq,
                                int rows_q, int rows_k, int hq, int hkv, int dim, const int64_t* q_strides, const int64_t* k_strides,
                                const int64_t* v_strides, float scale, void* stream);
-/* Its gradients; out, lse from the forward, delta_ws fp32 [hq][rows_q] scratch. */
-int genie_packed_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse, float* delta_ws, void* dq,
+/* Its gradients; out, lse from the forward, ws: genie_packed_attention_bwd_ws_floats, 16-byte aligned. */
+int64_t genie_packed_attention_bwd_ws_floats(int nseq, int rows_q, int rows_k, int hq, int hkv, int dim);
+int genie_packed_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse, float* ws, int64_t ws_floats, void* dq,
                                void* dk, void* dv, const int32_t* cu_q, const int32_t* cu_k, int nseq, int rows_q, int rows_k, int hq, int hkv, int dim,
                                const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int64_t* dout_strides, float scale,
                                void* stream);

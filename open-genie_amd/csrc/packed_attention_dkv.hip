@@ -1,0 +1,232 @@
+// Backward of packed causal attention, dK and dV (see packed_attention.hip for the formulas and the walk).
+//
+// A wave owns 32 KT keys of one key head and walks the query rows that see them, head after head of the group -- the sum over the group's heads happens in
+// the accumulators, in a fixed order.  S = Q K^T (lane = key): P and dS are operand-shaped for dV^T = dO^T P and dK^T = Q^T dS.  The rows' -lse / scale and
+// -delta are the accumulators' INPUT, read from LDS beside the tile, so that P = exp2(c S) and dS = P dP cost one multiplication each.
+//
+// Head widths above 64: KT = 2 and ONE wave per SIMD (this file is built without -amdgpu-mfma-vgpr-form: the 256 accumulator registers of dK and dV live in the AGPR
+// half of the file, K and V fragments in 128 of the others).  Every Q / dO fragment read from LDS feeds two products, and with 64 products per 32 rows the
+// matrix pipe has work while the exponentials run.  At 32 keys per wave the same registers hold half the work: two waves per SIMD need 192 of their 256
+// for K, V, dK and dV, which leaves one fragment in flight, and every product then waits out an LDS read.
+// Head widths up to 64: KT = 1, three waves per SIMD hide each other's latencies.
+#include "packed_common.h"
+
+template <int DH, int KT, int WPE>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) packed_dkv_kernel(const PackedArgs a) {
+    using G = PackedGeo<DH>;
+    constexpr int NW = 4, BN = 32 * KT * NW, NT = 64 * NW, STAGE = 2 * G::TILE + 512;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    const int kvh = (int)blockIdx.x % a.hkv, part = (int)blockIdx.x / a.hkv % a.nsplit, slot = (int)blockIdx.x / a.hkv / a.nsplit, group = a.hq / a.hkv;
+    // (slots ascending: the first keys of a sequence are seen by most rows)
+    const SeqSlot s = seq_find<BN>(a.cu_k, a.nseq, a.rows_k, slot);
+    if (s.tile < 0 || s.tile * BN >= s.len) return;
+    if (s.seq == a.nseq) {
+        if (a.nsplit > 1) return;                                               // (the reduction writes those rows)
+        packed_zero_rows<BN, NT>(a.dk, a.hkv, a.dim, s, kvh);
+        packed_zero_rows<BN, NT>(a.dv, a.hkv, a.dim, s, kvh);
+        return;
+    }
+    const int qstart = seq_cu(a.cu_q, s.seq, a.rows_q), qlen = max(0, seq_cu(a.cu_q, s.seq + 1, a.rows_q) - qstart);
+    const int shift = s.len - qlen;                                             // key j is seen by rows i >= j - shift
+    const int j0 = s.tile * BN + wave * 32 * KT, kj = j0 + (lane & 31);
+    const int first = max(0, s.tile * BN - shift) & ~63;                        // first query row the block needs, on a tile border
+    const int w_first = j0 - shift;
+    const int tiles = max(0, (qlen - first + 63) >> 6);
+    const int64_t all = (int64_t)tiles * group;                                 // (head, tile) steps; this block takes its part of them
+    const int i0 = (int)(all * part / a.nsplit), i1 = (int)(all * (part + 1) / a.nsplit);
+
+    bf16x8_t kf[KT][G::KS], vf[KT][G::KS];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+        const int64_t krow = s.start + kj + 32 * kt;
+        packed_row_frags<DH>(kf[kt], a.k + krow * a.k_row + kvh * a.k_head, kj + 32 * kt < s.len, a.dim);
+        packed_row_frags<DH>(vf[kt], a.v + krow * a.v_row + kvh * a.v_head, kj + 32 * kt < s.len, a.dim);
+    }
+    f32x16_t dk[KT][G::DT], dv[KT][G::DT];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int d = 0; d < G::DT; ++d) dk[kt][d] = dv[kt][d] = packed_splat(0.f);
+    const float c2 = a.scale * 1.4426950408889634f, inv_scale = 1.f / a.scale;
+
+    PackedDma<DH, NW> st;
+    st.init(wave, lane, a.dim, a.q_row, a.g_row);
+    float stat = 0.f;                                                           // threads 0..63: -lse / scale, 64..127: -delta of the tile's rows
+    auto load = [&](int i) {
+        const int head = kvh * group + i / tiles, r0 = first + (i % tiles) * 64;
+        const bf16_t* qp = a.q + (int64_t)(qstart + r0) * a.q_row + head * a.q_head;
+        const bf16_t* gp = a.dout + (int64_t)(qstart + r0) * a.g_row + head * a.g_head;
+        char* to = smem + (i & 1) * STAGE;
+        st.load(wave, qp, seq_bytes_left(qlen - r0, a.q_row * 2, a.dim), to, gp, seq_bytes_left(qlen - r0, a.g_row * 2, a.dim), to + G::TILE);
+        if (tid < 128) {
+            const int row = r0 + (tid & 63);
+            const int64_t at = (int64_t)head * a.rows_q + qstart + row;
+            stat = tid < 64 ? -INFINITY : 0.f;
+            if (row < qlen) {
+                const float x = tid < 64 ? a.lse[at] : a.delta[at];
+                stat = tid >= 64 ? -x : (x == -INFINITY ? -INFINITY : -x * inv_scale);
+            }
+        }
+    };
+    PackedLane<DH> at;
+    at.init(lane);
+
+    // 32 query rows rbase .. of the staged tile
+    auto rows32 = [&](const char* qt_, const char* gt_, const float* stats, int rbase) {
+        f32x16_t sacc[KT], dp[KT];                                              // start at -lse / scale and -delta: p = exp2(c2 S), dS = p dP
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const f32x4_t x = *reinterpret_cast<const f32x4_t*>(stats + 8 * g + 4 * h), y = *reinterpret_cast<const f32x4_t*>(stats + 64 + 8 * g + 4 * h);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) { sacc[kt][4 * g + e] = x[e]; dp[kt][4 * g + e] = y[e]; }
+        }
+#pragma unroll
+        for (int ks = 0; ks < G::KS; ++ks) {
+            const bf16x8_t qa = at.row_frag(qt_, ks), ga = at.row_frag(gt_, ks);
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+                sacc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qa, kf[kt][ks], sacc[kt], 0, 0, 0);
+                dp[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ga, vf[kt][ks], dp[kt], 0, 0, 0);
+            }
+        }
+        if (rbase < w_first + 32 * KT - 1) {                                    // some of these rows do not see all of the wave's keys
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+                const int lim = kj + 32 * kt - shift - rbase - 4 * h;           // rows below do not see this lane's key
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sacc[kt][r] = seq_crow(r) >= lim ? sacc[kt][r] : -INFINITY;
+            }
+        }
+        bf16x8_t pf[KT][2], ds[KT][2];
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2) {
+                float p[8], x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int r = 8 * s2 + e;
+                    p[e] = __builtin_amdgcn_exp2f(sacc[kt][r] * c2);
+                    x[e] = p[e] * dp[kt][r];
+                }
+                pf[kt][s2] = seq_pack8(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]);
+                ds[kt][s2] = seq_pack8(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
+            }
+        }
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+            for (int d = 0; d < G::DT; ++d) {
+                const bf16x8_t gt = at.tr_frag(gt_ + s2 * 16 * G::PITCH, d), qt = at.tr_frag(qt_ + s2 * 16 * G::PITCH, d);
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    dv[kt][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(gt, pf[kt][s2], dv[kt][d], 0, 0, 0);
+                    dk[kt][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qt, ds[kt][s2], dk[kt][d], 0, 0, 0);
+                }
+            }
+    };
+
+    if (i0 < i1) load(i0);
+    for (int i = i0; i < i1; ++i) {
+        const char* qt_ = smem + (i & 1) * STAGE;
+        const char* gt_ = qt_ + G::TILE;
+        float* stats = reinterpret_cast<float*>(smem + (i & 1) * STAGE + 2 * G::TILE);
+        if (tid < 128) stats[tid] = stat;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                        // this wave's slabs of tile i have landed ...
+        __syncthreads();                                                        // ... and everybody's
+        if (i + 1 < i1) load(i + 1);
+        const int r0 = first + (i % tiles) * 64;
+        if (r0 + 63 < w_first) continue;                                        // (wave-uniform) no row of these 64 sees this wave's keys
+        at.forget();
+#pragma unroll 1
+        for (int qt = 0; qt < 2; ++qt) rows32(qt_ + qt * 32 * G::PITCH, gt_ + qt * 32 * G::PITCH, stats + qt * 32, r0 + qt * 32);
+    }
+    if (a.nsplit > 1) {                                                         // fp32 parts, 16 B per lane and store
+        float* pk = a.part + (((int64_t)part * 2 * a.rows_k + s.start) * a.hkv + kvh) * a.dim;
+        float* pv = pk + (int64_t)a.rows_k * a.hkv * a.dim;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+            const int j = kj + 32 * kt;
+            if (j >= s.len) continue;
+            const int64_t at = (int64_t)j * a.hkv * a.dim;
+#pragma unroll
+            for (int d = 0; d < G::DT; ++d)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int col = 32 * d + 8 * g + 4 * h;
+                    if (col < a.dim) {
+                        *reinterpret_cast<f32x4_t*>(pk + at + col) = f32x4_t{dk[kt][d][4 * g], dk[kt][d][4 * g + 1], dk[kt][d][4 * g + 2], dk[kt][d][4 * g + 3]};
+                        *reinterpret_cast<f32x4_t*>(pv + at + col) = f32x4_t{dv[kt][d][4 * g], dv[kt][d][4 * g + 1], dv[kt][d][4 * g + 2], dv[kt][d][4 * g + 3]};
+                    }
+                }
+        }
+        return;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+        const int j = j0 + 32 * kt;
+        if (j >= s.len) break;
+        const int64_t to = ((int64_t)(s.start + j) * a.hkv + kvh) * a.dim;
+        char* region = smem + wave * 32 * G::PITCH;                             // (one region per wave: LDS serves a wave's accesses in order)
+        packed_write_rows<DH>(region, dk[kt], a.scale, a.dk + to, (int64_t)a.hkv * a.dim, min(32, s.len - j), a.dim);
+        packed_write_rows<DH>(region, dv[kt], 1.f, a.dv + to, (int64_t)a.hkv * a.dim, min(32, s.len - j), a.dim);
+    }
+}
+
+// dK, dV <- the parts' sums in order, rounded once; zeros behind the last sequence
+__global__ void __launch_bounds__(256) packed_dkv_sum_kernel(const PackedArgs a) {
+    const int64_t n = (int64_t)a.rows_k * a.hkv * a.dim, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+    if (i >= n) return;
+    const bool live = i / (a.hkv * a.dim) < seq_cu(a.cu_k, a.nseq, a.rows_k);
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (live)
+            for (int p = 0; p < a.nsplit; ++p) {
+                const float* src = a.part + (int64_t)(2 * p + m) * n + i;
+                const f32x4_t x = *reinterpret_cast<const f32x4_t*>(src), y = *reinterpret_cast<const f32x4_t*>(src + 4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { f[e] += x[e]; f[4 + e] += y[e]; }
+            }
+        if (m == 0)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] *= a.scale;
+        *reinterpret_cast<u32x4_t*>((m ? a.dv : a.dk) + i) = pack8(f);
+    }
+}
+
+#ifndef PACKED_DKV_BLOCKS
+#define PACKED_DKV_BLOCKS 1024
+#endif
+// parts a tile's (head, row tile) steps are cut into: as many as bring the launch to about PACKED_DKV_BLOCKS blocks, at most 8 and no more than there can be steps
+static int packed_dkv_splits(int nseq, int rows_q, int rows_k, int hq, int hkv, int dim) {
+    const int64_t blocks = (int64_t)(rows_k / (dim > 64 ? 256 : 128) + (nseq < rows_k ? nseq : rows_k)) * hkv, steps = (int64_t)(rows_q / 64 + 1) * (hq / hkv);
+    int64_t n = blocks > 0 ? (PACKED_DKV_BLOCKS + blocks / 2) / blocks : 1;
+    n = n < steps ? n : steps;
+    return (int)(n < 1 ? 1 : n > 8 ? 8 : n);
+}
+extern "C" int64_t genie_packed_attention_bwd_ws_floats(int nseq, int rows_q, int rows_k, int hq, int hkv, int dim) {
+    if (nseq < 0 || rows_q <= 0 || rows_k <= 0 || hkv <= 0 || hq <= 0 || hq % hkv != 0 || dim <= 0) return 0;
+    const int n = packed_dkv_splits(nseq, rows_q, rows_k, hq, hkv, dim);
+    return (int64_t)hq * rows_q + 4 + (n > 1 ? (int64_t)2 * n * rows_k * hkv * dim : 0);      // delta (rounded up to 16 B), parts
+}
+
+template <int DH, int KT, int WPE>
+static int packed_dkv_dispatch(PackedArgs& a, void* stream) {
+    a.nslots = a.rows_k / (128 * KT) + a.nseq + 1;
+    const int rc = packed_launch(packed_dkv_kernel<DH, KT, WPE>, a, (int64_t)a.nslots * a.hkv * a.nsplit, 256, 4 * PackedGeo<DH>::TILE + 1024, stream);
+    if (rc != GENIE_OK || a.nsplit == 1) return rc;
+    return packed_launch(packed_dkv_sum_kernel, a, ((int64_t)a.rows_k * a.hkv * a.dim / 8 + 255) / 256, 256, 0, stream);
+}
+int packed_dkv_run(PackedArgs& a, void* stream) {
+    a.nsplit = packed_dkv_splits(a.nseq, a.rows_q, a.rows_k, a.hq, a.hkv, a.dim);
+    a.part = a.delta + ((int64_t)a.hq * a.rows_q + 3) / 4 * 4;
+    if (a.dim <= 32) return packed_dkv_dispatch<32, 1, 3>(a, stream);
+    if (a.dim <= 64) return packed_dkv_dispatch<64, 1, 3>(a, stream);
+    if (a.dim <= 96) return packed_dkv_dispatch<96, 2, 1>(a, stream);
+    return packed_dkv_dispatch<128, 2, 1>(a, stream);
+}

@@ -65,6 +65,11 @@ __device__ __forceinline__ u32x4_t seq_load16(const void* base, int bytes_left, 
     const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, bytes_left, 0x00020000);
     return __builtin_amdgcn_raw_buffer_load_b128(r, voff, 0, 0);
 }
+// the same load with its destination in LDS: lane l's 16 B go to lds + 16 l (lds is wave-uniform)
+__device__ __forceinline__ void seq_dma16(const void* base, int bytes_left, char* lds, uint32_t voff) {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, bytes_left, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, LDS_PTR(lds), 16, voff, 0u, 0, 0);
+}
 // bytes a tile may read from its first row on, when `rows` rows remain
 __device__ __forceinline__ int seq_bytes_left(long long rows, long long stride_bytes, int dim) {
     if (rows <= 0) return 0;

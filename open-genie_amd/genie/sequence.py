@@ -165,9 +165,10 @@ class _PackedAttention(torch.autograd.Function):
         dk = torch.empty((rows_k, hkv, d), dtype=torch.bfloat16, device=q.device)
         dv = torch.empty_like(dk)
         if rows and rows_k:
-            delta = torch.empty((hq, rows), dtype=torch.float32, device=q.device)
             P = _hip.ptr
-            _launch('genie_packed_attention_bwd', q.device, P(q), P(k), P(v), P(out), P(dout), P(lse), P(delta), P(dq), P(dk), P(dv), P(cu_q), P(cu_k),
+            nws = _hip.load_library().genie_packed_attention_bwd_ws_floats(cu_q.shape[0] - 1, rows, rows_k, hq, hkv, d)
+            ws = torch.empty(nws, dtype=torch.float32, device=q.device)
+            _launch('genie_packed_attention_bwd', q.device, P(q), P(k), P(v), P(out), P(dout), P(lse), P(ws), nws, P(dq), P(dk), P(dv), P(cu_q), P(cu_k),
                     cu_q.shape[0] - 1, rows, rows_k, hq, hkv, d, _i64(sq), _i64(sk), _i64(sv), _i64(sg), scale)
         else:
             for t in (dq, dk, dv):
