@@ -538,15 +538,15 @@ int genie_cached_attention_step(const void* q, const void* k_new, const void* v_
                                 const int64_t* kn_strides, const int64_t* vn_strides, const int64_t* kc_strides, const int64_t* vc_strides, float scale,
                                 void* stream);
 /* Linear attention with a decay per head: S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T, o_t = scale q_t S_t; log_decay fp32 [heads] on the device, <= 0.
- * initial_state / final_state fp32 [nseq][heads][dk][dv], optional.  seg_ws (genie_decay_attention_ws_floats; may be 0): the states in front of the segments
- * that long sequences are cut into -- the backward call reads the forward's. */
-int64_t genie_decay_attention_ws_floats(int nseq, int rows, int heads, int dk, int dv);
+ * initial_state / final_state fp32 [nseq][heads][dk][dv], optional.  Sequences are cut into segments; states (bf16: the states in front of the segments, which the
+ * backward call reads again) and ws (fp32) hold genie_decay_attention_state_elems elements each, with_state = initial_state || final_state; it may be 0. */
+int64_t genie_decay_attention_state_elems(int nseq, int rows, int heads, int dk, int dv, int with_state);
 int genie_decay_attention_fwd(const void* q, const void* k, const void* v, const float* log_decay, const int32_t* cu, const float* initial_state, void* out,
-                              float* final_state, float* seg_ws, int64_t seg_ws_floats, int nseq, int rows, int heads, int dk, int dv,
+                              float* final_state, void* states, float* ws, int64_t state_elems, int nseq, int rows, int heads, int dk, int dv,
                               const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, float scale, void* stream);
-/* Its gradients (rev_ws: a second workspace of the same size). */
-int genie_decay_attention_bwd(const void* q, const void* k, const void* v, const void* dout, const float* log_decay, const int32_t* cu,
-                              const float* initial_state, float* seg_ws, float* rev_ws, int64_t ws_floats, void* dq, void* dk_out, void* dv_out, int nseq,
+/* Its gradients.  states: the forward's; rev_states, ws: genie_decay_attention_state_elems(.., 0) elements of bf16 and fp32; has_initial: the forward had a state. */
+int genie_decay_attention_bwd(const void* q, const void* k, const void* v, const void* dout, const float* log_decay, const int32_t* cu, int has_initial,
+                              const void* states, void* rev_states, float* ws, int64_t state_elems, void* dq, void* dk_out, void* dv_out, int nseq,
                               int rows, int heads, int dk, int dv, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
                               const int64_t* dout_strides, float scale, void* stream);
 /* The recurrence for one token: state / new_state fp32 [batch][heads][dk][dv], the same buffer or disjoint ones. */

@@ -4,35 +4,37 @@
 //
 // The forward and the three gradients are ONE form,  y_t = scale sum_{s <= t} l^(t-s) (a_t . b_s) c_s :
 //   o = form(q, k, v)   dq = form(do, v, k)   and, run from the sequence's end,   dv = form(k, q, do)   dk = form(v, do, q)
-// with the state M = sum l^.. b_s c_s^T (for dq the transpose of the forward's, for dk that of dv's).  Chunks of 64 tokens:
-//   y = l^(t+1) a_t M + (A B^T o D) C,  D_ts = l^(t-s) for s <= t;     M <- l^64 M + sum_s l^(63-s) b_s c_s^T
+// Segments of 256 tokens:  y_t = l^(t+1) a_t M + sum over the segment's own s <= t,  M = the state in front of the segment (for dq the transpose of the
+// forward's, for dk that of dv's).  Three kernels:
+//   state: what each segment adds, sum_s l^(n-1-s) b_s c_s^T          -- reads B and C once; parallel over segments, 64 tokens at a time
+//   scan:  the states in front of the segments, elementwise in fp32    -- stored as the bf16 operand that the products take
+//   out:   all rows at once, a wave owns 32: its product with M, then the segment's keys up to its diagonal, as softmax attention without the softmax
+// A single walk through each sequence that keeps M in registers would read everything once, but has only (sequences x heads) blocks and
+// a chain of dependent products per 64 tokens.  256 tokens balance the quadratic part (2.5 tiles of 64 keys a row) against the states
+// (at head width 128 an fp32 matrix is as large as 128 tokens of q, k, v and o).
 // All powers have exponents >= 0 (strong decays underflow to 0, nothing overflows).
 //
-// A block walks one SEGMENT of a sequence for one head; wave w owns columns 32 w .. 32 w + 31 of C, of the output and of M, which lives in its
-// accumulators: as the bf16 operand of a M it needs no exchange, because the accumulator layout is the operand layout up to an order of the
-// contraction index, and A and B are staged in that order.  Long sequences are cut into segments so that few sequences still fill 256 CUs: the segments'
-// own states first (B and C only), an elementwise scan over them, then all segments at once.
-//
-// Roundings to bf16: the scores and M as matrix operands of an output that is itself rounded to bf16 (M itself stays fp32).  The state update must not
-// round its decayed operand, because the state is an fp32 result that lives on: l^(63-s) c_s goes in as a sum of two bf16 values (2^-16 left).
-#include "seq_common.h"
-#include "genie_hip.h"
+// Roundings to bf16: the scores and M as matrix operands of an output that is itself rounded to bf16.  The states themselves are fp32 and so is what goes into them:
+// the state update's decayed operand l^(n-1-s) c_s enters as a sum of two bf16 values (2^-16 left).
+#include "packed_common.h"
+
+#define DECAY_SEG 256
 
 struct DecayRole {
     const bf16_t *a, *b, *c;
     bf16_t* y;                                   // [rows][heads][dc]
     int64_t a_row, a_head, b_row, b_head, c_row, c_head;
-    int da, dc, reverse;
-    int m_a, m_c;                                // element strides of M inside a stored matrix (the transposed use swaps them)
-    const float* seq_state;                      // state in front of each sequence, [nseq][heads][matrix], or NULL
-    float* seg_state;                            // [slot][heads][matrix]: state in front of every segment but a sequence's first
+    int da, dc, reverse, m_rows_a;               // m_rows_a: the stored states' rows are a's columns (else c's): the transposed use
+    float* local;                                // [slot][heads][dc][da] fp32: what each segment adds
+    bf16_t* states;                              // [slot][heads][dc][da] (m_rows_a: [da][dc]): state in front of each segment, or NULL
+    const float* initial;                        // [nseq][heads][da][dc]: state in front of each sequence, or NULL
     float* final_state;                          // [nseq][heads][da][dc], or NULL
 };
 struct DecayArgs {
     DecayRole r[3];
     const int32_t* cu;
     const float* log_decay;
-    int nseq, rows, heads, seg, nslots;
+    int nseq, rows, heads;
     float scale;
 };
 
@@ -45,17 +47,15 @@ struct DecayGeo {
 // l^e for e >= 0 (l = 0 included: l^0 = 1)
 __device__ __forceinline__ float decay_pow(float log2_l, int e) { return e == 0 ? 1.f : __builtin_amdgcn_exp2f(log2_l * (float)e); }
 
-// One 64-token tile of a matrix from memory into registers and on to LDS.  A chunk with nv < 64 tokens (a sequence's last) sits in the tile's LAST rows, so that
+// One 64-token tile of a matrix from memory into registers and on to LDS.  A chunk with nv < 64 tokens (a segment's last) sits in the tile's LAST rows, so that
 // the weights towards the chunk's end, l^(63-s), hold for it too; the rows in front of it read zeros: their offsets wrap past any range (forward) or lie
 // behind the last token (reverse, where row i of the tile is the token 63 - i rows up in memory).
-// ORDERED: inside each 16 columns the four 8-B pieces are stored in the order 0, 2, 1, 3, so that a lane half's 16 B are columns 4 h .. 4 h + 3 and
-// 8 + 4 h .. 8 + 4 h + 3 -- the accumulator layout's rows.
 // A thread's four pieces are 16 rows apart in one column chunk (the swizzle's keys use row bits 0..3: one LDS address and constant offsets).
-template <int DH, bool ORDERED>
+template <int DH>
 struct DecayTile {
     using G = DecayGeo<DH>;
     static_assert(G::NT / G::CPR == 16 && G::NT % G::CPR == 0, "pieces are 16 rows apart");
-    uint32_t off, lds0, lds1;
+    uint32_t off, lds;
     int step;
     u32x4_t r[G::PIECES];
     const bf16_t* base;
@@ -66,18 +66,11 @@ struct DecayTile {
         base = first; row = stride; dim = width; rev = reverse;
         const int rr = tid / G::CPR, c = tid % G::CPR;
         off = c * 8 < dim ? (uint32_t)((reverse ? 63 - rr : rr) * stride * 2) + c * 16 : SEQ_OOB;
-        step = (int)(reverse ? -32 * stride : 32 * stride);
-        if (c * 8 >= dim) step = 0;
-        if (ORDERED) {
-            lds0 = (uint32_t)(rr * G::PITCH + (attn_swz<G::SW>(rr, c & ~1) << 4) + (c & 1) * 8);
-            lds1 = (uint32_t)(rr * G::PITCH + (attn_swz<G::SW>(rr, c | 1) << 4) + (c & 1) * 8);
-        } else {
-            lds0 = (uint32_t)(rr * G::PITCH + (attn_swz<G::SW>(rr, c) << 4));
-        }
+        step = c * 8 < dim ? (int)(reverse ? -32 * stride : 32 * stride) : 0;
+        lds = packed_at<DH>(rr, c);
     }
     // the chunk of tokens p .. p + nv - 1 of the walk over a sequence of len tokens (reverse: counted from its end)
-    __device__ __forceinline__ void load(int p, int len) {
-        const int nv = min(64, len - p);
+    __device__ __forceinline__ void load(int p, int nv, int len) {
         const bf16_t* t = base + (int64_t)(rev ? len - p - nv : p) * row;
         const int left = seq_bytes_left(nv, row * 2, dim);
         const uint32_t o = off - (rev ? 0u : (uint32_t)((64 - nv) * row * 2));
@@ -86,74 +79,12 @@ struct DecayTile {
     }
     __device__ __forceinline__ void store(char* tile) const {
 #pragma unroll
-        for (int i = 0; i < G::PIECES; ++i) {
-            if constexpr (ORDERED) {
-                *reinterpret_cast<u32x2_t*>(tile + lds0 + i * 16 * G::PITCH) = u32x2_t{r[i][0], r[i][1]};
-                *reinterpret_cast<u32x2_t*>(tile + lds1 + i * 16 * G::PITCH) = u32x2_t{r[i][2], r[i][3]};
-            } else {
-                *reinterpret_cast<u32x4_t*>(tile + lds0 + i * 16 * G::PITCH) = r[i];
-            }
-        }
+        for (int i = 0; i < G::PIECES; ++i) *reinterpret_cast<u32x4_t*>(tile + lds + i * 16 * G::PITCH) = r[i];
     }
 };
 
-// lane offset of a transposing read of columns col0 + (lane & 31), rows 4 h + 0..3 (+ 8 rows: second = true) of a 16-row step
-template <int DH, bool ORDERED>
-__device__ __forceinline__ uint32_t decay_tr_offset(int lane, int col0, bool second) {
-    using G = DecayGeo<DH>;
-    const int g16 = lane >> 4, row = 4 * (g16 >> 1) + ((lane >> 2) & 3) + (second ? 8 : 0);
-    const int piece = (col0 + 16 * (g16 & 1) + 4 * (lane & 3)) >> 2;
-    int chunk = piece >> 1, half = piece & 1;
-    if (ORDERED) { const int c = chunk; chunk = (c & ~1) + half; half = c & 1; }
-    return (uint32_t)(row * G::PITCH + (attn_swz<G::SW>(row, chunk) << 4) + half * 8);
-}
-__device__ __forceinline__ bf16x8_t decay_tr(const char* tile, uint32_t o0, uint32_t o1) {
-    const bf16x4_t lo = seq_tr16(tile + o0), hi = seq_tr16(tile + o1);
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-}
-
-// M <- all M + sum_s l^(63-s) b_s c_s^T over a staged chunk (cf: this wave's 32 columns of C, transposed fragments).
-// fade[r] = l^(31 - row r of a 32-row half), p32 = l^32.
-template <int DH>
-__device__ __forceinline__ void decay_update(f32x16_t (&m)[DecayGeo<DH>::DT], const char* bt, const uint32_t (&boff)[DecayGeo<DH>::DT][2], const bf16x8_t (&cf)[4],
-                                             float all, const float (&fade)[16], float p32) {
-    using G = DecayGeo<DH>;
-#pragma unroll
-    for (int i = 0; i < G::DT; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) m[i][r] *= all;
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-        float hi[8], lo[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            hi[j] = bf16_to_f32((bf16_t)cf[ks][j]) * fade[8 * (ks & 1) + j];
-            if (ks < 2) hi[j] *= p32;
-        }
-        const u32x4_t fh = {pack_bf16x2(hi[0], hi[1]), pack_bf16x2(hi[2], hi[3]), pack_bf16x2(hi[4], hi[5]), pack_bf16x2(hi[6], hi[7])};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            lo[2 * j] = hi[2 * j] - __uint_as_float(fh[j] << 16);
-            lo[2 * j + 1] = hi[2 * j + 1] - __uint_as_float(fh[j] & 0xffff0000u);
-        }
-        const bf16x8_t fl = seq_pack8(lo[0], lo[1], lo[2], lo[3], lo[4], lo[5], lo[6], lo[7]);
-#pragma unroll
-        for (int i = 0; i < G::DT; ++i) {
-            const bf16x8_t bf = decay_tr(bt + ks * 16 * G::PITCH, boff[i][0], boff[i][1]);
-            m[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bf, __builtin_bit_cast(bf16x8_t, fh), m[i], 0, 0, 0);
-            m[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bf, fl, m[i], 0, 0, 0);
-        }
-    }
-}
-
-__device__ __forceinline__ f32x16_t decay_zero() {
-    f32x16_t x;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) x[r] = 0.f;
-    return x;
-}
-
-// The state each segment leaves behind when it starts from nothing (every segment but a sequence's last), into the slot AFTER its own.
+// What one segment adds to the state, M = sum_s l^(n-1-s) b_s c_s^T over its n tokens, stored transposed ([dc][da]); wave w owns columns 32 w .. of C.  A
+// sequence's last segment is only needed where the final state is.
 template <int DH>
 __global__ void __launch_bounds__(64 * (DH / 32), 2) decay_state_kernel(const DecayArgs g) {
     using G = DecayGeo<DH>;
@@ -161,231 +92,269 @@ __global__ void __launch_bounds__(64 * (DH / 32), 2) decay_state_kernel(const De
     const DecayRole& R = g.r[0];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int head = (int)blockIdx.x % g.heads, slot = (int)blockIdx.x / g.heads;
-    const SeqSlot s = seq_find_n(g.cu, g.nseq, g.rows, g.seg, slot);
-    if (s.seq == g.nseq || s.tile < 0 || (int64_t)(s.tile + 1) * g.seg >= s.len) return;
+    const SeqSlot s = seq_find<DECAY_SEG>(g.cu, g.nseq, g.rows, slot);
+    const int p0 = s.tile * DECAY_SEG;
+    if (s.seq == g.nseq || s.tile < 0 || p0 >= s.len) return;
+    if (p0 + DECAY_SEG >= s.len && !R.final_state) return;
+    const int p1 = min(s.len, p0 + DECAY_SEG);
     const float log2_l = g.log_decay[head] * 1.4426950408889634f;
     float fade[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) fade[r] = decay_pow(log2_l, 31 - (seq_crow(r) + 4 * h));
     const float p32 = decay_pow(log2_l, 32);
-    uint32_t boff[G::DT][2], coff[2];
-#pragma unroll
-    for (int i = 0; i < G::DT; ++i) { boff[i][0] = decay_tr_offset<DH, true>(lane, 32 * i, false); boff[i][1] = decay_tr_offset<DH, true>(lane, 32 * i, true); }
-    coff[0] = decay_tr_offset<DH, false>(lane, 32 * wave, false);
-    coff[1] = decay_tr_offset<DH, false>(lane, 32 * wave, true);
-    DecayTile<DH, true> tb;
-    DecayTile<DH, false> tc;
+    PackedLane<DH> at;
+    at.init(lane);
+    DecayTile<DH> tb, tc;
     tb.init(tid, R.b + (int64_t)s.start * R.b_row + head * R.b_head, R.b_row, R.da, R.reverse);
     tc.init(tid, R.c + (int64_t)s.start * R.c_row + head * R.c_head, R.c_row, R.dc, R.reverse);
     f32x16_t m[G::DT];
 #pragma unroll
-    for (int i = 0; i < G::DT; ++i) m[i] = decay_zero();
-    const int p0 = s.tile * g.seg, p1 = p0 + g.seg;
+    for (int i = 0; i < G::DT; ++i) m[i] = packed_splat(0.f);
     char *bt = smem, *ct = smem + G::TILE;
-    tb.load(p0, s.len);
-    tc.load(p0, s.len);
-    for (int p = p0; p < p1; p += 64) {
+    // the chunk that does not fill a tile comes first: all others end where the next one begins
+    int nv = (p1 - p0 - 1) % 64 + 1;
+    tb.load(p0, nv, s.len);
+    tc.load(p0, nv, s.len);
+    for (int p = p0; p < p1;) {
         tb.store(bt);
         tc.store(ct);
         __syncthreads();
-        if (p + 64 < p1) { tb.load(p + 64, s.len); tc.load(p + 64, s.len); }
-        bf16x8_t cf[4];
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) cf[ks] = decay_tr(ct + ks * 16 * G::PITCH, coff[0], coff[1]);
-        decay_update<DH>(m, bt, boff, cf, p32 * p32, fade, p32);
-        __syncthreads();
-    }
-    float* dst = R.seg_state + ((int64_t)(slot + 1) * g.heads + head) * R.da * R.dc;
-    const int col = 32 * wave + (lane & 31);
-    if (col < R.dc) {
+        p += nv;
+        nv = 64;
+        if (p < p1) {
+            tb.load(p, 64, s.len);
+            tc.load(p, 64, s.len);
+        }
+        at.forget();
 #pragma unroll
         for (int i = 0; i < G::DT; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int row = 32 * i + seq_crow(r) + 4 * h;
-                if (row < R.da) dst[(uint32_t)(row * R.dc + col)] = m[i][r];
+            for (int r = 0; r < 16; ++r) m[i][r] *= p32 * p32;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            const bf16x8_t cf = at.tr_frag(ct + ks * 16 * G::PITCH, wave);
+            float hi[8], lo[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                hi[j] = bf16_to_f32((bf16_t)cf[j]) * fade[8 * (ks & 1) + j];
+                if (ks < 2) hi[j] *= p32;
             }
+            const u32x4_t fh = {pack_bf16x2(hi[0], hi[1]), pack_bf16x2(hi[2], hi[3]), pack_bf16x2(hi[4], hi[5]), pack_bf16x2(hi[6], hi[7])};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                lo[2 * j] = hi[2 * j] - __uint_as_float(fh[j] << 16);
+                lo[2 * j + 1] = hi[2 * j + 1] - __uint_as_float(fh[j] & 0xffff0000u);
+            }
+            const bf16x8_t fl = seq_pack8(lo[0], lo[1], lo[2], lo[3], lo[4], lo[5], lo[6], lo[7]);
+#pragma unroll
+            for (int i = 0; i < G::DT; ++i) {
+                const bf16x8_t bf = at.tr_frag(bt + ks * 16 * G::PITCH, i);
+                m[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, fh), bf, m[i], 0, 0, 0);
+                m[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fl, bf, m[i], 0, 0, 0);
+            }
+        }
+        __syncthreads();
     }
-}
-
-// seg_state[first slot + i] <- l^seg (state in front of segment i - 1) + (what segment i - 1 adds), i = 1 ..: elementwise over the matrix, one thread per four
-// elements, the next segments' values requested ahead of the chain.
-__global__ void __launch_bounds__(256) decay_scan_kernel(const DecayArgs g, int matrix) {
-    const DecayRole& R = g.r[0];
-    const int seq = (int)blockIdx.x / g.heads, head = (int)blockIdx.x % g.heads;
-    const int e = ((int)blockIdx.y * 256 + (int)threadIdx.x) * 4;
-    if (e >= matrix) return;
-    const int start = seq_cu(g.cu, seq, g.rows), len = max(0, seq_cu(g.cu, seq + 1, g.rows) - start);
-    const int nseg = (len + g.seg - 1) / g.seg;
-    if (nseg < 2) return;
-    const float l = decay_pow(g.log_decay[head] * 1.4426950408889634f, g.seg);
-    f32x4_t m = {0.f, 0.f, 0.f, 0.f};
-    if (R.seq_state) m = *reinterpret_cast<const f32x4_t*>(R.seq_state + ((int64_t)seq * g.heads + head) * matrix + e);
-    const int64_t step = (int64_t)g.heads * matrix;
-    // first slot of the sequence; wrong cu contents can reach past the last slot: clamp
-    const int s0 = start / g.seg + seq, last = min(nseg - 1, g.nslots - 1 - s0);
-    float* p = R.seg_state + ((int64_t)(s0 + 1) * g.heads + head) * matrix + e;
-    int i = 0;
-    for (; i + 8 <= last; i += 8) {
-        f32x4_t x[8];
+    float* dst = R.local + ((int64_t)slot * g.heads + head) * R.da * R.dc;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = *reinterpret_cast<const f32x4_t*>(p + (i + j) * step);
+    for (int i = 0; i < G::DT; ++i) {
+        const int col = 32 * i + (lane & 31);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) m[q] = __builtin_fmaf(m[q], l, x[j][q]);
-            *reinterpret_cast<f32x4_t*>(p + (i + j) * step) = m;
+        for (int r = 0; r < 16; ++r) {
+            const int row = 32 * wave + seq_crow(r) + 4 * h;
+            if (col < R.da && row < R.dc) dst[(uint32_t)(row * R.da + col)] = m[i][r];
         }
     }
-    for (; i < last; ++i) {
-        const f32x4_t x = *reinterpret_cast<const f32x4_t*>(p + i * step);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) m[q] = __builtin_fmaf(m[q], l, x[q]);
-        *reinterpret_cast<f32x4_t*>(p + i * step) = m;
-    }
 }
 
+// States in front of the segments: M_0 = initial or 0, M_{i+1} = l^256 M_i + local_i, elementwise in fp32 with a thread per four elements; each M_i is stored rounded
+// to bf16 as the operand that it becomes, the last sum is the final state.  The segments' values are requested eight ahead of the chain.
+__global__ void __launch_bounds__(256) decay_scan_kernel(const DecayArgs g) {
+    const DecayRole& R = g.r[0];
+    const int seq = (int)blockIdx.x / g.heads, head = (int)blockIdx.x % g.heads, matrix = R.da * R.dc;
+    const int e = ((int)blockIdx.y * 256 + (int)threadIdx.x) * 4;
+    if (e >= matrix) return;
+    const int start = seq_cu(g.cu, seq, g.rows), len = max(0, seq_cu(g.cu, seq + 1, g.rows) - start), nseg = (len + DECAY_SEG - 1) / DECAY_SEG;
+    const float log2_l = g.log_decay[head] * 1.4426950408889634f, l = decay_pow(log2_l, DECAY_SEG);
+    const int c = e / R.da, a = e % R.da;                                       // element (a .. a + 3, c) of the natural matrix
+    f32x4_t m = {0.f, 0.f, 0.f, 0.f};
+    if (R.initial) {
+        const float* src = R.initial + ((int64_t)seq * g.heads + head) * matrix;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m[j] = src[(a + j) * R.dc + c];
+    }
+    const int64_t step = (int64_t)g.heads * matrix, first = ((int64_t)(start / DECAY_SEG + seq) * g.heads + head) * matrix + e;
+    const float* src = R.local + first;
+    bf16_t* dst = R.states + first;
+    const int full = nseg - 1;                                                  // segments whose sum is followed by another segment
+    f32x4_t x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (j < full) x[j] = *reinterpret_cast<const f32x4_t*>(src + j * step);
+    for (int i = 0; i < full; i += 8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (i + j >= full) break;
+            *reinterpret_cast<u32x2_t*>(dst + (i + j) * step) = u32x2_t{pack_bf16x2(m[0], m[1]), pack_bf16x2(m[2], m[3])};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) m[q] = __builtin_fmaf(m[q], l, x[j][q]);
+            if (i + j + 8 < full) x[j] = *reinterpret_cast<const f32x4_t*>(src + (i + j + 8) * step);
+        }
+    }
+    if (nseg > 0) *reinterpret_cast<u32x2_t*>(dst + (nseg - 1) * step) = u32x2_t{pack_bf16x2(m[0], m[1]), pack_bf16x2(m[2], m[3])};
+    if (!R.final_state) return;
+    if (nseg > 0) {
+        const f32x4_t last = *reinterpret_cast<const f32x4_t*>(src + (nseg - 1) * step);
+        const float ln = decay_pow(log2_l, len - (nseg - 1) * DECAY_SEG);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) m[q] = __builtin_fmaf(m[q], ln, last[q]);
+    }
+    float* out = R.final_state + ((int64_t)seq * g.heads + head) * matrix;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[(a + j) * R.dc + c] = m[j];
+}
+
+// A pair of 64-row tiles straight into LDS, as PackedDma, for tokens walked in either direction (reverse: row i is token nv - 1 - i from the base; the rows behind
+// the nv-th wrap past any range).
 template <int DH>
-__global__ void __launch_bounds__(64 * (DH / 32), 2) decay_sweep_kernel(const DecayArgs g) {
-    using G = DecayGeo<DH>;
-    __shared__ __attribute__((aligned(16))) char smem[4 * G::TILE];
+struct DecayDma {
+    using G = PackedGeo<DH>;
+    static constexpr int SLABS = G::TILE / 1024 / 4, ROWS = 1024 / G::PITCH;
+    int row0, slot;
+    __device__ __forceinline__ void init(int wave, int lane) { row0 = wave * SLABS * ROWS + lane / G::SW; slot = lane % G::SW; }
+    __device__ __forceinline__ void load(int wave, char* tile, const bf16_t* base, int64_t stride, int rows, int dim, int rev_last) {
+        asm volatile("" : "+v"(row0), "+v"(slot));                              // (offsets are formed anew: registers are short)
+        const int left = seq_bytes_left(rows, stride * 2, dim);
+        const uint32_t pitch = (uint32_t)(stride * 2);
+#pragma unroll
+        for (int i = 0; i < SLABS; ++i) {
+            const int row = row0 + i * ROWS, c = attn_swz<G::SW>(row, slot);
+            const uint32_t o = (uint32_t)(rev_last >= 0 ? rev_last - row : row) * pitch + c * 16;
+            seq_dma16(base, left, tile + (wave * SLABS + i) * 1024, c * 8 < dim ? o : SEQ_OOB);
+        }
+    }
+};
+
+#ifndef DECAY_OUT_WPE64
+#define DECAY_OUT_WPE64 3
+#endif
+// All outputs of one role: four waves of 32 rows, the state in front of the segment as tile pair 0 of the walk, the segment's keys after it.
+template <int DH>
+__global__ void __launch_bounds__(256, DH <= 64 ? DECAY_OUT_WPE64 : 2) decay_out_kernel(const DecayArgs g) {
+    using G = PackedGeo<DH>;
+    constexpr int BM = 128;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
     const DecayRole& R = g.r[blockIdx.y];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int head = (int)blockIdx.x % g.heads, slot = (int)blockIdx.x / g.heads;
-    const int64_t matrix = (int64_t)R.da * R.dc;
-    if (slot >= g.nslots) {                                                     // (launched when final states are asked for) sequences without tokens
-        const int seq = slot - g.nslots;
-        if (R.final_state && seq_cu(g.cu, seq + 1, g.rows) <= seq_cu(g.cu, seq, g.rows)) {
-            const int64_t at = ((int64_t)seq * g.heads + head) * matrix;
-            for (int i = tid; i < matrix; i += G::NT) R.final_state[at + i] = R.seq_state ? R.seq_state[at + i] : 0.f;
-        }
+    const SeqSlot s = seq_find<BM>(g.cu, g.nseq, g.rows, slot);
+    if (s.tile < 0 || s.tile * BM >= s.len) return;
+    if (s.seq == g.nseq) {
+        packed_zero_rows<BM, 256>(R.y, g.heads, R.dc, s, head);
         return;
     }
-    const SeqSlot s = seq_find_n(g.cu, g.nseq, g.rows, g.seg, slot);
-    const int p0 = s.tile * g.seg;
-    if (s.tile < 0 || p0 >= s.len) return;
-    const int p1 = min(s.len, p0 + g.seg), cpr = R.dc / 8;
-    if (s.seq == g.nseq) {                                                      // rows behind the last sequence
-        for (int i = tid; i < (p1 - p0) * cpr; i += G::NT)
-            *reinterpret_cast<u32x4_t*>(R.y + ((int64_t)(s.start + p0 + i / cpr) * g.heads + head) * R.dc + (i % cpr) * 8) = u32x4_t{0, 0, 0, 0};
-        return;
-    }
+    const int rev = R.reverse, r0 = s.tile * BM, seg = r0 / DECAY_SEG, seg0 = seg * DECAY_SEG, end = min(s.len, r0 + BM);
+    const int q0 = r0 + wave * 32, qi = q0 + (lane & 31);                        // rows in the order of the walk
     const float log2_l = g.log_decay[head] * 1.4426950408889634f;
-    float near[16], fade[16];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const int k = seq_crow(r) + 4 * h, d = (lane & 31) - k;                 // query - key inside a 32 x 32 tile on the diagonal
-        near[r] = d >= 0 ? decay_pow(log2_l, max(0, d)) : 0.f;
-        fade[r] = decay_pow(log2_l, 31 - k);
-    }
-    const float next = decay_pow(log2_l, (lane & 31) + 1), p32 = decay_pow(log2_l, 32);
-    uint32_t roff[G::KS], boff[G::DT][2], coff[2];
-#pragma unroll
-    for (int ks = 0; ks < G::KS; ++ks) roff[ks] = (uint32_t)((lane & 31) * G::PITCH + (attn_swz<G::SW>(lane & 31, 2 * ks + h) << 4));
-#pragma unroll
-    for (int i = 0; i < G::DT; ++i) { boff[i][0] = decay_tr_offset<DH, true>(lane, 32 * i, false); boff[i][1] = decay_tr_offset<DH, true>(lane, 32 * i, true); }
-    coff[0] = decay_tr_offset<DH, false>(lane, 32 * wave, false);
-    coff[1] = decay_tr_offset<DH, false>(lane, 32 * wave, true);
+    const bool carried = R.states && (seg > 0 || R.initial);                     // M is not zero
+    const int tiles = (end - seg0 + 63) >> 6;
 
-    f32x16_t m[G::DT];
-    const float* init = p0 > 0 ? R.seg_state + ((int64_t)slot * g.heads + head) * matrix
-                               : (R.seq_state ? R.seq_state + ((int64_t)s.seq * g.heads + head) * matrix : nullptr);
-    const int mcol = 32 * wave + (lane & 31);
-    // (clamped addresses and selects: a branch per element would make the compiler copy whole accumulators)
-    const float keep = init && mcol < R.dc ? 1.f : 0.f;
-    const float* from = init ? init : g.log_decay;
-    const int mc_ = mcol < R.dc ? mcol * R.m_c : 0;
-#pragma unroll
-    for (int i = 0; i < G::DT; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int row = 32 * i + seq_crow(r) + 4 * h;
-            const float x = from[(uint32_t)(init && row < R.da ? row * R.m_a + mc_ : 0)];
-            m[i][r] = keep != 0.f && row < R.da ? x : 0.f;
+    const bf16_t* arow = R.a + (int64_t)(s.start + (rev ? s.len - 1 - qi : qi)) * R.a_row + head * R.a_head;
+    bf16x8_t af[G::KS];
+    packed_row_frags<DH>(af, arow, qi < s.len, R.da);
+    const bf16_t* bp = R.b + (int64_t)s.start * R.b_row + head * R.b_head;
+    const bf16_t* cp = R.c + (int64_t)s.start * R.c_row + head * R.c_head;
+    DecayDma<DH> st;
+    st.init(wave, lane);
+    auto load = [&](int t) {                                                     // t = -1: the state; 0 ..: keys
+        char* to = smem + ((t + 1) & 1) * 2 * G::TILE;
+        if (t < 0) {
+            const int mr = R.m_rows_a ? R.da : R.dc, mc = R.m_rows_a ? R.dc : R.da;
+            const bf16_t* m = R.states + ((int64_t)(s.start / DECAY_SEG + s.seq + seg) * g.heads + head) * mr * mc;
+            st.load(wave, to, m, mc, min(64, mr), mc, -1);
+            if (DH > 64) st.load(wave, to + G::TILE, m + 64 * mc, mc, mr - 64, mc, -1);
+            return;
         }
+        const int p = seg0 + t * 64, nv = min(64, s.len - p), from = rev ? s.len - p - nv : p;
+        st.load(wave, to, bp + (int64_t)from * R.b_row, R.b_row, nv, R.da, rev ? nv - 1 : -1);
+        st.load(wave, to + G::TILE, cp + (int64_t)from * R.c_row, R.c_row, nv, R.dc, rev ? nv - 1 : -1);
+    };
+    PackedLane<DH> at;
+    at.init(lane);
+    float fade[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) fade[r] = decay_pow(log2_l, 31 - (seq_crow(r) + 4 * h));
+    f32x16_t y[G::DT];
+#pragma unroll
+    for (int d = 0; d < G::DT; ++d) y[d] = packed_splat(0.f);
 
-    DecayTile<DH, true> ta, tb;
-    DecayTile<DH, false> tc;
-    ta.init(tid, R.a + (int64_t)s.start * R.a_row + head * R.a_head, R.a_row, R.da, R.reverse);
-    tb.init(tid, R.b + (int64_t)s.start * R.b_row + head * R.b_head, R.b_row, R.da, R.reverse);
-    tc.init(tid, R.c + (int64_t)s.start * R.c_row + head * R.c_head, R.c_row, R.dc, R.reverse);
-    const int orow = tid / G::CPR, ocol = (tid % G::CPR) * 8, oat = orow * G::PITCH + (attn_swz<G::SW>(orow, tid % G::CPR) << 4);
-    char *at = smem, *bt = at + G::TILE, *ct = bt + G::TILE, *yt = ct + G::TILE;
-    ta.load(p0, s.len);
-    tb.load(p0, s.len);
-    tc.load(p0, s.len);
-    for (int p = p0; p < p1; p += 64) {
-        ta.store(at);
-        tb.store(bt);
-        tc.store(ct);
+    load(carried ? -1 : 0);
+    if (carried) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        const int nv = min(64, p1 - p), blank = 64 - nv;                        // tile rows in front of the chunk's first token
-        const bool more = p + 64 < p1;
-        if (more) {
-            ta.load(p + 64, s.len);
-            tb.load(p + 64, s.len);
-            tc.load(p + 64, s.len);
-        }
-        bf16x8_t cf[4];
+        load(0);
+        if (!R.m_rows_a) {
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) cf[ks] = decay_tr(ct + ks * 16 * G::PITCH, coff[0], coff[1]);
+            for (int ks = 0; ks < G::KS; ++ks)
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt) {
-            bf16x8_t af[G::KS];
-#pragma unroll
-            for (int ks = 0; ks < G::KS; ++ks) af[ks] = *reinterpret_cast<const bf16x8_t*>(at + tt * 32 * G::PITCH + roff[ks]);
-            f32x16_t y = decay_zero();
+                for (int d = 0; d < G::DT; ++d) y[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at.row_frag(smem + d * 32 * G::PITCH, ks), af[ks], y[d], 0, 0, 0);
+        } else {
+            // the transposing read delivers columns of a in the accumulator order: this lane's row again, 4 + 4 values at a time
 #pragma unroll
             for (int ks = 0; ks < G::KS; ++ks) {
-                const int i = ks >> 1, r = 8 * (ks & 1);
-                const bf16x8_t mf = seq_pack8(m[i][r], m[i][r + 1], m[i][r + 2], m[i][r + 3], m[i][r + 4], m[i][r + 5], m[i][r + 6], m[i][r + 7]);
-                y = __builtin_amdgcn_mfma_f32_32x32x16_bf16(mf, af[ks], y, 0, 0, 0);
-            }
-            const float lead = decay_pow(log2_l, max(0, tt * 32 + (lane & 31) + 1 - blank));
+                u32x2_t lo = {0, 0}, hi = {0, 0};
+                const int col = ks * 16 + 4 * h;
+                if (qi < s.len && col < R.da) lo = *reinterpret_cast<const u32x2_t*>(arow + col);
+                if (qi < s.len && col + 8 < R.da) hi = *reinterpret_cast<const u32x2_t*>(arow + col + 8);
+                const bf16x8_t ap = __builtin_bit_cast(bf16x8_t, u32x4_t{lo[0], lo[1], hi[0], hi[1]});
 #pragma unroll
-            for (int r = 0; r < 16; ++r) y[r] *= lead;
-#pragma unroll
-            for (int st = 0; st <= tt; ++st) {
-                f32x16_t x = decay_zero();
-#pragma unroll
-                for (int ks = 0; ks < G::KS; ++ks)
-                    x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8_t*>(bt + st * 32 * G::PITCH + roff[ks]), af[ks], x, 0, 0, 0);
-#pragma unroll
-                for (int s2 = 0; s2 < 2; ++s2) {
-                    float w[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) w[e] = x[8 * s2 + e] * (st == tt ? near[8 * s2 + e] : fade[8 * s2 + e] * next);
-                    y = __builtin_amdgcn_mfma_f32_32x32x16_bf16(cf[2 * st + s2], seq_pack8(w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]), y, 0, 0, 0);
-                }
-            }
-            // y^T (column = token) to the output tile, rows = tokens
-            const int row = tt * 32 + (lane & 31);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const u32x2_t w = {pack_bf16x2(y[4 * q] * g.scale, y[4 * q + 1] * g.scale), pack_bf16x2(y[4 * q + 2] * g.scale, y[4 * q + 3] * g.scale)};
-                *reinterpret_cast<u32x2_t*>(yt + row * G::PITCH + (attn_swz<G::SW>(row, 4 * wave + q) << 4) + 8 * h) = w;
+                for (int d = 0; d < G::DT; ++d) y[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at.tr_frag(smem + ks * 16 * G::PITCH, d), ap, y[d], 0, 0, 0);
             }
         }
-        decay_update<DH>(m, bt, boff, cf, nv == 64 ? p32 * p32 : decay_pow(log2_l, nv), fade, p32);
-        __syncthreads();
+        const float lead = decay_pow(log2_l, qi - seg0 + 1);
 #pragma unroll
-        for (int i = 0; i < G::PIECES; ++i) {
-            const int rr = orow + 16 * i, t = p + rr - blank;
-            if (rr >= blank && ocol < R.dc) {
-                const int64_t tok = s.start + (R.reverse ? s.len - 1 - t : t);
-                *reinterpret_cast<u32x4_t*>(R.y + (tok * g.heads + head) * R.dc + ocol) = *reinterpret_cast<const u32x4_t*>(yt + oat + i * 16 * G::PITCH);
+        for (int d = 0; d < G::DT; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) y[d][r] *= lead;
+    }
+    for (int t = 0; t < tiles; ++t) {
+        char* bt = smem + ((t + 1) & 1) * 2 * G::TILE;
+        char* ct = bt + G::TILE;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (t + 1 < tiles) load(t + 1);
+        at.forget();
+#pragma unroll 1
+        for (int kt = 0; kt < 2; ++kt) {
+            const int k0 = seg0 + t * 64 + kt * 32;
+            if (k0 > q0) break;                                                  // (wave-uniform) behind this wave's rows
+            f32x16_t x = packed_splat(0.f);
+#pragma unroll
+            for (int ks = 0; ks < G::KS; ++ks) x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at.row_frag(bt + kt * 32 * G::PITCH, ks), af[ks], x, 0, 0, 0);
+            if (k0 == q0) {                                                      // the diagonal: l^(t-s) for s <= t
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int d = (lane & 31) - (seq_crow(r) + 4 * h);
+                    x[r] = d >= 0 ? x[r] * decay_pow(log2_l, max(0, d)) : 0.f;
+                }
+            } else {                                                             // l^(t-s) = l^(31 - s) l^(t + 1 + distance of the tiles - 32)
+                const float f = decay_pow(log2_l, (lane & 31) + 1 + q0 - k0 - 32);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[r] *= fade[r] * f;
+            }
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2) {
+                const bf16x8_t pf = seq_pack8(x[8 * s2], x[8 * s2 + 1], x[8 * s2 + 2], x[8 * s2 + 3], x[8 * s2 + 4], x[8 * s2 + 5], x[8 * s2 + 6], x[8 * s2 + 7]);
+#pragma unroll
+                for (int d = 0; d < G::DT; ++d) y[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at.tr_frag(ct + (kt * 2 + s2) * 16 * G::PITCH, d), pf, y[d], 0, 0, 0);
             }
         }
     }
-    if (R.final_state && p1 == s.len && mcol < R.dc) {
-        float* dst = R.final_state + ((int64_t)s.seq * g.heads + head) * matrix;
-#pragma unroll
-        for (int i = 0; i < G::DT; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int row = 32 * i + seq_crow(r) + 4 * h;
-                if (row < R.da) dst[(uint32_t)(row * R.dc + mcol)] = m[i][r];
-            }
+    __syncthreads();
+    if (q0 < s.len) {
+        const int64_t pitch = (int64_t)g.heads * R.dc;
+        packed_write_rows<DH>(smem + wave * 32 * G::PITCH, y, g.scale, R.y + ((int64_t)(s.start + (rev ? s.len - 1 - q0 : q0)) * g.heads + head) * R.dc,
+                              rev ? -pitch : pitch, min(32, s.len - q0), R.dc);
     }
 }
 
@@ -455,18 +424,10 @@ __global__ void __launch_bounds__(256) decay_step_kernel(const DecayStepArgs a) 
 // ------------------------------------------------------------------------------------------------------------------------------
 // C entry points
 // ------------------------------------------------------------------------------------------------------------------------------
-// tokens per segment: about 1024 blocks over the chip, but not under 256 tokens (a segment's state costs as much traffic as 128 / 256 tokens of it at head
-// width 64 / 128) and not over 4096
-static int decay_segment(int64_t rows, int heads) {
-    int seg = 256;
-    while (seg < 4096 && rows * heads / seg > 1024) seg *= 2;
-    return seg;
-}
-
-extern "C" int64_t genie_decay_attention_ws_floats(int nseq, int rows, int heads, int dk, int dv) {
-    if (nseq <= 0 || rows <= 0 || heads <= 0 || dk <= 0 || dv <= 0) return 0;
-    const int seg = decay_segment(rows, heads);
-    return rows <= seg ? 0 : (int64_t)(rows / seg + nseq + 1) * heads * dk * dv;
+// matrix elements of a call's segment states (one bf16 operand and one fp32 sum each); none where every sequence is one segment and no state goes in or out
+extern "C" int64_t genie_decay_attention_state_elems(int nseq, int rows, int heads, int dk, int dv, int with_state) {
+    if (nseq <= 0 || rows <= 0 || heads <= 0 || dk <= 0 || dv <= 0 || (rows <= DECAY_SEG && !with_state)) return 0;
+    return (int64_t)(rows / DECAY_SEG + nseq + 1) * heads * dk * dv;
 }
 
 static int decay_check(const char* what, const DecayArgs& g) {
@@ -487,32 +448,32 @@ static int decay_check_role(const char* what, const DecayRole& r) {
     return GENIE_OK;
 }
 
+// role 0's states, then all roles' outputs
 template <int DH>
-static int decay_run(const DecayArgs& g, int roles, bool build_states, bool empties, void* stream) {
-    const int NT = DecayGeo<DH>::NT;
-    const int64_t blocks = (int64_t)g.nslots * g.heads;
-    GENIE_CHECK_ARG(blocks + (int64_t)g.nseq * g.heads < (1ll << 31), "decay attention: too many blocks");
-    if (build_states && g.rows > g.seg && g.nseq > 0) {
-        hipLaunchKernelGGL(decay_state_kernel<DH>, dim3((unsigned)blocks), dim3(NT), 0, (hipStream_t)stream, g);
+static int decay_run(const DecayArgs& g, int roles, void* stream) {
+    const int64_t segs = (int64_t)(g.rows / DECAY_SEG + g.nseq + 1) * g.heads, blocks = (int64_t)(g.rows / 128 + g.nseq + 1) * g.heads;
+    GENIE_CHECK_ARG(segs < (1ll << 31) && blocks < (1ll << 31), "decay attention: too many blocks");
+    const DecayRole& r = g.r[0];
+    if (r.local && g.nseq > 0) {
+        hipLaunchKernelGGL(decay_state_kernel<DH>, dim3((unsigned)segs), dim3(DecayGeo<DH>::NT), 0, (hipStream_t)stream, g);
         GENIE_CHECK_LAUNCH();
-        const int matrix = g.r[0].da * g.r[0].dc;
-        hipLaunchKernelGGL(decay_scan_kernel, dim3((unsigned)(g.nseq * g.heads), (unsigned)((matrix + 1023) / 1024)), dim3(256), 0, (hipStream_t)stream, g, matrix);
+        hipLaunchKernelGGL(decay_scan_kernel, dim3((unsigned)(g.nseq * g.heads), (unsigned)((r.da * r.dc + 1023) / 1024)), dim3(256), 0, (hipStream_t)stream, g);
         GENIE_CHECK_LAUNCH();
     }
-    hipLaunchKernelGGL(decay_sweep_kernel<DH>, dim3((unsigned)(blocks + (empties ? (int64_t)g.nseq * g.heads : 0)), roles), dim3(NT), 0, (hipStream_t)stream, g);
+    hipLaunchKernelGGL(decay_out_kernel<DH>, dim3((unsigned)blocks, roles), dim3(256), 4 * PackedGeo<DH>::TILE, (hipStream_t)stream, g);
     GENIE_CHECK_LAUNCH();
     return GENIE_OK;
 }
-static int decay_run_any(const DecayArgs& g, int roles, bool build_states, bool empties, void* stream) {
+static int decay_run_any(const DecayArgs& g, int roles, void* stream) {
     const int d = g.r[0].da > g.r[0].dc ? g.r[0].da : g.r[0].dc;
-    if (d <= 32) return decay_run<32>(g, roles, build_states, empties, stream);
-    if (d <= 64) return decay_run<64>(g, roles, build_states, empties, stream);
-    if (d <= 96) return decay_run<96>(g, roles, build_states, empties, stream);
-    return decay_run<128>(g, roles, build_states, empties, stream);
+    if (d <= 32) return decay_run<32>(g, roles, stream);
+    if (d <= 64) return decay_run<64>(g, roles, stream);
+    if (d <= 96) return decay_run<96>(g, roles, stream);
+    return decay_run<128>(g, roles, stream);
 }
 
 extern "C" int genie_decay_attention_fwd(const void* q, const void* k, const void* v, const float* log_decay, const int32_t* cu, const float* initial_state, void* out,
-                                         float* final_state, float* seg_ws, int64_t seg_ws_floats, int nseq, int rows, int heads, int dk, int dv,
+                                         float* final_state, void* states, float* ws, int64_t state_elems, int nseq, int rows, int heads, int dk, int dv,
                                          const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, float scale, void* stream) {
     const char* what = "genie_decay_attention_fwd";
     GENIE_CHECK_ARG(q_strides && k_strides && v_strides, "%s: null strides", what);
@@ -520,21 +481,21 @@ extern "C" int genie_decay_attention_fwd(const void* q, const void* k, const voi
     g.cu = cu; g.log_decay = log_decay; g.nseq = nseq; g.rows = rows; g.heads = heads; g.scale = scale;
     int rc = decay_check(what, g);
     if (rc != GENIE_OK) return rc;
-    g.seg = decay_segment(rows, heads);
-    g.nslots = rows / g.seg + nseq + 1;
     DecayRole& r = g.r[0];
     r.a = (const bf16_t*)q; r.b = (const bf16_t*)k; r.c = (const bf16_t*)v; r.y = (bf16_t*)out;
     r.a_row = q_strides[0]; r.a_head = q_strides[1]; r.b_row = k_strides[0]; r.b_head = k_strides[1]; r.c_row = v_strides[0]; r.c_head = v_strides[1];
-    r.da = dk; r.dc = dv; r.m_a = dv; r.m_c = 1; r.seq_state = initial_state; r.seg_state = seg_ws; r.final_state = final_state;
+    r.da = dk; r.dc = dv; r.states = (bf16_t*)states; r.local = ws; r.initial = initial_state; r.final_state = final_state;
     rc = decay_check_role(what, r);
     if (rc != GENIE_OK) return rc;
-    GENIE_CHECK_ARG(seg_ws_floats >= genie_decay_attention_ws_floats(nseq, rows, heads, dk, dv) && (seg_ws || rows <= g.seg), "%s: workspace too small", what);
-    return decay_run_any(g, 1, true, final_state != nullptr, stream);
+    const int64_t need = genie_decay_attention_state_elems(nseq, rows, heads, dk, dv, initial_state || final_state);
+    GENIE_CHECK_ARG(state_elems >= need && (need == 0 || (states && ws)), "%s: workspace too small", what);
+    if (need == 0) { r.states = nullptr; r.local = nullptr; }
+    return decay_run_any(g, 1, stream);
 }
 
-extern "C" int genie_decay_attention_bwd(const void* q, const void* k, const void* v, const void* dout, const float* log_decay, const int32_t* cu,
-                                         const float* initial_state, float* seg_ws, float* rev_ws, int64_t ws_floats, void* dq, void* dk_out, void* dv_out, int nseq,
-                                         int rows, int heads, int dk, int dv, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+extern "C" int genie_decay_attention_bwd(const void* q, const void* k, const void* v, const void* dout, const float* log_decay, const int32_t* cu, int has_initial,
+                                         const void* states, void* rev_states, float* ws, int64_t state_elems, void* dq, void* dk_out, void* dv_out, int nseq, int rows,
+                                         int heads, int dk, int dv, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
                                          const int64_t* dout_strides, float scale, void* stream) {
     const char* what = "genie_decay_attention_bwd";
     GENIE_CHECK_ARG(q_strides && k_strides && v_strides && dout_strides, "%s: null strides", what);
@@ -542,25 +503,26 @@ extern "C" int genie_decay_attention_bwd(const void* q, const void* k, const voi
     g.cu = cu; g.log_decay = log_decay; g.nseq = nseq; g.rows = rows; g.heads = heads; g.scale = scale;
     int rc = decay_check(what, g);
     if (rc != GENIE_OK) return rc;
-    g.seg = decay_segment(rows, heads);
-    g.nslots = rows / g.seg + nseq + 1;
-    // role 0 is the one whose states are built here (reverse, from q and do): dv.  Role 1 uses their transposes: dk.  Role 2 uses the forward's: dq.
+    // role 0 is the one whose states are built here (from the end, of q and do): dv.  Role 1 uses their transposes: dk.  Role 2 those of the forward's: dq.
     DecayRole &rv = g.r[0], &rk = g.r[1], &rq = g.r[2];
     rv.a = (const bf16_t*)k; rv.b = (const bf16_t*)q; rv.c = (const bf16_t*)dout; rv.y = (bf16_t*)dv_out;
     rv.a_row = k_strides[0]; rv.a_head = k_strides[1]; rv.b_row = q_strides[0]; rv.b_head = q_strides[1]; rv.c_row = dout_strides[0]; rv.c_head = dout_strides[1];
-    rv.da = dk; rv.dc = dv; rv.reverse = 1; rv.m_a = dv; rv.m_c = 1; rv.seg_state = rev_ws;
+    rv.da = dk; rv.dc = dv; rv.reverse = 1;
     rk.a = (const bf16_t*)v; rk.b = (const bf16_t*)dout; rk.c = (const bf16_t*)q; rk.y = (bf16_t*)dk_out;
     rk.a_row = v_strides[0]; rk.a_head = v_strides[1]; rk.b_row = dout_strides[0]; rk.b_head = dout_strides[1]; rk.c_row = q_strides[0]; rk.c_head = q_strides[1];
-    rk.da = dv; rk.dc = dk; rk.reverse = 1; rk.m_a = 1; rk.m_c = dv; rk.seg_state = rev_ws;
+    rk.da = dv; rk.dc = dk; rk.reverse = 1; rk.m_rows_a = 1;
     rq.a = (const bf16_t*)dout; rq.b = (const bf16_t*)v; rq.c = (const bf16_t*)k; rq.y = (bf16_t*)dq;
     rq.a_row = dout_strides[0]; rq.a_head = dout_strides[1]; rq.b_row = v_strides[0]; rq.b_head = v_strides[1]; rq.c_row = k_strides[0]; rq.c_head = k_strides[1];
-    rq.da = dv; rq.dc = dk; rq.reverse = 0; rq.m_a = 1; rq.m_c = dv; rq.seq_state = initial_state; rq.seg_state = seg_ws;
+    rq.da = dv; rq.dc = dk; rq.m_rows_a = 1; rq.states = (bf16_t*)const_cast<void*>(states);
+    rq.initial = has_initial ? log_decay : nullptr;                             // (only asked whether it is there: the state itself is in `states`)
     for (int i = 0; i < 3; ++i) {
         rc = decay_check_role(what, g.r[i]);
         if (rc != GENIE_OK) return rc;
     }
-    GENIE_CHECK_ARG(ws_floats >= genie_decay_attention_ws_floats(nseq, rows, heads, dk, dv) && ((seg_ws && rev_ws) || rows <= g.seg), "%s: workspace too small", what);
-    return decay_run_any(g, 3, true, false, stream);
+    const int64_t need = genie_decay_attention_state_elems(nseq, rows, heads, dk, dv, 0);
+    GENIE_CHECK_ARG(state_elems >= need && (need == 0 || (states && rev_states && ws)) && (!has_initial || states), "%s: workspace too small", what);
+    if (need > 0) { rv.states = rk.states = (bf16_t*)rev_states; rv.local = ws; }
+    return decay_run_any(g, 3, stream);
 }
 
 extern "C" int genie_decay_attention_step(const void* q, const void* k, const void* v, const float* log_decay, const float* state, float* new_state, void* out, int batch,

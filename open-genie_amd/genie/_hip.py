@@ -141,9 +141,9 @@ SIGNATURES = {
     'genie_packed_attention_bwd': (C.c_int, [_P] * 7 + [_L] + [_P] * 5 + [_I] * 6 + [_PL] * 4 + [_F, _P]),
     'genie_cached_attention_ws_floats': (C.c_int64, [_I, _I, _I, _I, _I]),
     'genie_cached_attention_step': (C.c_int, [_P] * 8 + [_L] + [_I] * 5 + [_PL] * 5 + [_F, _P]),
-    'genie_decay_attention_ws_floats': (C.c_int64, [_I, _I, _I, _I, _I]),
-    'genie_decay_attention_fwd': (C.c_int, [_P] * 9 + [_L] + [_I] * 5 + [_PL] * 3 + [_F, _P]),
-    'genie_decay_attention_bwd': (C.c_int, [_P] * 9 + [_L] + [_P] * 3 + [_I] * 5 + [_PL] * 4 + [_F, _P]),
+    'genie_decay_attention_state_elems': (C.c_int64, [_I] * 6),
+    'genie_decay_attention_fwd': (C.c_int, [_P] * 10 + [_L] + [_I] * 5 + [_PL] * 3 + [_F, _P]),
+    'genie_decay_attention_bwd': (C.c_int, [_P] * 6 + [_I] + [_P] * 3 + [_L] + [_P] * 3 + [_I] * 5 + [_PL] * 4 + [_F, _P]),
     'genie_decay_attention_step': (C.c_int, [_P] * 7 + [_I] * 4 + [_PL] * 3 + [_F, _P]),
     'genie_probe_ds_read_tr16': (C.c_int, [_P, _P, _P, _P]),
 }

@@ -291,16 +291,17 @@ def _decay_forward(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, cu: Tenso
     (q, sq), (k, sk), (v, sv) = _rows(q), _rows(k), _rows(v)
     out = torch.empty((rows, h, dv), dtype=torch.bfloat16, device=dev)
     final = torch.empty((nseq, h, dk, dv), dtype=torch.float32, device=dev) if return_state else None
-    seg, nws = None, 0
+    states = ws = None
     if rows:
         P = _hip.ptr
-        nws = _hip.load_library().genie_decay_attention_ws_floats(nseq, rows, h, dk, dv)
-        seg = torch.empty(nws, dtype=torch.float32, device=dev) if nws else None
-        _launch('genie_decay_attention_fwd', dev, P(q), P(k), P(v), P(log_decay), P(cu), P(initial_state), P(out), P(final), P(seg), nws, nseq, rows, h, dk, dv,
+        n = _hip.load_library().genie_decay_attention_state_elems(nseq, rows, h, dk, dv, initial_state is not None or return_state)
+        if n:
+            states, ws = torch.empty(n, dtype=torch.bfloat16, device=dev), torch.empty(n, dtype=torch.float32, device=dev)
+        _launch('genie_decay_attention_fwd', dev, P(q), P(k), P(v), P(log_decay), P(cu), P(initial_state), P(out), P(final), P(states), P(ws), n, nseq, rows, h, dk, dv,
                 _i64(sq), _i64(sk), _i64(sv), scale)
     elif return_state:
         final.zero_() if initial_state is None else final.copy_(initial_state)
-    return out, final, ((q, k, v, log_decay, cu, initial_state, seg), (sq, sk, sv, scale, nws))
+    return out, final, ((q, k, v, log_decay, cu, states), (sq, sk, sv, scale, initial_state is not None))
 
 
 class _DecayAttention(torch.autograd.Function):
@@ -316,18 +317,19 @@ class _DecayAttention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout: Tensor, *_):
-        q, k, v, log_decay, cu, initial_state, seg = ctx.saved_tensors
-        sq, sk, sv, scale, nws = ctx.cfg
+        q, k, v, log_decay, cu, states = ctx.saved_tensors
+        sq, sk, sv, scale, has_initial = ctx.cfg
         rows, h, dk = q.shape
         dv, nseq, dev = v.shape[2], cu.shape[0] - 1, q.device
         dout, sg = _rows(dout)
         gq, gk = (torch.empty((rows, h, dk), dtype=torch.bfloat16, device=dev) for _ in range(2))
         gv = torch.empty((rows, h, dv), dtype=torch.bfloat16, device=dev)
         if rows:
-            rev = torch.empty(nws, dtype=torch.float32, device=dev) if nws else None
-            P = _hip.ptr
-            _launch('genie_decay_attention_bwd', dev, P(q), P(k), P(v), P(dout), P(log_decay), P(cu), P(initial_state), P(seg), P(rev), nws, P(gq), P(gk), P(gv), nseq,
-                    rows, h, dk, dv, _i64(sq), _i64(sk), _i64(sv), _i64(sg), scale)
+            n, rev, ws, P = _hip.load_library().genie_decay_attention_state_elems(nseq, rows, h, dk, dv, 0), None, None, _hip.ptr
+            if n:
+                rev, ws = torch.empty(n, dtype=torch.bfloat16, device=dev), torch.empty(n, dtype=torch.float32, device=dev)
+            _launch('genie_decay_attention_bwd', dev, P(q), P(k), P(v), P(dout), P(log_decay), P(cu), int(has_initial), P(states), P(rev), P(ws), n, P(gq), P(gk), P(gv),
+                    nseq, rows, h, dk, dv, _i64(sq), _i64(sk), _i64(sv), _i64(sg), scale)
         need = ctx.needs_input_grad
         return gq if need[0] else None, gk if need[1] else None, gv if need[2] else None, None, None, None, None, None
 

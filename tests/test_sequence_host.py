@@ -109,9 +109,9 @@ def test_c_entries_refuse_before_any_device_work():
     assert need > 0
     assert lib.genie_cached_attention_step(16, None, None, 16, 16, 16, 16, 16, need - 1, 1, 8, 2, 64, 4096, two, None, None, three, three, 1.0, None) == -1
     assert b'workspace' in lib.genie_last_error()
-    need = lib.genie_decay_attention_ws_floats(1, 4096, 8, 64, 64)
+    need = lib.genie_decay_attention_state_elems(1, 4096, 8, 64, 64, 0)
     assert need > 0
-    assert lib.genie_decay_attention_fwd(16, 16, 16, 16, 16, None, 16, None, 16, need - 1, 1, 4096, 8, 64, 64, two, two, two, 1.0, None) == -1
+    assert lib.genie_decay_attention_fwd(16, 16, 16, 16, 16, None, 16, None, 16, 16, need - 1, 1, 4096, 8, 64, 64, two, two, two, 1.0, None) == -1
     assert b'workspace' in lib.genie_last_error()
     assert lib.genie_decay_attention_step(16, 16, 16, 16, 16, 16, 16, 0, 8, 64, 64, two, two, two, 1.0, None) == -1
     assert isinstance(ctypes.c_int64(need).value, int)
