@@ -48,9 +48,11 @@ __global__ void __launch_bounds__(64 * NW, DH <= 64 ? 3 : 2) packed_fwd_kernel(c
     const bf16_t* vp = a.v + (int64_t)kstart * a.v_row + blk.kvh * a.v_head;
     PackedStage<DH, NT> st;
     st.init(tid, a.dim, a.k_row, a.v_row);
-    auto load = [&](int t) {
-        st.load(kp + (int64_t)t * 64 * a.k_row, seq_bytes_left(klen - t * 64, a.k_row * 2, a.dim), vp + (int64_t)t * 64 * a.v_row,
-                seq_bytes_left(klen - t * 64, a.v_row * 2, a.dim));
+    const int64_t k_step = 64 * a.k_row, v_step = 64 * a.v_row;
+    auto load = [&](int t) {                                                    // (called for t = 0, 1, 2 ..)
+        st.load(kp, seq_bytes_left(klen - t * 64, a.k_row * 2, a.dim), vp, seq_bytes_left(klen - t * 64, a.v_row * 2, a.dim));
+        kp += k_step;
+        vp += v_step;
     };
     PackedLane<DH> at;
     at.init(lane);
@@ -76,7 +78,8 @@ __global__ void __launch_bounds__(64 * NW, DH <= 64 ? 3 : 2) packed_fwd_kernel(c
                 for (int kt = 0; kt < 2; ++kt)
                     sacc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at.row_frag(kt_ + kt * 32 * G::PITCH, ks), qf[ks], sacc[kt], 0, 0, 0);
             if (k0 + 64 > klen || k0 + 63 > q0 + shift) {                       // the tile crosses the last key or the diagonal of these rows
-                const int lim = min(klen, qi + shift + 1) - k0 - 4 * h;
+                int lim = min(klen, qi + shift + 1) - k0 - 4 * h;
+                asm volatile("" : "+v"(lim));                                   // (the comparisons stay in this branch)
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -183,9 +186,11 @@ __global__ void __launch_bounds__(64 * NW, DH <= 64 ? 3 : 2) packed_dq_kernel(co
     const bf16_t* vp = a.v + (int64_t)kstart * a.v_row + blk.kvh * a.v_head;
     PackedStage<DH, NT> st;
     st.init(tid, a.dim, a.k_row, a.v_row);
-    auto load = [&](int t) {
-        st.load(kp + (int64_t)t * 64 * a.k_row, seq_bytes_left(klen - t * 64, a.k_row * 2, a.dim), vp + (int64_t)t * 64 * a.v_row,
-                seq_bytes_left(klen - t * 64, a.v_row * 2, a.dim));
+    const int64_t k_step = 64 * a.k_row, v_step = 64 * a.v_row;
+    auto load = [&](int t) {                                                    // (called for t = 0, 1, 2 ..)
+        st.load(kp, seq_bytes_left(klen - t * 64, a.k_row * 2, a.dim), vp, seq_bytes_left(klen - t * 64, a.v_row * 2, a.dim));
+        kp += k_step;
+        vp += v_step;
     };
     PackedLane<DH> at;
     at.init(lane);
@@ -208,8 +213,12 @@ __global__ void __launch_bounds__(64 * NW, DH <= 64 ? 3 : 2) packed_dq_kernel(co
                 sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at.row_frag(kt_ + kt * 32 * G::PITCH, ks), qf[ks], sacc, 0, 0, 0);
                 dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at.row_frag(vt_ + kt * 32 * G::PITCH, ks), gf[ks], dp, 0, 0, 0);
             }
-            const bool edge = k0 + 64 > klen || k0 + 63 > q0 + shift;
-            const int lim = min(klen, qi + shift + 1) - k0 - 4 * h;
+            if (k0 + 64 > klen || k0 + 63 > q0 + shift) {
+                int lim = min(klen, qi + shift + 1) - k0 - 32 * kt - 4 * h;
+                asm volatile("" : "+v"(lim));
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sacc[r] = seq_crow(r) < lim ? sacc[r] : -INFINITY;
+            }
             bf16x8_t ds[2];
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2) {
@@ -218,7 +227,6 @@ __global__ void __launch_bounds__(64 * NW, DH <= 64 ? 3 : 2) packed_dq_kernel(co
                 for (int e = 0; e < 8; ++e) {
                     const int r = 8 * s2 + e;
                     x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[r], c2, -lse2)) * dp[r];
-                    if (edge) x[e] = kt * 32 + seq_crow(r) < lim ? x[e] : 0.f;
                 }
                 ds[s2] = seq_pack8(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
             }

@@ -4,14 +4,14 @@
 // the accumulators, in a fixed order.  S = Q K^T (lane = key): P and dS are operand-shaped for dV^T = dO^T P and dK^T = Q^T dS.  The rows' -lse / scale and
 // -delta are the accumulators' INPUT, read from LDS beside the tile, so that P = exp2(c S) and dS = P dP cost one multiplication each.
 //
-// Head widths above 64: KT = 2 and ONE wave per SIMD (this file is built without -amdgpu-mfma-vgpr-form: the 256 accumulator registers of dK and dV live in the AGPR
-// half of the file, K and V fragments in 128 of the others).  Every Q / dO fragment read from LDS feeds two products, and with 64 products per 32 rows the
-// matrix pipe has work while the exponentials run.  At 32 keys per wave the same registers hold half the work: two waves per SIMD need 192 of their 256
-// for K, V, dK and dV, which leaves one fragment in flight, and every product then waits out an LDS read.
+// Head widths above 64: KT = 2 and ONE wave per SIMD.  dK and dV take 256 accumulator registers (the AGPR half of the file), the K fragments, S, dP, P and dS 160 of the
+// others; the V fragments, which would be 64 more, wait in LDS (129 of 160 KB: one block per CU anyway).  Every Q / dO fragment read from LDS feeds two
+// products, and with 64 products per 32 rows the matrix pipe has work while the exponentials run.  At 32 keys per wave and two waves per SIMD, K, V, dK and
+// dV take 192 of 256 registers, which leaves one fragment in flight, and every product waits out an LDS read.
 // Head widths up to 64: KT = 1, three waves per SIMD hide each other's latencies.
 #include "packed_common.h"
 
-template <int DH, int KT, int WPE>
+template <int DH, int KT, int WPE, bool VLDS>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) packed_dkv_kernel(const PackedArgs a) {
     using G = PackedGeo<DH>;
     constexpr int NW = 4, BN = 32 * KT * NW, NT = 64 * NW, STAGE = 2 * G::TILE + 512;
@@ -36,12 +36,18 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, W
     const int64_t all = (int64_t)tiles * group;                                 // (head, tile) steps; this block takes its part of them
     const int i0 = (int)(all * part / a.nsplit), i1 = (int)(all * (part + 1) / a.nsplit);
 
-    bf16x8_t kf[KT][G::KS], vf[KT][G::KS];
+    PackedLane<DH> at;
+    at.init(lane);
+    char* vt_ = smem + 2 * STAGE + wave * KT * 32 * G::PITCH;                   // VLDS: this wave's V rows, laid out like a staged tile
+    bf16x8_t kf[KT][G::KS], vf[VLDS ? 1 : KT][G::KS];
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
         const int64_t krow = s.start + kj + 32 * kt;
         packed_row_frags<DH>(kf[kt], a.k + krow * a.k_row + kvh * a.k_head, kj + 32 * kt < s.len, a.dim);
-        packed_row_frags<DH>(vf[kt], a.v + krow * a.v_row + kvh * a.v_head, kj + 32 * kt < s.len, a.dim);
+        packed_row_frags<DH>(vf[VLDS ? 0 : kt], a.v + krow * a.v_row + kvh * a.v_head, kj + 32 * kt < s.len, a.dim);
+        if (VLDS)
+#pragma unroll
+            for (int ks = 0; ks < G::KS; ++ks) *reinterpret_cast<bf16x8_t*>(vt_ + kt * 32 * G::PITCH + (at.rows ^ (uint32_t)(ks * 32))) = vf[0][ks];
     }
     f32x16_t dk[KT][G::DT], dv[KT][G::DT];
 #pragma unroll
@@ -69,8 +75,6 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, W
             }
         }
     };
-    PackedLane<DH> at;
-    at.init(lane);
 
     // 32 query rows rbase .. of the staged tile
     auto rows32 = [&](const char* qt_, const char* gt_, const float* stats, int rbase) {
@@ -89,13 +93,14 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, W
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) {
                 sacc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qa, kf[kt][ks], sacc[kt], 0, 0, 0);
-                dp[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ga, vf[kt][ks], dp[kt], 0, 0, 0);
+                dp[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ga, VLDS ? at.row_frag(vt_ + kt * 32 * G::PITCH, ks) : vf[VLDS ? 0 : kt][ks], dp[kt], 0, 0, 0);
             }
         }
         if (rbase < w_first + 32 * KT - 1) {                                    // some of these rows do not see all of the wave's keys
 #pragma unroll
             for (int kt = 0; kt < KT; ++kt) {
-                const int lim = kj + 32 * kt - shift - rbase - 4 * h;           // rows below do not see this lane's key
+                int lim = kj + 32 * kt - shift - rbase - 4 * h;                 // rows below do not see this lane's key
+                asm volatile("" : "+v"(lim));
 #pragma unroll
                 for (int r = 0; r < 16; ++r) sacc[kt][r] = seq_crow(r) >= lim ? sacc[kt][r] : -INFINITY;
             }
@@ -217,8 +222,10 @@ extern "C" int64_t genie_packed_attention_bwd_ws_floats(int nseq, int rows_q, in
 
 template <int DH, int KT, int WPE>
 static int packed_dkv_dispatch(PackedArgs& a, void* stream) {
+    constexpr bool VLDS = KT > 1;
     a.nslots = a.rows_k / (128 * KT) + a.nseq + 1;
-    const int rc = packed_launch(packed_dkv_kernel<DH, KT, WPE>, a, (int64_t)a.nslots * a.hkv * a.nsplit, 256, 4 * PackedGeo<DH>::TILE + 1024, stream);
+    const int rc = packed_launch(packed_dkv_kernel<DH, KT, WPE, VLDS>, a, (int64_t)a.nslots * a.hkv * a.nsplit, 256,
+                                 4 * PackedGeo<DH>::TILE + 1024 + (VLDS ? 128 * KT * PackedGeo<DH>::PITCH : 0), stream);
     if (rc != GENIE_OK || a.nsplit == 1) return rc;
     return packed_launch(packed_dkv_sum_kernel, a, ((int64_t)a.rows_k * a.hkv * a.dim / 8 + 255) / 256, 256, 0, stream);
 }

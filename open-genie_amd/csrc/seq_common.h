@@ -70,11 +70,9 @@ __device__ __forceinline__ void seq_dma16(const void* base, int bytes_left, char
     const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, bytes_left, 0x00020000);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, LDS_PTR(lds), 16, voff, 0u, 0, 0);
 }
-// bytes a tile may read from its first row on, when `rows` rows remain
-__device__ __forceinline__ int seq_bytes_left(long long rows, long long stride_bytes, int dim) {
-    if (rows <= 0) return 0;
-    const long long b = (rows - 1) * stride_bytes + dim * 2;
-    return (int)(b < 0x3fff0000ll ? b : 0x3fff0000ll);
+// bytes a tile of at most 64 rows may read from its first row on, when `rows` rows remain (row strides are under 2^22 bytes: 32 bits hold it)
+__device__ __forceinline__ int seq_bytes_left(int rows, int64_t stride_bytes, int dim) {
+    return rows <= 0 ? 0 : (min(rows, 64) - 1) * (int)stride_bytes + dim * 2;
 }
 
 // ds_read_b64_tr_b16: in each group of 16 lanes, lane i names 4 consecutive 16-bit values of row i / 4 (columns 4 (i % 4) ...) and receives column i of the
