@@ -16,14 +16,22 @@
 // maximum as it stands, and only a lane whose partial row sum passes 2^8 (inf and NaN too) has the tile redone with its exact maximum -- no
 // per-tile maximum tree in the steady state.  The first tile always takes its maximum, and every row that sees any key sees key 0.
 // ------------------------------------------------------------------------------------------------------------------------------
+#ifndef FWD_WPE
+#define FWD_WPE 3
+#endif
+#ifdef FWD_DMA
+#define FwdTiles PackedDma
+#else
+#define FwdTiles PackedTiles
+#endif
 template <int DH, int NW>
-__global__ void __launch_bounds__(64 * NW, DH <= 64 ? 3 : 2) packed_fwd_kernel(const PackedArgs a) {
+__global__ void __launch_bounds__(64 * NW, DH <= 64 ? FWD_WPE : 2) packed_fwd_kernel(const PackedArgs a) {
     using G = PackedGeo<DH>;
     constexpr int BM = 32 * NW, NT = 64 * NW;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const PackedBlock blk = packed_block(a, a.hq);
-    const SeqSlot s = seq_find<BM>(a.cu_q, a.nseq, a.rows_q, blk.slot);
+    const SeqSlot s = seq_find_longest<BM, false>(a.cu_q, a.nseq, a.rows_q, blk.slot, a.nslots);
     if (s.tile < 0 || s.tile * BM >= s.len) return;
     if (s.seq == a.nseq) {
         packed_zero_rows<BM, NT>(a.out, a.hq, a.dim, s, blk.head);
@@ -46,11 +54,12 @@ __global__ void __launch_bounds__(64 * NW, DH <= 64 ? 3 : 2) packed_fwd_kernel(c
 
     const bf16_t* kp = a.k + (int64_t)kstart * a.k_row + blk.kvh * a.k_head;
     const bf16_t* vp = a.v + (int64_t)kstart * a.v_row + blk.kvh * a.v_head;
-    PackedStage<DH, NT> st;
-    st.init(tid, a.dim, a.k_row, a.v_row);
+    FwdTiles<DH, NW> st;
+    st.init(wave, lane, a.dim, a.k_row, a.v_row);
     const int64_t k_step = 64 * a.k_row, v_step = 64 * a.v_row;
     auto load = [&](int t) {                                                    // (called for t = 0, 1, 2 ..)
-        st.load(kp, seq_bytes_left(klen - t * 64, a.k_row * 2, a.dim), vp, seq_bytes_left(klen - t * 64, a.v_row * 2, a.dim));
+        char* to = smem + (t & 1) * 2 * G::TILE;
+        st.load(wave, kp, seq_bytes_left(klen - t * 64, a.k_row * 2, a.dim), to, vp, seq_bytes_left(klen - t * 64, a.v_row * 2, a.dim), to + G::TILE);
         kp += k_step;
         vp += v_step;
     };
@@ -61,7 +70,7 @@ __global__ void __launch_bounds__(64 * NW, DH <= 64 ? 3 : 2) packed_fwd_kernel(c
     for (int t = 0; t < ntile; ++t) {
         char* kt_ = smem + (t & 1) * 2 * G::TILE;
         char* vt_ = kt_ + G::TILE;
-        st.store(kt_, vt_);
+        st.land(kt_, vt_);
         __syncthreads();
         if (t + 1 < ntile) load(t + 1);
         const int k0 = t * 64;
@@ -72,11 +81,16 @@ __global__ void __launch_bounds__(64 * NW, DH <= 64 ? 3 : 2) packed_fwd_kernel(c
         float psum;
         for (;;) {
             f32x16_t sacc[2] = {packed_splat(0.f), packed_splat(0.f)};
+            bf16x8_t kf[2][G::KS];                                              // all of the tile's fragments requested before the first product
 #pragma unroll
             for (int ks = 0; ks < G::KS; ++ks)
 #pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
-                    sacc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at.row_frag(kt_ + kt * 32 * G::PITCH, ks), qf[ks], sacc[kt], 0, 0, 0);
+                for (int kt = 0; kt < 2; ++kt) kf[kt][ks] = at.row_frag(kt_ + kt * 32 * G::PITCH, ks);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int ks = 0; ks < G::KS; ++ks)
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) sacc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kt][ks], qf[ks], sacc[kt], 0, 0, 0);
             if (k0 + 64 > klen || k0 + 63 > q0 + shift) {                       // the tile crosses the last key or the diagonal of these rows
                 int lim = min(klen, qi + shift + 1) - k0 - 4 * h;
                 asm volatile("" : "+v"(lim));                                   // (the comparisons stay in this branch)
@@ -120,6 +134,26 @@ __global__ void __launch_bounds__(64 * NW, DH <= 64 ? 3 : 2) packed_fwd_kernel(c
             with_max = true;
         }
         l_run += psum;
+#ifdef FWD_ASM
+        if constexpr (G::DT % 2 == 0) {
+            const uint32_t vb = attn_lds_offset(vt_);
+#pragma unroll
+            for (int dd = 0; dd < G::DT; dd += 2) {
+                const uint32_t a0 = vb + (at.tr0 ^ (dd * 64)), a1 = vb + (at.tr1 ^ (dd * 64)), a2 = vb + (at.tr0 ^ (dd * 64 + 64)), a3 = vb + (at.tr1 ^ (dd * 64 + 64));
+                bf16x8_t f[4];
+                seq_tr16x4<0, 16 * G::PITCH>(f, a0, a1, a2, a3);
+                oacc[dd] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[0], pf[0], oacc[dd], 0, 0, 0);
+                oacc[dd + 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[1], pf[0], oacc[dd + 1], 0, 0, 0);
+                oacc[dd] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[2], pf[1], oacc[dd], 0, 0, 0);
+                oacc[dd + 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[3], pf[1], oacc[dd + 1], 0, 0, 0);
+                seq_tr16x4<32 * G::PITCH, 48 * G::PITCH>(f, a0, a1, a2, a3);
+                oacc[dd] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[0], pf[2], oacc[dd], 0, 0, 0);
+                oacc[dd + 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[1], pf[2], oacc[dd + 1], 0, 0, 0);
+                oacc[dd] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[2], pf[3], oacc[dd], 0, 0, 0);
+                oacc[dd + 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[3], pf[3], oacc[dd + 1], 0, 0, 0);
+            }
+        } else
+#endif
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
@@ -147,7 +181,7 @@ __global__ void __launch_bounds__(64 * NW, DH <= 64 ? 3 : 2) packed_dq_kernel(co
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const PackedBlock blk = packed_block(a, a.hq);
-    const SeqSlot s = seq_find<BM>(a.cu_q, a.nseq, a.rows_q, blk.slot);
+    const SeqSlot s = seq_find_longest<BM, false>(a.cu_q, a.nseq, a.rows_q, blk.slot, a.nslots);
     if (s.tile < 0 || s.tile * BM >= s.len) return;
     if (s.seq == a.nseq) {
         packed_zero_rows<BM, NT>(a.dq, a.hq, a.dim, s, blk.head);
@@ -184,11 +218,12 @@ __global__ void __launch_bounds__(64 * NW, DH <= 64 ? 3 : 2) packed_dq_kernel(co
     const float c2 = a.scale * 1.4426950408889634f;
     const bf16_t* kp = a.k + (int64_t)kstart * a.k_row + blk.kvh * a.k_head;
     const bf16_t* vp = a.v + (int64_t)kstart * a.v_row + blk.kvh * a.v_head;
-    PackedStage<DH, NT> st;
-    st.init(tid, a.dim, a.k_row, a.v_row);
+    PackedTiles<DH, NW> st;
+    st.init(wave, lane, a.dim, a.k_row, a.v_row);
     const int64_t k_step = 64 * a.k_row, v_step = 64 * a.v_row;
     auto load = [&](int t) {                                                    // (called for t = 0, 1, 2 ..)
-        st.load(kp, seq_bytes_left(klen - t * 64, a.k_row * 2, a.dim), vp, seq_bytes_left(klen - t * 64, a.v_row * 2, a.dim));
+        char* to = smem + (t & 1) * 2 * G::TILE;
+        st.load(wave, kp, seq_bytes_left(klen - t * 64, a.k_row * 2, a.dim), to, vp, seq_bytes_left(klen - t * 64, a.v_row * 2, a.dim), to + G::TILE);
         kp += k_step;
         vp += v_step;
     };
@@ -199,7 +234,7 @@ __global__ void __launch_bounds__(64 * NW, DH <= 64 ? 3 : 2) packed_dq_kernel(co
     for (int t = 0; t < ntile; ++t) {
         char* kt_ = smem + (t & 1) * 2 * G::TILE;
         char* vt_ = kt_ + G::TILE;
-        st.store(kt_, vt_);
+        st.land(kt_, vt_);
         __syncthreads();
         if (t + 1 < ntile) load(t + 1);
         const int k0 = t * 64;

@@ -18,8 +18,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, W
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int kvh = (int)blockIdx.x % a.hkv, part = (int)blockIdx.x / a.hkv % a.nsplit, slot = (int)blockIdx.x / a.hkv / a.nsplit, group = a.hq / a.hkv;
-    // (slots ascending: the first keys of a sequence are seen by most rows)
-    const SeqSlot s = seq_find<BN>(a.cu_k, a.nseq, a.rows_k, slot);
+    const SeqSlot s = seq_find_longest<BN, true>(a.cu_k, a.nseq, a.rows_k, slot, a.nslots);
     if (s.tile < 0 || s.tile * BN >= s.len) return;
     if (s.seq == a.nseq) {
         if (a.nsplit > 1) return;                                               // (the reduction writes those rows)
@@ -136,12 +135,12 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, W
 
     if (i0 < i1) load(i0);
     for (int i = i0; i < i1; ++i) {
-        const char* qt_ = smem + (i & 1) * STAGE;
-        const char* gt_ = qt_ + G::TILE;
-        float* stats = reinterpret_cast<float*>(smem + (i & 1) * STAGE + 2 * G::TILE);
+        char* qt_ = smem + (i & 1) * STAGE;
+        char* gt_ = qt_ + G::TILE;
+        float* stats = reinterpret_cast<float*>(gt_ + G::TILE);
         if (tid < 128) stats[tid] = stat;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                        // this wave's slabs of tile i have landed ...
-        __syncthreads();                                                        // ... and everybody's
+        st.land(qt_, gt_);
+        __syncthreads();
         if (i + 1 < i1) load(i + 1);
         const int r0 = first + (i % tiles) * 64;
         if (r0 + 63 < w_first) continue;                                        // (wave-uniform) no row of these 64 sees this wave's keys
@@ -207,10 +206,13 @@ __global__ void __launch_bounds__(256) packed_dkv_sum_kernel(const PackedArgs a)
 #ifndef PACKED_DKV_BLOCKS
 #define PACKED_DKV_BLOCKS 1024
 #endif
+#ifndef PACKED_DKV_BLOCKS_WIDE
+#define PACKED_DKV_BLOCKS_WIDE 512
+#endif
 // parts a tile's (head, row tile) steps are cut into: as many as bring the launch to about PACKED_DKV_BLOCKS blocks, at most 8 and no more than there can be steps
 static int packed_dkv_splits(int nseq, int rows_q, int rows_k, int hq, int hkv, int dim) {
     const int64_t blocks = (int64_t)(rows_k / (dim > 64 ? 256 : 128) + (nseq < rows_k ? nseq : rows_k)) * hkv, steps = (int64_t)(rows_q / 64 + 1) * (hq / hkv);
-    int64_t n = blocks > 0 ? (PACKED_DKV_BLOCKS + blocks / 2) / blocks : 1;
+    int64_t n = blocks > 0 ? ((dim > 64 ? PACKED_DKV_BLOCKS_WIDE : PACKED_DKV_BLOCKS) + blocks / 2) / blocks : 1;
     n = n < steps ? n : steps;
     return (int)(n < 1 ? 1 : n > 8 ? 8 : n);
 }

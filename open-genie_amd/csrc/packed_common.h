@@ -54,32 +54,34 @@ struct PackedLane {
     }
 };
 
-// A pair of 64-row tiles (K and V, or Q and dO) on its way from memory to LDS.
-template <int DH, int NT>
-struct PackedStage {
+// A pair of 64-row tiles (K and V, or Q and dO) on its way from memory to LDS, two ways with one interface: load() asks for tile t + 1 while tile t is worked on,
+// land() ends the trip in front of the barrier that publishes it.
+// Through registers: head widths up to 64, where they are free (8 or 16 of them) and an iteration is short.
+template <int DH, int NW>
+struct PackedRegs {
     using G = PackedGeo<DH>;
-    static constexpr int PIECES = 64 * G::CPR / NT;
+    static constexpr int NT = 64 * NW, PIECES = 64 * G::CPR / NT;
     static_assert(64 * G::CPR % NT == 0, "every thread stages the same number of pieces");
     uint32_t va[PIECES], vb[PIECES], lds[PIECES];
     u32x4_t ra[PIECES], rb[PIECES];
-    __device__ __forceinline__ void init(int tid, int dim, int64_t stride_a, int64_t stride_b) {
+    __device__ __forceinline__ void init(int wave, int lane, int dim, int64_t stride_a, int64_t stride_b) {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-            const int idx = tid + i * NT, row = idx / G::CPR, c = idx % G::CPR;
+            const int idx = wave * 64 + lane + i * NT, row = idx / G::CPR, c = idx % G::CPR;
             const bool has = c * 8 < dim;
             va[i] = has ? (uint32_t)(row * stride_a * 2) + c * 16 : SEQ_OOB;
             vb[i] = has ? (uint32_t)(row * stride_b * 2) + c * 16 : SEQ_OOB;
             lds[i] = packed_at<DH>(row, c);
         }
     }
-    __device__ __forceinline__ void load(const bf16_t* a, int left_a, const bf16_t* b, int left_b) {
+    __device__ __forceinline__ void load(int, const bf16_t* a, int left_a, char*, const bf16_t* b, int left_b, char*) {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
             ra[i] = seq_load16(a, left_a, va[i]);
             rb[i] = seq_load16(b, left_b, vb[i]);
         }
     }
-    __device__ __forceinline__ void store(char* ta, char* tb) {
+    __device__ __forceinline__ void land(char* ta, char* tb) const {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
             *reinterpret_cast<u32x4_t*>(ta + lds[i]) = ra[i];
@@ -87,9 +89,10 @@ struct PackedStage {
         }
     }
 };
-
-// The same pair of tiles straight into LDS (buffer_load ... lds, 16 B per lane, no registers): a wave fills 1-KiB slabs of consecutive LDS, lane l's slot of
-// row l / SW gets the chunk that the swizzle (its own inverse) puts there; slots of chunks behind the head's width get zeros.
+// Wider heads: straight into LDS (buffer_load ... lds, 16 B per lane, no registers): a wave fills 1-KiB slabs of consecutive LDS,
+// lane l's slot of row l / SW gets the chunk that the swizzle (its own inverse) puts there; slots of chunks behind the head's width get zeros.
+// The compiler waits for all outstanding loads at the first transposing read of an iteration: by then the first product and the exponentials have passed,
+// which is longer than a tile takes from L2.
 template <int DH, int NW>
 struct PackedDma {
     using G = PackedGeo<DH>;
@@ -110,15 +113,18 @@ struct PackedDma {
             seq_dma16(b, left_b, tb + (wave * SLABS + i) * 1024, has ? row * pb + c * 16 : SEQ_OOB);
         }
     }
+    __device__ __forceinline__ void land(char*, char*) const { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }      // this wave's slabs; the barrier does the rest
 };
+template <int DH, int NW>
+using PackedTiles = std::conditional_t<(DH > 64), PackedDma<DH, NW>, PackedRegs<DH, NW>>;
 
-// (slot, head) of a block.  Slots in descending order: the tiles with the most keys start first.  Heads fastest, key heads before the query heads that
-// share them: consecutive blocks go round-robin over the 8 XCDs, so with 8, 4, 2 or 1 key heads an XCD's L2 sees one key head only.
+// (slot, head) of a block.  Heads fastest, key heads before the query heads that share them: consecutive blocks go round-robin over the 8 XCDs, so with 8, 4, 2 or 1
+// key heads an XCD's L2 sees one key head only.
 struct PackedBlock { int slot, head, kvh; };
 __device__ __forceinline__ PackedBlock packed_block(const PackedArgs& a, int nh) {
     PackedBlock b;
     const int id = (int)blockIdx.x, hi = id % nh;
-    b.slot = a.nslots - 1 - id / nh;
+    b.slot = id / nh;
     b.kvh = hi % a.hkv;
     b.head = b.kvh * (nh / a.hkv) + hi / a.hkv;
     return b;

@@ -35,24 +35,44 @@ __device__ __forceinline__ SeqSlot seq_find(const int32_t* cu, int nseq, int row
     return r;
 }
 
-// The same closed form with TILE a launch argument (the decay kernels' segment length).
-__device__ __forceinline__ SeqSlot seq_find_n(const int32_t* cu, int nseq, int rows, int tile_rows, int slot) {
+// The same list in descending order of the rows of its sequence behind (or, FIRST, in front of) a tile, which is what a causal tile costs: the longest blocks start
+// first, over all sequences.  Up to 63 sequences a lane holds one sequence's tile count n; C(u) = sum of max(0, n - u) tiles have u tiles or more on that side.
+// The lanes try 63 values of u at a time (one level up to 63 tiles, two up to 3969, ..), a ballot finds the u of rank `slot`, another its sequence.  More
+// sequences: the order of the slots above, from the end (FIRST: from the start).
+template <int TILE, bool FIRST>
+__device__ __forceinline__ SeqSlot seq_find_longest(const int32_t* cu, int nseq, int rows, int slot, int nslots) {
+    if (nseq > 63) return seq_find<TILE>(cu, nseq, rows, FIRST ? slot : nslots - 1 - slot);
     const int lane = threadIdx.x & 63;
-    int lo = 0, n = nseq + 1;
-    while (n > 1) {
-        const int step = (n + 63) >> 6;
-        const int i = lane * step;
-        const bool ok = i < n && seq_cu(cu, lo + i, rows) / tile_rows + lo + i <= slot;
-        const int cnt = max(1, (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(ok)));
-        lo += (cnt - 1) * step;
-        n = min(step, n - (cnt - 1) * step);
-    }
+    const int start = seq_cu(cu, min(lane, nseq), rows), next = seq_cu(cu, min(lane + 1, nseq), rows);
+    const int n = (max(0, next - start) + TILE - 1) / TILE;
     SeqSlot r;
-    r.seq = __builtin_amdgcn_readfirstlane(lo);
-    r.start = __builtin_amdgcn_readfirstlane(seq_cu(cu, r.seq, rows));
-    const int end = r.seq < nseq ? __builtin_amdgcn_readfirstlane(seq_cu(cu, r.seq + 1, rows)) : rows;
-    r.len = max(0, end - r.start);
-    r.tile = slot - (r.start / tile_rows + r.seq);
+    int lo = 0, range = rows / TILE + 2, above = 0;                             // C(lo) > slot; above: C(lo + 1) in the end
+    do {
+        const int step = (range + 62) / 63, u = lo + lane * step;
+        int c = 0;
+        for (int q = 0; q < nseq; ++q) c += max(0, __builtin_amdgcn_readlane(n, q) - u);
+        if (lo == 0) {
+            const int total = __builtin_amdgcn_readfirstlane(c);
+            if (slot >= total) {                                                // the rows behind the last sequence
+                r.seq = nseq;
+                r.start = __builtin_amdgcn_readlane(start, nseq);
+                r.len = rows - r.start;
+                r.tile = slot - total;
+                return r;
+            }
+        }
+        const int cnt = max(1, (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(c > slot)));      // C descends: the first cnt lanes (lane 63 is past the end)
+        lo += (cnt - 1) * step;
+        above = __builtin_amdgcn_readlane(c, min(cnt, 63));
+        range = step;
+    } while (range > 1);
+    // tiles with exactly lo behind them: one of every sequence with n > lo, after the C(lo + 1) longer ones
+    uint64_t who = __builtin_amdgcn_ballot_w64(n > lo);
+    for (int k = slot - above; k > 0; --k) who &= who - 1;
+    r.seq = who ? (int)__builtin_ctzll(who) : 0;
+    r.start = __builtin_amdgcn_readlane(start, r.seq);
+    r.len = max(0, __builtin_amdgcn_readlane(next, r.seq) - r.start);
+    r.tile = FIRST ? (r.len + TILE - 1) / TILE - 1 - lo : lo;
     return r;
 }
 
@@ -79,6 +99,24 @@ __device__ __forceinline__ int seq_bytes_left(int rows, int64_t stride_bytes, in
 // four rows.  The builtin: the compiler tracks the wait itself (tiles here are staged through registers, no LDS-DMA is in flight beside it).
 typedef __attribute__((address_space(3))) bf16x4_t seq_lds_b16x4;
 __device__ __forceinline__ bf16x4_t seq_tr16(const char* p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((seq_lds_b16x4*)p); }
+
+// Four fragments by eight such reads and their wait in ONE asm block: for loops with an LDS-DMA in flight, where the compiler would wait for the DMA in front of the
+// builtin.  a0, a1: LDS byte addresses of fragments 0 and 1 (lower and upper half each); OFF1: byte distance of fragments 2 and 3.
+template <int OFF0, int OFF1>
+__device__ __forceinline__ void seq_tr16x4(bf16x8_t (&f)[4], uint32_t a0lo, uint32_t a0hi, uint32_t a1lo, uint32_t a1hi) {
+    bf16x4_t r0, r1, r2, r3, r4, r5, r6, r7;
+    asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %9 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %2, %10 offset:%12\n\tds_read_b64_tr_b16 %3, %11 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %4, %8 offset:%13\n\tds_read_b64_tr_b16 %5, %9 offset:%13\n\t"
+                 "ds_read_b64_tr_b16 %6, %10 offset:%13\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(r0), "=&v"(r1), "=&v"(r2), "=&v"(r3), "=&v"(r4), "=&v"(r5), "=&v"(r6), "=&v"(r7)
+                 : "v"(a0lo), "v"(a0hi), "v"(a1lo), "v"(a1hi), "n"(OFF0), "n"(OFF1)
+                 : "memory");
+    f[0] = __builtin_shufflevector(r0, r1, 0, 1, 2, 3, 4, 5, 6, 7);
+    f[1] = __builtin_shufflevector(r2, r3, 0, 1, 2, 3, 4, 5, 6, 7);
+    f[2] = __builtin_shufflevector(r4, r5, 0, 1, 2, 3, 4, 5, 6, 7);
+    f[3] = __builtin_shufflevector(r6, r7, 0, 1, 2, 3, 4, 5, 6, 7);
+}
 
 __device__ __forceinline__ bf16x8_t seq_pack8(const float a0, const float a1, const float a2, const float a3, const float a4, const float a5, const float a6,
                                               const float a7) {
