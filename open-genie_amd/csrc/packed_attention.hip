@@ -9,72 +9,88 @@
 // layout of the second product -- the transposed V / K / dO / Q fragments are read in that order by ds_read_b64_tr_b16, nothing is exchanged.
 // The sequences' lengths live on the device only: seq_common.h maps slots to (sequence, tile).
 #include "packed_common.h"
+#ifndef DQ_UNROLL
+#define DQ_UNROLL 2
+#endif
+
+// ------------------------------------------------------------------------------------------------------------------------------
+// A block of the forward and dQ kernels: 128 query rows, 4 row groups of 32 x NG key groups of waves.  With two key groups alternate 64-key tiles pass through LDS two
+// per step and the groups join their sums at the end: a causal tile's time is a chain of (its keys / 64 NG) dependent steps, and with few sequences the
+// longest chain, not the chip, is what a launch waits for.
+// ------------------------------------------------------------------------------------------------------------------------------
+struct PackedRows {
+    SeqSlot s;
+    PackedBlock blk;
+    int kstart, klen, shift, q0, qi, nstep, w_end, grp, rw;
+};
+template <int NG>
+__device__ __forceinline__ bool packed_rows(const PackedArgs& a, PackedRows& r, bf16_t* out) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    r.grp = wave >> 2;
+    r.rw = wave & 3;
+    r.blk = packed_block(a, a.hq);
+    r.s = seq_find_longest<128, false>(a.cu_q, a.nseq, a.rows_q, r.blk.slot, a.nslots);
+    if (r.s.tile < 0 || r.s.tile * 128 >= r.s.len) return false;
+    if (r.s.seq == a.nseq) {
+        packed_zero_rows<128, 256 * NG>(out, a.hq, a.dim, r.s, r.blk.head);
+        return false;
+    }
+    r.kstart = seq_cu(a.cu_k, r.s.seq, a.rows_k);
+    r.klen = max(0, seq_cu(a.cu_k, r.s.seq + 1, a.rows_k) - r.kstart);
+    r.shift = r.klen - r.s.len;                                                 // query i sees keys 0 .. i + shift
+    r.q0 = r.s.tile * 128 + r.rw * 32;
+    r.qi = r.q0 + (lane & 31);
+    const int k_end = min(r.klen, min(r.s.tile * 128 + 128, r.s.len) + r.shift);     // of the block (<= 0: nothing to see)
+    r.w_end = min(r.klen, min(r.q0 + 32, r.s.len) + r.shift);                   // of this wave
+    r.nstep = (max(k_end, 0) + 64 * NG - 1) / (64 * NG);
+    return true;
+}
 
 // ------------------------------------------------------------------------------------------------------------------------------
 // Forward.  Online softmax in the exp2 domain with fp32 maximum, sum and accumulator; P is rounded to bf16 (at most 2^-8 of a weight, the precision
 // of V itself) because the second product runs on the matrix cores.  The running maximum is "sum-triggered": a tile is exponentiated against the
 // maximum as it stands, and only a lane whose partial row sum passes 2^8 (inf and NaN too) has the tile redone with its exact maximum -- no
-// per-tile maximum tree in the steady state.  The first tile always takes its maximum, and every row that sees any key sees key 0.
+// per-tile maximum tree in the steady state.  A wave's first tile always takes its maximum; a row that sees nothing of it (the second key group's first tile may lie
+// behind it) sees nothing after it either.
 // ------------------------------------------------------------------------------------------------------------------------------
-#ifndef FWD_WPE
-#define FWD_WPE 3
-#endif
-#ifdef FWD_DMA
-#define FwdTiles PackedDma
-#else
-#define FwdTiles PackedTiles
-#endif
-template <int DH, int NW>
-__global__ void __launch_bounds__(64 * NW, DH <= 64 ? FWD_WPE : 2) packed_fwd_kernel(const PackedArgs a) {
+template <int DH, int NG, int WPE>
+__global__ void __launch_bounds__(256 * NG, WPE) packed_fwd_kernel(const PackedArgs a) {
     using G = PackedGeo<DH>;
-    constexpr int BM = 32 * NW, NT = 64 * NW;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-    const PackedBlock blk = packed_block(a, a.hq);
-    const SeqSlot s = seq_find_longest<BM, false>(a.cu_q, a.nseq, a.rows_q, blk.slot, a.nslots);
-    if (s.tile < 0 || s.tile * BM >= s.len) return;
-    if (s.seq == a.nseq) {
-        packed_zero_rows<BM, NT>(a.out, a.hq, a.dim, s, blk.head);
-        return;
-    }
-    const int kstart = seq_cu(a.cu_k, s.seq, a.rows_k), klen = max(0, seq_cu(a.cu_k, s.seq + 1, a.rows_k) - kstart);
-    const int shift = klen - s.len;                                             // query i sees keys 0 .. i + shift
-    const int q0 = s.tile * BM + wave * 32, qi = q0 + (lane & 31);
-    const int k_end = min(klen, min(s.tile * BM + BM, s.len) + shift);          // of the block (<= 0: nothing to see)
-    const int w_end = min(klen, min(q0 + 32, s.len) + shift);                   // of this wave
-    const int ntile = (max(k_end, 0) + 63) >> 6;
-
+    PackedRows r;
+    if (!packed_rows<NG>(a, r, a.out)) return;
     bf16x8_t qf[G::KS];
-    packed_row_frags<DH>(qf, a.q + (int64_t)(s.start + qi) * a.q_row + blk.head * a.q_head, qi < s.len, a.dim);
+    packed_row_frags<DH>(qf, a.q + (int64_t)(r.s.start + r.qi) * a.q_row + r.blk.head * a.q_head, r.qi < r.s.len, a.dim);
     f32x16_t oacc[G::DT];
 #pragma unroll
     for (int d = 0; d < G::DT; ++d) oacc[d] = packed_splat(0.f);
     float m_run = -INFINITY, mc = 0.f, l_run = 0.f;                             // mc: m_run in the exp2 domain, 0 while there is none; l_run: this lane's half
     const float c2 = a.scale * 1.4426950408889634f;
 
-    const bf16_t* kp = a.k + (int64_t)kstart * a.k_row + blk.kvh * a.k_head;
-    const bf16_t* vp = a.v + (int64_t)kstart * a.v_row + blk.kvh * a.v_head;
-    FwdTiles<DH, NW> st;
+    const bf16_t* kp = a.k + (int64_t)r.kstart * a.k_row + r.blk.kvh * a.k_head;
+    const bf16_t* vp = a.v + (int64_t)r.kstart * a.v_row + r.blk.kvh * a.v_head;
+    const int64_t k_step = 64 * NG * a.k_row, v_step = 64 * NG * a.v_row;
+    PackedDma<DH, 4 * NG, NG, (DH <= 64)> st;
     st.init(wave, lane, a.dim, a.k_row, a.v_row);
-    const int64_t k_step = 64 * a.k_row, v_step = 64 * a.v_row;
     auto load = [&](int t) {                                                    // (called for t = 0, 1, 2 ..)
-        char* to = smem + (t & 1) * 2 * G::TILE;
-        st.load(wave, kp, seq_bytes_left(klen - t * 64, a.k_row * 2, a.dim), to, vp, seq_bytes_left(klen - t * 64, a.v_row * 2, a.dim), to + G::TILE);
+        char* to = smem + (t & 1) * 2 * NG * G::TILE;
+        st.load(wave, kp, seq_bytes_left(r.klen - t * 64 * NG, a.k_row * 2, a.dim), to, vp, seq_bytes_left(r.klen - t * 64 * NG, a.v_row * 2, a.dim), to + NG * G::TILE);
         kp += k_step;
         vp += v_step;
     };
     PackedLane<DH> at;
     at.init(lane);
 
-    if (ntile > 0) load(0);
-    for (int t = 0; t < ntile; ++t) {
-        char* kt_ = smem + (t & 1) * 2 * G::TILE;
-        char* vt_ = kt_ + G::TILE;
-        st.land(kt_, vt_);
+    if (r.nstep > 0) load(0);
+    for (int t = 0; t < r.nstep; ++t) {
+        const char* kt_ = smem + (t & 1) * 2 * NG * G::TILE + r.grp * G::TILE;
+        const char* vt_ = kt_ + NG * G::TILE;
+        st.land();
         __syncthreads();
-        if (t + 1 < ntile) load(t + 1);
-        const int k0 = t * 64;
-        if (k0 >= w_end) continue;                                              // (wave-uniform) nothing of this tile is visible to these 32 rows
+        if (t + 1 < r.nstep) load(t + 1);
+        const int k0 = (t * NG + r.grp) * 64;
+        if (k0 >= r.w_end) continue;                                            // (wave-uniform) nothing of this tile is visible to these 32 rows
         at.forget();
         bool with_max = t == 0;
         bf16x8_t pf[4];
@@ -91,20 +107,20 @@ __global__ void __launch_bounds__(64 * NW, DH <= 64 ? FWD_WPE : 2) packed_fwd_ke
             for (int ks = 0; ks < G::KS; ++ks)
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt) sacc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kt][ks], qf[ks], sacc[kt], 0, 0, 0);
-            if (k0 + 64 > klen || k0 + 63 > q0 + shift) {                       // the tile crosses the last key or the diagonal of these rows
-                int lim = min(klen, qi + shift + 1) - k0 - 4 * h;
+            if (k0 + 64 > r.klen || k0 + 63 > r.q0 + r.shift) {                 // the tile crosses the last key or the diagonal of these rows
+                int lim = min(r.klen, r.qi + r.shift + 1) - k0 - 4 * h;
                 asm volatile("" : "+v"(lim));                                   // (the comparisons stay in this branch)
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) sacc[kt][r] = kt * 32 + seq_crow(r) < lim ? sacc[kt][r] : -INFINITY;
+                    for (int e = 0; e < 16; ++e) sacc[kt][e] = kt * 32 + seq_crow(e) < lim ? sacc[kt][e] : -INFINITY;
             }
             if (with_max) {
                 float tm = -INFINITY;
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) tm = fmaxf(tm, sacc[kt][r]);
+                    for (int e = 0; e < 16; ++e) tm = fmaxf(tm, sacc[kt][e]);
                 const float m_new = fmaxf(m_run, seq_xmax32(tm));
                 const float mc_new = m_new == -INFINITY ? 0.f : m_new * c2;
                 const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mc - mc_new);
@@ -112,7 +128,7 @@ __global__ void __launch_bounds__(64 * NW, DH <= 64 ? FWD_WPE : 2) packed_fwd_ke
 #pragma unroll
                 for (int d = 0; d < G::DT; ++d)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) oacc[d][r] *= alpha;
+                    for (int e = 0; e < 16; ++e) oacc[d][e] *= alpha;
                 m_run = m_new;
                 mc = mc_new;
             }
@@ -134,39 +150,46 @@ __global__ void __launch_bounds__(64 * NW, DH <= 64 ? FWD_WPE : 2) packed_fwd_ke
             with_max = true;
         }
         l_run += psum;
-#ifdef FWD_ASM
-        if constexpr (G::DT % 2 == 0) {
-            const uint32_t vb = attn_lds_offset(vt_);
-#pragma unroll
-            for (int dd = 0; dd < G::DT; dd += 2) {
-                const uint32_t a0 = vb + (at.tr0 ^ (dd * 64)), a1 = vb + (at.tr1 ^ (dd * 64)), a2 = vb + (at.tr0 ^ (dd * 64 + 64)), a3 = vb + (at.tr1 ^ (dd * 64 + 64));
-                bf16x8_t f[4];
-                seq_tr16x4<0, 16 * G::PITCH>(f, a0, a1, a2, a3);
-                oacc[dd] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[0], pf[0], oacc[dd], 0, 0, 0);
-                oacc[dd + 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[1], pf[0], oacc[dd + 1], 0, 0, 0);
-                oacc[dd] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[2], pf[1], oacc[dd], 0, 0, 0);
-                oacc[dd + 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[3], pf[1], oacc[dd + 1], 0, 0, 0);
-                seq_tr16x4<32 * G::PITCH, 48 * G::PITCH>(f, a0, a1, a2, a3);
-                oacc[dd] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[0], pf[2], oacc[dd], 0, 0, 0);
-                oacc[dd + 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[1], pf[2], oacc[dd + 1], 0, 0, 0);
-                oacc[dd] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[2], pf[3], oacc[dd], 0, 0, 0);
-                oacc[dd + 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[3], pf[3], oacc[dd + 1], 0, 0, 0);
-            }
-        } else
-#endif
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
             for (int d = 0; d < G::DT; ++d)
                 oacc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at.tr_frag(vt_ + ks * 16 * G::PITCH, d), pf[ks], oacc[d], 0, 0, 0);
     }
-    const float l = seq_xsum32(l_run);
-    if (a.lse && h == 0 && qi < s.len)
-        a.lse[(int64_t)blk.head * a.rows_q + s.start + qi] = l == 0.f ? -INFINITY : mc * 0.6931471805599453f + __logf(l);
-    __syncthreads();                                                            // the staging tiles become the waves' output regions
-    if (q0 < s.len)
-        packed_write_rows<DH>(smem + wave * 32 * G::PITCH, oacc, l == 0.f ? 0.f : 1.f / l, a.out + ((int64_t)(s.start + q0) * a.hq + blk.head) * a.dim,
-                              (int64_t)a.hq * a.dim, min(32, s.len - q0), a.dim);
+    float l = 0.f;
+    if constexpr (NG == 1) {
+        l = seq_xsum32(l_run);
+    } else {
+        // the second key group's sums join the first's: through LDS, register by register (lane = the same row and columns in both)
+        __syncthreads();
+        float* xs = reinterpret_cast<float*>(smem) + r.rw * (G::DT * 16 + 2) * 64 + lane;
+        if (r.grp == 1) {
+            xs[0] = m_run == -INFINITY ? -INFINITY : mc;
+            xs[64] = l_run;
+#pragma unroll
+            for (int d = 0; d < G::DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) xs[(2 + d * 16 + e) * 64] = oacc[d][e];
+        }
+        __syncthreads();
+        if (r.grp == 0) {
+            const float m1 = xs[0], m0 = m_run == -INFINITY ? -INFINITY : mc, mx = fmaxf(m0, m1), l1 = xs[64];
+            // (a part without a maximum has nothing, or NaN: it goes in as it is)
+            const float f0 = m0 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m0 - mx), f1 = m1 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m1 - mx);
+            mc = mx == -INFINITY ? 0.f : mx;
+            l = seq_xsum32(l_run * f0 + l1 * f1);
+#pragma unroll
+            for (int d = 0; d < G::DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) oacc[d][e] = oacc[d][e] * f0 + xs[(2 + d * 16 + e) * 64] * f1;
+        }
+    }
+    if (r.grp == 0 && a.lse && h == 0 && r.qi < r.s.len)
+        a.lse[(int64_t)r.blk.head * a.rows_q + r.s.start + r.qi] = l == 0.f ? -INFINITY : mc * 0.6931471805599453f + __logf(l);
+    __syncthreads();                                                            // tiles and exchange area become the waves' output regions
+    if (r.grp == 0 && r.q0 < r.s.len)
+        packed_write_rows<DH>(smem + r.rw * 32 * G::PITCH, oacc, l == 0.f ? 0.f : 1.f / l, a.out + ((int64_t)(r.s.start + r.q0) * a.hq + r.blk.head) * a.dim,
+                              (int64_t)a.hq * a.dim, min(32, r.s.len - r.q0), a.dim);
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------
@@ -174,73 +197,61 @@ __global__ void __launch_bounds__(64 * NW, DH <= 64 ? FWD_WPE : 2) packed_fwd_ke
 // operand fragments, written out for the other kernel, and fed negated as the accumulator INPUT of dP^T = V dO^T, so that dS = P o (dP - delta) costs
 // no subtraction.  dS is rounded to bf16 for the last product, like P in the forward.
 // ------------------------------------------------------------------------------------------------------------------------------
-template <int DH, int NW>
-__global__ void __launch_bounds__(64 * NW, DH <= 64 ? 3 : 2) packed_dq_kernel(const PackedArgs a) {
+template <int DH, int NG, int WPE>
+__global__ void __launch_bounds__(256 * NG, WPE) packed_dq_kernel(const PackedArgs a) {
     using G = PackedGeo<DH>;
-    constexpr int BM = 32 * NW, NT = 64 * NW;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-    const PackedBlock blk = packed_block(a, a.hq);
-    const SeqSlot s = seq_find_longest<BM, false>(a.cu_q, a.nseq, a.rows_q, blk.slot, a.nslots);
-    if (s.tile < 0 || s.tile * BM >= s.len) return;
-    if (s.seq == a.nseq) {
-        packed_zero_rows<BM, NT>(a.dq, a.hq, a.dim, s, blk.head);
-        return;
-    }
-    const int kstart = seq_cu(a.cu_k, s.seq, a.rows_k), klen = max(0, seq_cu(a.cu_k, s.seq + 1, a.rows_k) - kstart);
-    const int shift = klen - s.len;
-    const int q0 = s.tile * BM + wave * 32, qi = q0 + (lane & 31);
-    const int k_end = min(klen, min(s.tile * BM + BM, s.len) + shift), w_end = min(klen, min(q0 + 32, s.len) + shift);
-    const int ntile = (max(k_end, 0) + 63) >> 6;
-
+    PackedRows r;
+    if (!packed_rows<NG>(a, r, a.dq)) return;
     bf16x8_t qf[G::KS], gf[G::KS];
-    const int64_t qrow = s.start + qi;
-    packed_row_frags<DH>(qf, a.q + qrow * a.q_row + blk.head * a.q_head, qi < s.len, a.dim);
-    packed_row_frags<DH>(gf, a.dout + qrow * a.g_row + blk.head * a.g_head, qi < s.len, a.dim);
+    const int64_t qrow = r.s.start + r.qi;
+    packed_row_frags<DH>(qf, a.q + qrow * a.q_row + r.blk.head * a.q_head, r.qi < r.s.len, a.dim);
+    packed_row_frags<DH>(gf, a.dout + qrow * a.g_row + r.blk.head * a.g_head, r.qi < r.s.len, a.dim);
     float delta = 0.f, lse2 = INFINITY;                                         // a row that sees nothing, or none at all: exp2(x - inf) = 0
     {
         bf16x8_t of[G::KS];
-        packed_row_frags<DH>(of, a.o + (qrow * a.hq + blk.head) * a.dim, qi < s.len, a.dim);
+        packed_row_frags<DH>(of, a.o + (qrow * a.hq + r.blk.head) * a.dim, r.qi < r.s.len, a.dim);
 #pragma unroll
         for (int ks = 0; ks < G::KS; ++ks)
 #pragma unroll
             for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(bf16_to_f32((bf16_t)gf[ks][e]), bf16_to_f32((bf16_t)of[ks][e]), delta);
         delta = seq_xsum32(delta);
-        if (qi < s.len) {
-            const float lse = a.lse[(int64_t)blk.head * a.rows_q + qrow];
+        if (r.qi < r.s.len) {
+            const float lse = a.lse[(int64_t)r.blk.head * a.rows_q + qrow];
             lse2 = lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f;
-            if (h == 0) a.delta[(int64_t)blk.head * a.rows_q + qrow] = delta;
+            if (h == 0 && r.grp == 0) a.delta[(int64_t)r.blk.head * a.rows_q + qrow] = delta;
         }
     }
     f32x16_t acc[G::DT];
 #pragma unroll
     for (int d = 0; d < G::DT; ++d) acc[d] = packed_splat(0.f);
     const float c2 = a.scale * 1.4426950408889634f;
-    const bf16_t* kp = a.k + (int64_t)kstart * a.k_row + blk.kvh * a.k_head;
-    const bf16_t* vp = a.v + (int64_t)kstart * a.v_row + blk.kvh * a.v_head;
-    PackedTiles<DH, NW> st;
+    const bf16_t* kp = a.k + (int64_t)r.kstart * a.k_row + r.blk.kvh * a.k_head;
+    const bf16_t* vp = a.v + (int64_t)r.kstart * a.v_row + r.blk.kvh * a.v_head;
+    const int64_t k_step = 64 * NG * a.k_row, v_step = 64 * NG * a.v_row;
+    PackedDma<DH, 4 * NG, NG, (DH <= 64)> st;
     st.init(wave, lane, a.dim, a.k_row, a.v_row);
-    const int64_t k_step = 64 * a.k_row, v_step = 64 * a.v_row;
     auto load = [&](int t) {                                                    // (called for t = 0, 1, 2 ..)
-        char* to = smem + (t & 1) * 2 * G::TILE;
-        st.load(wave, kp, seq_bytes_left(klen - t * 64, a.k_row * 2, a.dim), to, vp, seq_bytes_left(klen - t * 64, a.v_row * 2, a.dim), to + G::TILE);
+        char* to = smem + (t & 1) * 2 * NG * G::TILE;
+        st.load(wave, kp, seq_bytes_left(r.klen - t * 64 * NG, a.k_row * 2, a.dim), to, vp, seq_bytes_left(r.klen - t * 64 * NG, a.v_row * 2, a.dim), to + NG * G::TILE);
         kp += k_step;
         vp += v_step;
     };
     PackedLane<DH> at;
     at.init(lane);
 
-    if (ntile > 0) load(0);
-    for (int t = 0; t < ntile; ++t) {
-        char* kt_ = smem + (t & 1) * 2 * G::TILE;
-        char* vt_ = kt_ + G::TILE;
-        st.land(kt_, vt_);
+    if (r.nstep > 0) load(0);
+    for (int t = 0; t < r.nstep; ++t) {
+        const char* kt_ = smem + (t & 1) * 2 * NG * G::TILE + r.grp * G::TILE;
+        const char* vt_ = kt_ + NG * G::TILE;
+        st.land();
         __syncthreads();
-        if (t + 1 < ntile) load(t + 1);
-        const int k0 = t * 64;
-        if (k0 >= w_end) continue;
+        if (t + 1 < r.nstep) load(t + 1);
+        const int k0 = (t * NG + r.grp) * 64;
+        if (k0 >= r.w_end) continue;
         at.forget();
-#pragma unroll
+#pragma unroll DQ_UNROLL
         for (int kt = 0; kt < 2; ++kt) {
             f32x16_t sacc = packed_splat(0.f), dp = packed_splat(-delta);
 #pragma unroll
@@ -248,21 +259,18 @@ __global__ void __launch_bounds__(64 * NW, DH <= 64 ? 3 : 2) packed_dq_kernel(co
                 sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at.row_frag(kt_ + kt * 32 * G::PITCH, ks), qf[ks], sacc, 0, 0, 0);
                 dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at.row_frag(vt_ + kt * 32 * G::PITCH, ks), gf[ks], dp, 0, 0, 0);
             }
-            if (k0 + 64 > klen || k0 + 63 > q0 + shift) {
-                int lim = min(klen, qi + shift + 1) - k0 - 32 * kt - 4 * h;
+            if (k0 + 64 > r.klen || k0 + 63 > r.q0 + r.shift) {
+                int lim = min(r.klen, r.qi + r.shift + 1) - k0 - 32 * kt - 4 * h;
                 asm volatile("" : "+v"(lim));
 #pragma unroll
-                for (int r = 0; r < 16; ++r) sacc[r] = seq_crow(r) < lim ? sacc[r] : -INFINITY;
+                for (int e = 0; e < 16; ++e) sacc[e] = seq_crow(e) < lim ? sacc[e] : -INFINITY;
             }
             bf16x8_t ds[2];
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2) {
                 float x[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int r = 8 * s2 + e;
-                    x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[r], c2, -lse2)) * dp[r];
-                }
+                for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[8 * s2 + e], c2, -lse2)) * dp[8 * s2 + e];
                 ds[s2] = seq_pack8(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
             }
 #pragma unroll
@@ -272,10 +280,25 @@ __global__ void __launch_bounds__(64 * NW, DH <= 64 ? 3 : 2) packed_dq_kernel(co
                     acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at.tr_frag(kt_ + (kt * 2 + s2) * 16 * G::PITCH, d), ds[s2], acc[d], 0, 0, 0);
         }
     }
+    if constexpr (NG == 2) {
+        __syncthreads();
+        float* xs = reinterpret_cast<float*>(smem) + r.rw * G::DT * 16 * 64 + lane;
+        if (r.grp == 1)
+#pragma unroll
+            for (int d = 0; d < G::DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) xs[(d * 16 + e) * 64] = acc[d][e];
+        __syncthreads();
+        if (r.grp == 0)
+#pragma unroll
+            for (int d = 0; d < G::DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[d][e] += xs[(d * 16 + e) * 64];
+    }
     __syncthreads();
-    if (q0 < s.len)
-        packed_write_rows<DH>(smem + wave * 32 * G::PITCH, acc, a.scale, a.dq + ((int64_t)(s.start + q0) * a.hq + blk.head) * a.dim, (int64_t)a.hq * a.dim,
-                              min(32, s.len - q0), a.dim);
+    if (r.grp == 0 && r.q0 < r.s.len)
+        packed_write_rows<DH>(smem + r.rw * 32 * G::PITCH, acc, a.scale, a.dq + ((int64_t)(r.s.start + r.q0) * a.hq + r.blk.head) * a.dim, (int64_t)a.hq * a.dim,
+                              min(32, r.s.len - r.q0), a.dim);
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------
@@ -294,20 +317,27 @@ static int packed_check(const char* what, const PackedArgs& a) {
     return GENIE_OK;
 }
 
+#ifndef FWD_NG
+#define FWD_NG 2
+#define FWD_WPE 4
+#endif
+#ifndef DQ_NG
+#define DQ_NG 1
+#define DQ_WPE 3
+#endif
 template <int DH>
 static int packed_fwd_dispatch(PackedArgs& a, void* stream) {
-    constexpr int NW = 4;
-    a.nslots = a.rows_q / (32 * NW) + a.nseq + 1;
-    return packed_launch(packed_fwd_kernel<DH, NW>, a, (int64_t)a.nslots * a.hq, 64 * NW, 4 * PackedGeo<DH>::TILE, stream);
+    constexpr int NG = DH <= 64 ? FWD_NG : 1, WPE = DH <= 64 ? FWD_WPE : 2;
+    a.nslots = a.rows_q / 128 + a.nseq + 1;
+    return packed_launch(packed_fwd_kernel<DH, NG, WPE>, a, (int64_t)a.nslots * a.hq, 256 * NG, 4 * NG * PackedGeo<DH>::TILE, stream);
 }
 
 template <int DH>
 static int packed_bwd_dispatch(PackedArgs& a, void* stream) {
-    constexpr int NW = 4;
-    a.nslots = a.rows_q / (32 * NW) + a.nseq + 1;
-    const int rc = packed_launch(packed_dq_kernel<DH, NW>, a, (int64_t)a.nslots * a.hq, 64 * NW, 4 * PackedGeo<DH>::TILE, stream);
-    if (rc != GENIE_OK) return rc;
-    return packed_dkv_run(a, stream);
+    constexpr int NG = DH <= 64 ? DQ_NG : 1, WPE = DH <= 64 ? DQ_WPE : 2;
+    a.nslots = a.rows_q / 128 + a.nseq + 1;
+    const int rc = packed_launch(packed_dq_kernel<DH, NG, WPE>, a, (int64_t)a.nslots * a.hq, 256 * NG, 4 * NG * PackedGeo<DH>::TILE, stream);
+    return rc != GENIE_OK ? rc : packed_dkv_run(a, stream);
 }
 
 extern "C" int genie_packed_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int32_t* cu_q, const int32_t* cu_k, int nseq,

@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, W
         for (int d = 0; d < G::DT; ++d) dk[kt][d] = dv[kt][d] = packed_splat(0.f);
     const float c2 = a.scale * 1.4426950408889634f, inv_scale = 1.f / a.scale;
 
-    PackedDma<DH, NW> st;
+    PackedDma<DH, NW, 1, false> st;
     st.init(wave, lane, a.dim, a.q_row, a.g_row);
     float stat = 0.f;                                                           // threads 0..63: -lse / scale, 64..127: -delta of the tile's rows
     auto load = [&](int i) {
@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, W
         char* gt_ = qt_ + G::TILE;
         float* stats = reinterpret_cast<float*>(gt_ + G::TILE);
         if (tid < 128) stats[tid] = stat;
-        st.land(qt_, gt_);
+        st.land();
         __syncthreads();
         if (i + 1 < i1) load(i + 1);
         const int r0 = first + (i % tiles) * 64;

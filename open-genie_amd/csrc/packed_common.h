@@ -54,69 +54,39 @@ struct PackedLane {
     }
 };
 
-// A pair of 64-row tiles (K and V, or Q and dO) on its way from memory to LDS, two ways with one interface: load() asks for tile t + 1 while tile t is worked on,
-// land() ends the trip in front of the barrier that publishes it.
-// Through registers: head widths up to 64, where they are free (8 or 16 of them) and an iteration is short.
-template <int DH, int NW>
-struct PackedRegs {
-    using G = PackedGeo<DH>;
-    static constexpr int NT = 64 * NW, PIECES = 64 * G::CPR / NT;
-    static_assert(64 * G::CPR % NT == 0, "every thread stages the same number of pieces");
-    uint32_t va[PIECES], vb[PIECES], lds[PIECES];
-    u32x4_t ra[PIECES], rb[PIECES];
-    __device__ __forceinline__ void init(int wave, int lane, int dim, int64_t stride_a, int64_t stride_b) {
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            const int idx = wave * 64 + lane + i * NT, row = idx / G::CPR, c = idx % G::CPR;
-            const bool has = c * 8 < dim;
-            va[i] = has ? (uint32_t)(row * stride_a * 2) + c * 16 : SEQ_OOB;
-            vb[i] = has ? (uint32_t)(row * stride_b * 2) + c * 16 : SEQ_OOB;
-            lds[i] = packed_at<DH>(row, c);
-        }
-    }
-    __device__ __forceinline__ void load(int, const bf16_t* a, int left_a, char*, const bf16_t* b, int left_b, char*) {
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            ra[i] = seq_load16(a, left_a, va[i]);
-            rb[i] = seq_load16(b, left_b, vb[i]);
-        }
-    }
-    __device__ __forceinline__ void land(char* ta, char* tb) const {
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            *reinterpret_cast<u32x4_t*>(ta + lds[i]) = ra[i];
-            *reinterpret_cast<u32x4_t*>(tb + lds[i]) = rb[i];
-        }
-    }
-};
-// Wider heads: straight into LDS (buffer_load ... lds, 16 B per lane, no registers): a wave fills 1-KiB slabs of consecutive LDS,
-// lane l's slot of row l / SW gets the chunk that the swizzle (its own inverse) puts there; slots of chunks behind the head's width get zeros.
-// The compiler waits for all outstanding loads at the first transposing read of an iteration: by then the first product and the exponentials have passed,
-// which is longer than a tile takes from L2.
-template <int DH, int NW>
+// A pair of tiles of 64 MUL rows (K and V, or Q and dO) straight into LDS (buffer_load ... lds, 16 B per lane, no registers): a wave fills 1-KiB slabs of consecutive
+// LDS, lane l's slot of row l / SW gets the chunk that the swizzle (its own inverse) puts there; slots of chunks behind the head's width get zeros.
+// load() asks for the next pair while one is worked on; land() ends the trip in front of the barrier that publishes it.
+// KEEP: the lane offsets stay in registers (head widths up to 64: a few); else they are formed anew each time.
+template <int DH, int NW, int MUL, bool KEEP>
 struct PackedDma {
     using G = PackedGeo<DH>;
-    static constexpr int SLABS = G::TILE / 1024 / NW, ROWS = 1024 / G::PITCH;
+    static constexpr int SLABS = MUL * G::TILE / 1024 / NW, ROWS = 1024 / G::PITCH;
+    static_assert(MUL * G::TILE / 1024 % NW == 0, "every wave fills the same number of slabs");
     int row0, slot, dim;
     uint32_t pa, pb;                                                            // row strides in bytes
+    uint32_t va[KEEP ? SLABS : 1], vb[KEEP ? SLABS : 1];
+    __device__ __forceinline__ uint32_t offset(int i, uint32_t pitch) const {
+        const int row = row0 + i * ROWS, c = attn_swz<G::SW>(row, slot);
+        return c * 8 < dim ? row * pitch + c * 16 : SEQ_OOB;
+    }
     __device__ __forceinline__ void init(int wave, int lane, int width, int64_t stride_a, int64_t stride_b) {
         row0 = wave * SLABS * ROWS + lane / G::SW; slot = lane % G::SW; dim = width;
         pa = (uint32_t)(stride_a * 2); pb = (uint32_t)(stride_b * 2);
+        if (KEEP)
+#pragma unroll
+            for (int i = 0; i < SLABS; ++i) { va[i] = offset(i, pa); vb[i] = offset(i, pb); }
     }
     __device__ __forceinline__ void load(int wave, const bf16_t* a, int left_a, char* ta, const bf16_t* b, int left_b, char* tb) {
-        asm volatile("" : "+v"(row0), "+v"(slot));                              // (offsets are formed anew: registers are short)
+        if (!KEEP) asm volatile("" : "+v"(row0), "+v"(slot));
 #pragma unroll
         for (int i = 0; i < SLABS; ++i) {
-            const int row = row0 + i * ROWS, c = attn_swz<G::SW>(row, slot);
-            const bool has = c * 8 < dim;
-            seq_dma16(a, left_a, ta + (wave * SLABS + i) * 1024, has ? row * pa + c * 16 : SEQ_OOB);
-            seq_dma16(b, left_b, tb + (wave * SLABS + i) * 1024, has ? row * pb + c * 16 : SEQ_OOB);
+            seq_dma16(a, left_a, ta + (wave * SLABS + i) * 1024, KEEP ? va[KEEP ? i : 0] : offset(i, pa));
+            seq_dma16(b, left_b, tb + (wave * SLABS + i) * 1024, KEEP ? vb[KEEP ? i : 0] : offset(i, pb));
         }
     }
-    __device__ __forceinline__ void land(char*, char*) const { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }      // this wave's slabs; the barrier does the rest
+    __device__ __forceinline__ void land() const { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }      // this wave's slabs; the barrier does the rest
 };
-template <int DH, int NW>
-using PackedTiles = std::conditional_t<(DH > 64), PackedDma<DH, NW>, PackedRegs<DH, NW>>;
 
 // (slot, head) of a block.  Heads fastest, key heads before the query heads that share them: consecutive blocks go round-robin over the 8 XCDs, so with 8, 4, 2 or 1
 // key heads an XCD's L2 sees one key head only.

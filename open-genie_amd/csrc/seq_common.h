@@ -78,7 +78,7 @@ __device__ __forceinline__ SeqSlot seq_find_longest(const int32_t* cu, int nseq,
 
 // ------------------------------------------------------------------------------------------------------------------------------
 // Range-checked 16-B load: lanes whose offset reaches past `bytes_left` get zeros.  Offsets are inside one tile (the base moves in 64 bits), and the
-// host refuses row strides whose tile does not fit 2^28 bytes.  SEQ_OOB marks a lane that never has data (columns behind the head's width).
+// host refuses row strides whose tile does not fit 2^29 bytes.  SEQ_OOB marks a lane that never has data (columns behind the head's width).
 // ------------------------------------------------------------------------------------------------------------------------------
 #define SEQ_OOB 0x7ff00000u
 __device__ __forceinline__ u32x4_t seq_load16(const void* base, int bytes_left, uint32_t voff) {
@@ -90,9 +90,9 @@ __device__ __forceinline__ void seq_dma16(const void* base, int bytes_left, char
     const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, bytes_left, 0x00020000);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, LDS_PTR(lds), 16, voff, 0u, 0, 0);
 }
-// bytes a tile of at most 64 rows may read from its first row on, when `rows` rows remain (row strides are under 2^22 bytes: 32 bits hold it)
+// bytes a tile of at most 128 rows may read from its first row on, when `rows` rows remain (row strides are under 2^22 bytes: 32 bits hold it)
 __device__ __forceinline__ int seq_bytes_left(int rows, int64_t stride_bytes, int dim) {
-    return rows <= 0 ? 0 : (min(rows, 64) - 1) * (int)stride_bytes + dim * 2;
+    return rows <= 0 ? 0 : (min(rows, 128) - 1) * (int)stride_bytes + dim * 2;
 }
 
 // ds_read_b64_tr_b16: in each group of 16 lanes, lane i names 4 consecutive 16-bit values of row i / 4 (columns 4 (i % 4) ...) and receives column i of the
