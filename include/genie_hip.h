@@ -519,13 +519,14 @@ int genie_attention_lean_occupancy(int which);
  *   - all sums in a fixed order (no atomics); every workspace is the caller's, nothing is kept between calls.
  * ------------------------------------------------------------------------------------------- */
 /* Causal softmax attention with hq query heads over hkv key / value heads (hq % hkv == 0): query i of a sequence sees keys 0 .. i + n_k - n_q; a query that sees
- * none gives zeros.  lse [hq][rows_q] fp32 (optional in the forward): natural-log sum of the scaled scores' exponentials, -inf where nothing is seen. */
-int genie_packed_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int32_t* cu_q, const int32_t* cu_k, int nseq,
+ * none gives zeros.  For the backward call (optional): out_lo, bf16 like out, what the rounding of out left over; lse [hq][rows_q] fp32, the natural logarithm of the
+ * sum of the scaled scores' exponentials, -inf where nothing is seen. */
+int genie_packed_attention_fwd(const void* q, const void* k, const void* v, void* out, void* out_lo, float* lse, const int32_t* cu_q, const int32_t* cu_k, int nseq,
                                int rows_q, int rows_k, int hq, int hkv, int dim, const int64_t* q_strides, const int64_t* k_strides,
                                const int64_t* v_strides, float scale, void* stream);
-/* Its gradients; out, lse from the forward, ws: genie_packed_attention_bwd_ws_floats, 16-byte aligned. */
+/* Its gradients; out, out_lo, lse from the forward, ws: genie_packed_attention_bwd_ws_floats, 16-byte aligned. */
 int64_t genie_packed_attention_bwd_ws_floats(int nseq, int rows_q, int rows_k, int hq, int hkv, int dim);
-int genie_packed_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse, float* ws, int64_t ws_floats, void* dq,
+int genie_packed_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* out_lo, const void* dout, const float* lse, float* ws, int64_t ws_floats, void* dq,
                                void* dk, void* dv, const int32_t* cu_q, const int32_t* cu_k, int nseq, int rows_q, int rows_k, int hq, int hkv, int dim,
                                const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int64_t* dout_strides, float scale,
                                void* stream);
@@ -539,8 +540,8 @@ int genie_cached_attention_step(const void* q, const void* k_new, const void* v_
                                 void* stream);
 /* Linear attention with a decay per head: S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T, o_t = scale q_t S_t; log_decay fp32 [heads] on the device, <= 0.
  * initial_state / final_state fp32 [nseq][heads][dk][dv], optional.  Sequences are cut into segments; states (bf16: the states in front of the segments, which the
- * backward call reads again) and ws (fp32) hold genie_decay_attention_state_elems elements each, with_state = initial_state || final_state; it may be 0. */
-int64_t genie_decay_attention_state_elems(int nseq, int rows, int heads, int dk, int dv, int with_state);
+ * backward call reads again) and ws (fp32) hold genie_decay_attention_state_elems elements each; it may be 0. */
+int64_t genie_decay_attention_state_elems(int nseq, int rows, int heads, int dk, int dv, int has_initial);
 int genie_decay_attention_fwd(const void* q, const void* k, const void* v, const float* log_decay, const int32_t* cu, const float* initial_state, void* out,
                               float* final_state, void* states, float* ws, int64_t state_elems, int nseq, int rows, int heads, int dk, int dv,
                               const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, float scale, void* stream);

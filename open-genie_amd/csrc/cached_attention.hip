@@ -5,10 +5,13 @@
 // Bound by reading K and V once: 4 n Hkv D bytes against 4 n Hq D operations.  The query heads that share a key head are the 16 columns of one
 // 16x16x32 product, so a cache row is read once for all of them and the vector units do no dot products; a wave walks 32-key tiles on its own --
 // K straight into operand registers, V through its private LDS tile for the transposing read, the next tile's loads in flight meanwhile -- and there is
-// no barrier in the key loop.  The key axis is split over blocks when batch x key heads do not fill the chip; the parts (maximum, sum, unnormalised fp32
-// output) are joined by a second small kernel in a fixed order.  Lengths are read on the device: a captured graph replays with the lengths of the day.
+// no barrier in the key loop.  Where batch x key heads do not fill the chip, short caches get blocks of more waves (their parts meet in LDS), long ones are
+// split over blocks, and a second small kernel joins the parts (maximum, sum, unnormalised fp32 output) in a fixed order.  Lengths are read on the device: a captured graph replays with the lengths of the day.
 #include "seq_common.h"
 #include "genie_hip.h"
+#ifndef CACHED_NT
+#define CACHED_NT true
+#endif
 
 struct CachedArgs {
     const bf16_t *q, *k_new, *v_new;
@@ -21,12 +24,16 @@ struct CachedArgs {
 };
 
 template <int DH>
-__global__ void __launch_bounds__(256, 2) cached_step_kernel(const CachedArgs a) {
+constexpr int cached_wave_bytes() {                                             // one wave's V tile, later its output part, rows padded by 16 B against bank conflicts
+    const int tile = 32 * (DH <= 64 ? 128 : 256), part = 16 * (DH + 4) * 4;
+    return tile > part ? tile : part;
+}
+
+template <int DH, int NW>
+__global__ void __launch_bounds__(64 * NW, DH <= 64 ? 4 : 2) cached_step_kernel(const CachedArgs a) {
     constexpr int KS = DH / 32, DT = DH / 16, CPR = DH / 8, PITCH = DH <= 64 ? 128 : 256, SW = PITCH / 16, VP = 32 * CPR / 64;
-    constexpr int WBYTES = 32 * PITCH;                                          // one wave's V tile
-    constexpr int OBYTES = 16 * (DH + 4) * 4;                                   // one wave's output part, rows padded by 16 B against bank conflicts
-    constexpr int WREG = WBYTES > OBYTES ? WBYTES : OBYTES;
-    __shared__ __attribute__((aligned(16))) char smem[4 * WREG + 4 * 16 * 8];
+    constexpr int WREG = cached_wave_bytes<DH>();
+    extern __shared__ __attribute__((aligned(16))) char smem[];                 // NW WREG + 128 NW
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
     int id = (int)blockIdx.x;
@@ -139,25 +146,12 @@ __global__ void __launch_bounds__(256, 2) cached_step_kernel(const CachedArgs a)
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) kr[kt][ks] = seq_load16(kp, kl, koff[kt][ks]);
+            for (int ks = 0; ks < KS; ++ks) kr[kt][ks] = seq_load16<CACHED_NT>(kp, kl, koff[kt][ks]);
 #pragma unroll
-        for (int i = 0; i < VP; ++i) vr[i] = seq_load16(vp, vl, voff[i]);
+        for (int i = 0; i < VP; ++i) vr[i] = seq_load16<CACHED_NT>(vp, vl, voff[i]);
     };
-    int t = split * per + wave;
-    if (t < t_end) load(t);
-    while (t < t_end) {
-        u32x4_t kc[2][KS], vc[VP];
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) { kc[0][ks] = kr[0][ks]; kc[1][ks] = kr[1][ks]; }
-#pragma unroll
-        for (int i = 0; i < VP; ++i) vc[i] = vr[i];
-        const int live = min(32, n - t * 32);
-        t += 4;
-        if (t < t_end) load(t);
-        tile(kc, vc, live);
-    }
-    if (append && split == 0 && wave == 0 && !bad && !idle) {
-        // the new token: a tile of one key, taken from the arguments and put into the cache by the same lanes (no other lane of this launch reads that row)
+    if (append && split == 0 && wave == NW - 1 && !bad && !idle) {
+        // the new token, in the wave with the fewest tiles: a tile of one key, taken from the arguments and put into the cache by the same lanes (no other lane of this launch reads that row)
         const bf16_t* kp = a.k_new + b * a.kn_b + kvh * a.kn_h;
         const bf16_t* vp = a.v_new + b * a.vn_b + kvh * a.vn_h;
         bf16_t* kd = a.kc + b * a.k_b + kvh * a.k_h + (int64_t)n * a.k_t;
@@ -182,10 +176,23 @@ __global__ void __launch_bounds__(256, 2) cached_step_kernel(const CachedArgs a)
         }
         tile(kr, vr, 1);
     }
-    // the four waves' parts: maxima, sums, outputs through LDS
+    int t = split * per + wave;
+    if (t < t_end) load(t);
+    while (t < t_end) {
+        u32x4_t kc[2][KS], vc[VP];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) { kc[0][ks] = kr[0][ks]; kc[1][ks] = kr[1][ks]; }
+#pragma unroll
+        for (int i = 0; i < VP; ++i) vc[i] = vr[i];
+        const int live = min(32, n - t * 32);
+        t += NW;
+        if (t < t_end) load(t);
+        tile(kc, vc, live);
+    }
+    // the waves' parts: maxima, sums, outputs through LDS
     l_run += __shfl_xor(l_run, 16);
     l_run += __shfl_xor(l_run, 32);
-    float* ml = reinterpret_cast<float*>(smem + 4 * WREG);
+    float* ml = reinterpret_cast<float*>(smem + NW * WREG);
     float* ob = reinterpret_cast<float*>(smem + wave * WREG);                   // this wave's own tile region: [16 heads][DH + 4]
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
 #pragma unroll
@@ -196,15 +203,15 @@ __global__ void __launch_bounds__(256, 2) cached_step_kernel(const CachedArgs a)
     }
     __syncthreads();
     const int nh = min(16, group - hg * 16), vec = a.dim / 4;
-    for (int i = tid; i < nh * vec; i += 256) {
+    for (int i = tid; i < nh * vec; i += 64 * NW) {
         const int hh = i / vec, d = (i % vec) * 4, ho = kvh * group + hg * 16 + hh;
         float m = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) m = fmaxf(m, ml[(w * 16 + hh) * 2]);
+        for (int w = 0; w < NW; ++w) m = fmaxf(m, ml[(w * 16 + hh) * 2]);
         float l = 0.f;
         f32x4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < NW; ++w) {
             const float mw = ml[(w * 16 + hh) * 2], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - m);
             const float lw = ml[(w * 16 + hh) * 2 + 1];
             const f32x4_t x = *reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(smem + w * WREG) + hh * (DH + 4) + d);
@@ -272,9 +279,16 @@ __global__ void __launch_bounds__(256) cached_join_kernel(const CachedArgs a) {
     }
 }
 
-static int cached_splits(int batch, int hq, int hkv, int cap) {
+#ifndef CACHED_BLOCKS
+#define CACHED_BLOCKS 2048
+#endif
+// waves of a block that takes a whole short cache, four tiles of 32 keys each
+static int cached_wide(int dim) { return dim <= 64 ? 16 : 8; }
+// parts of the key axis (0: one part, a wide block)
+static int cached_splits(int batch, int hq, int hkv, int dim, int cap) {
     const int64_t base = (int64_t)batch * hkv * ((hq / hkv + 15) / 16);
-    int64_t n = base > 0 ? (1024 + base - 1) / base : 1;
+    if (base < 512 && cap <= 128 * cached_wide(dim)) return 0;
+    int64_t n = base > 0 ? (CACHED_BLOCKS + base - 1) / base : 1;
     const int64_t most = (cap + 127) / 128;
     n = n < most ? n : most;
     return (int)(n < 1 ? 1 : n > 128 ? 128 : n);
@@ -282,15 +296,27 @@ static int cached_splits(int batch, int hq, int hkv, int cap) {
 
 extern "C" int64_t genie_cached_attention_ws_floats(int batch, int hq, int hkv, int dim, int capacity) {
     if (batch <= 0 || hkv <= 0 || hq <= 0 || hq % hkv != 0 || dim <= 0 || capacity <= 0) return 0;
-    const int n = cached_splits(batch, hq, hkv, capacity);
-    return n == 1 ? 0 : (int64_t)batch * hq * n * (dim + 4);
+    const int n = cached_splits(batch, hq, hkv, dim, capacity);
+    return n <= 1 ? 0 : (int64_t)batch * hq * n * (dim + 4);
 }
 
 template <int DH>
-static int cached_dispatch(const CachedArgs& a, void* stream) {
+static int cached_dispatch(CachedArgs& a, void* stream) {
+    constexpr int NWIDE = DH <= 64 ? 16 : 8, WREG = cached_wave_bytes<DH>();
+    const bool wide = a.nsplit == 0;
+    a.nsplit = wide ? 1 : a.nsplit;
     const int64_t blocks = (int64_t)a.batch * a.hkv * a.hgroups * a.nsplit;
     GENIE_CHECK_ARG(blocks < (1ll << 31), "genie_cached_attention_step: too many blocks");
-    hipLaunchKernelGGL(cached_step_kernel<DH>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a);
+    const int nw = wide ? NWIDE : 4, lds = nw * (WREG + 128);
+    auto* kernel = wide ? cached_step_kernel<DH, NWIDE> : cached_step_kernel<DH, 4>;
+    if (lds > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) {
+            genie_set_error("genie_cached_attention_step: %s", hipGetErrorString(e));
+            return GENIE_ERR_HIP;
+        }
+    }
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * nw), lds, (hipStream_t)stream, a);
     GENIE_CHECK_LAUNCH();
     if (a.nsplit > 1) {
         hipLaunchKernelGGL(cached_join_kernel, dim3((unsigned)(a.batch * a.hq)), dim3(256), 0, (hipStream_t)stream, a);
@@ -319,7 +345,7 @@ extern "C" int genie_cached_attention_step(const void* q, const void* k_new, con
     const int64_t s[12] = {a.q_b, a.q_h, a.kn_b, a.kn_h, a.vn_b, a.vn_h, a.k_b, a.k_t, a.k_h, a.v_b, a.v_t, a.v_h};
     for (int i = 0; i < 12; ++i) GENIE_CHECK_ARG(s[i] >= 0 && s[i] % 8 == 0, "%s: strides must be multiples of 8 elements", what);
     GENIE_CHECK_ARG(a.k_t >= dim && a.v_t >= dim && a.k_t < (1 << 21) && a.v_t < (1 << 21), "%s: a cache row's stride must be between the head width and 2^21 elements", what);
-    a.nsplit = cached_splits(batch, hq, hkv, capacity);
+    a.nsplit = cached_splits(batch, hq, hkv, dim, capacity);
     a.hgroups = (hq / hkv + 15) / 16;
     if (a.nsplit > 1) {
         GENIE_CHECK_ARG(ws && ws_floats >= genie_cached_attention_ws_floats(batch, hq, hkv, dim, capacity), "%s: workspace too small", what);

@@ -15,10 +15,14 @@
 // All powers have exponents >= 0 (strong decays underflow to 0, nothing overflows).
 //
 // Roundings to bf16: the scores and M as matrix operands of an output that is itself rounded to bf16.  The states themselves are fp32 and so is what goes into them:
-// the state update's decayed operand l^(n-1-s) c_s enters as a sum of two bf16 values (2^-16 left).
+// the state update's decayed operand l^(n-1-s) c_s enters as a sum of three bf16 values (2^-24 left: fp32).  The backward's states, which only become
+// operands of gradients, take two (2^-16, far under the operand's own 2^-8).
 #include "packed_common.h"
 
 #define DECAY_SEG 256
+#ifndef STEP_NT
+#define STEP_NT 1
+#endif
 
 struct DecayRole {
     const bf16_t *a, *b, *c;
@@ -84,8 +88,8 @@ struct DecayTile {
 };
 
 // What one segment adds to the state, M = sum_s l^(n-1-s) b_s c_s^T over its n tokens, stored transposed ([dc][da]); wave w owns columns 32 w .. of C.  A
-// sequence's last segment is only needed where the final state is.
-template <int DH>
+// sequence's last segment is only needed where the final state is.  DIRECT: every sequence is one segment and starts from nothing: the sum is the final state.
+template <int DH, int TERMS, bool DIRECT>
 __global__ void __launch_bounds__(64 * (DH / 32), 2) decay_state_kernel(const DecayArgs g) {
     using G = DecayGeo<DH>;
     __shared__ __attribute__((aligned(16))) char smem[2 * G::TILE];
@@ -94,7 +98,7 @@ __global__ void __launch_bounds__(64 * (DH / 32), 2) decay_state_kernel(const De
     const int head = (int)blockIdx.x % g.heads, slot = (int)blockIdx.x / g.heads;
     const SeqSlot s = seq_find<DECAY_SEG>(g.cu, g.nseq, g.rows, slot);
     const int p0 = s.tile * DECAY_SEG;
-    if (s.seq == g.nseq || s.tile < 0 || p0 >= s.len) return;
+    if (s.seq == g.nseq || s.tile < 0 || p0 >= max(s.len, DIRECT ? 1 : 0)) return;      // (DIRECT: an empty sequence's state is written too)
     if (p0 + DECAY_SEG >= s.len && !R.final_state) return;
     const int p1 = min(s.len, p0 + DECAY_SEG);
     const float log2_l = g.log_decay[head] * 1.4426950408889634f;
@@ -112,9 +116,11 @@ __global__ void __launch_bounds__(64 * (DH / 32), 2) decay_state_kernel(const De
     for (int i = 0; i < G::DT; ++i) m[i] = packed_splat(0.f);
     char *bt = smem, *ct = smem + G::TILE;
     // the chunk that does not fill a tile comes first: all others end where the next one begins
-    int nv = (p1 - p0 - 1) % 64 + 1;
-    tb.load(p0, nv, s.len);
-    tc.load(p0, nv, s.len);
+    int nv = (p1 - p0 + 63) % 64 + 1;
+    if (p0 < p1) {
+        tb.load(p0, nv, s.len);
+        tc.load(p0, nv, s.len);
+    }
     for (int p = p0; p < p1;) {
         tb.store(bt);
         tc.store(ct);
@@ -133,27 +139,45 @@ __global__ void __launch_bounds__(64 * (DH / 32), 2) decay_state_kernel(const De
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
             const bf16x8_t cf = at.tr_frag(ct + ks * 16 * G::PITCH, wave);
-            float hi[8], lo[8];
+            float x[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                hi[j] = bf16_to_f32((bf16_t)cf[j]) * fade[8 * (ks & 1) + j];
-                if (ks < 2) hi[j] *= p32;
+                x[j] = bf16_to_f32((bf16_t)cf[j]) * fade[8 * (ks & 1) + j];
+                if (ks < 2) x[j] *= p32;
             }
-            const u32x4_t fh = {pack_bf16x2(hi[0], hi[1]), pack_bf16x2(hi[2], hi[3]), pack_bf16x2(hi[4], hi[5]), pack_bf16x2(hi[6], hi[7])};
+            bf16x8_t part[TERMS];                                               // x = the sum of the parts
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                lo[2 * j] = hi[2 * j] - __uint_as_float(fh[j] << 16);
-                lo[2 * j + 1] = hi[2 * j + 1] - __uint_as_float(fh[j] & 0xffff0000u);
+            for (int n = 0; n < TERMS; ++n) {
+                const u32x4_t f = {pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
+                part[n] = __builtin_bit_cast(bf16x8_t, f);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    x[2 * j] -= __uint_as_float(f[j] << 16);
+                    x[2 * j + 1] -= __uint_as_float(f[j] & 0xffff0000u);
+                }
             }
-            const bf16x8_t fl = seq_pack8(lo[0], lo[1], lo[2], lo[3], lo[4], lo[5], lo[6], lo[7]);
 #pragma unroll
             for (int i = 0; i < G::DT; ++i) {
                 const bf16x8_t bf = at.tr_frag(bt + ks * 16 * G::PITCH, i);
-                m[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, fh), bf, m[i], 0, 0, 0);
-                m[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fl, bf, m[i], 0, 0, 0);
+#pragma unroll
+                for (int n = TERMS - 1; n >= 0; --n) m[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(part[n], bf, m[i], 0, 0, 0);
             }
         }
         __syncthreads();
+    }
+    if (DIRECT) {                                                               // natural layout: four consecutive columns of a row per store
+        float* dst = R.final_state + ((int64_t)s.seq * g.heads + head) * R.da * R.dc;
+#pragma unroll
+        for (int i = 0; i < G::DT; ++i) {
+            const int row = 32 * i + (lane & 31);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int col = 32 * wave + 8 * q + 4 * h;
+                if (row < R.da && col < R.dc)
+                    *reinterpret_cast<f32x4_t*>(dst + (uint32_t)(row * R.dc + col)) = f32x4_t{m[i][4 * q], m[i][4 * q + 1], m[i][4 * q + 2], m[i][4 * q + 3]};
+            }
+        }
+        return;
     }
     float* dst = R.local + ((int64_t)slot * g.heads + head) * R.da * R.dc;
 #pragma unroll
@@ -167,40 +191,64 @@ __global__ void __launch_bounds__(64 * (DH / 32), 2) decay_state_kernel(const De
     }
 }
 
-// States in front of the segments: M_0 = initial or 0, M_{i+1} = l^256 M_i + local_i, elementwise in fp32 with a thread per four elements; each M_i is stored rounded
-// to bf16 as the operand that it becomes, the last sum is the final state.  The segments' values are requested eight ahead of the chain.
+// States in front of the segments: M_0 = initial or 0, M_{i+1} = l^256 M_i + local_i, elementwise in fp32; each M_i is stored rounded to bf16 as the operand that it
+// becomes, the last sum is the final state.  A lane owns four elements, the block's four waves take eight segments each of 32 at a time: all 32 loads of a
+// step are in flight together, the waves' sums meet in LDS, and each wave walks its own eight from there.  (One wave walking all of them, eight loads ahead: 18 us
+// for 128 segments of 8 heads of width 64 -- a chain of store and load latencies.)
 __global__ void __launch_bounds__(256) decay_scan_kernel(const DecayArgs g) {
+    __shared__ __attribute__((aligned(16))) f32x4_t part[2][4][64];
     const DecayRole& R = g.r[0];
     const int seq = (int)blockIdx.x / g.heads, head = (int)blockIdx.x % g.heads, matrix = R.da * R.dc;
-    const int e = ((int)blockIdx.y * 256 + (int)threadIdx.x) * 4;
-    if (e >= matrix) return;
+    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int e0 = ((int)blockIdx.y * 64 + lane) * 4, e = min(e0, matrix - 4);   // (lanes past the end repeat the last elements' work and store the same)
     const int start = seq_cu(g.cu, seq, g.rows), len = max(0, seq_cu(g.cu, seq + 1, g.rows) - start), nseg = (len + DECAY_SEG - 1) / DECAY_SEG;
     const float log2_l = g.log_decay[head] * 1.4426950408889634f, l = decay_pow(log2_l, DECAY_SEG);
-    const int c = e / R.da, a = e % R.da;                                       // element (a .. a + 3, c) of the natural matrix
+    const int c = e / R.da, a = e % R.da;                                       // elements (a .. a + 3, c) of the states that go in and out
+    const int64_t of_seq = ((int64_t)seq * g.heads + head) * matrix;
     f32x4_t m = {0.f, 0.f, 0.f, 0.f};
     if (R.initial) {
-        const float* src = R.initial + ((int64_t)seq * g.heads + head) * matrix;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) m[j] = src[(a + j) * R.dc + c];
+        for (int j = 0; j < 4; ++j) m[j] = R.initial[of_seq + (a + j) * R.dc + c];
     }
     const int64_t step = (int64_t)g.heads * matrix, first = ((int64_t)(start / DECAY_SEG + seq) * g.heads + head) * matrix + e;
     const float* src = R.local + first;
     bf16_t* dst = R.states + first;
     const int full = nseg - 1;                                                  // segments whose sum is followed by another segment
-    f32x4_t x[8];
+    const float l8 = decay_pow(log2_l, 8 * DECAY_SEG);
+    for (int base = 0, flip = 0; base < full; base += 32, flip ^= 1) {
+        const int i0 = base + wave * 8, n = min(8, full - i0);
+        f32x4_t x[8], sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (j < full) x[j] = *reinterpret_cast<const f32x4_t*>(src + j * step);
-    for (int i = 0; i < full; i += 8) {
+        for (int j = 0; j < 8; ++j)
+            if (j < n) x[j] = *reinterpret_cast<const f32x4_t*>(src + (i0 + j) * step);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if (i + j >= full) break;
-            *reinterpret_cast<u32x2_t*>(dst + (i + j) * step) = u32x2_t{pack_bf16x2(m[0], m[1]), pack_bf16x2(m[2], m[3])};
+        for (int j = 0; j < 8; ++j)
+            if (j < n)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) m[q] = __builtin_fmaf(m[q], l, x[j][q]);
-            if (i + j + 8 < full) x[j] = *reinterpret_cast<const f32x4_t*>(src + (i + j + 8) * step);
+                for (int q = 0; q < 4; ++q) sum[q] = __builtin_fmaf(sum[q], l, x[j][q]);
+        part[flip][wave][lane] = sum;
+        __syncthreads();
+        f32x4_t mine = m;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            if (w == wave) mine = m;
+            const int nw = min(8, full - base - w * 8);
+            if (nw > 0) {
+                const float f = nw == 8 ? l8 : decay_pow(log2_l, nw * DECAY_SEG);
+                const f32x4_t s = part[flip][w][lane];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) m[q] = __builtin_fmaf(m[q], f, s[q]);
+            }
         }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < n) {
+                *reinterpret_cast<u32x2_t*>(dst + (i0 + j) * step) = u32x2_t{pack_bf16x2(mine[0], mine[1]), pack_bf16x2(mine[2], mine[3])};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) mine[q] = __builtin_fmaf(mine[q], l, x[j][q]);
+            }
     }
+    if (wave != 0) return;
     if (nseg > 0) *reinterpret_cast<u32x2_t*>(dst + (nseg - 1) * step) = u32x2_t{pack_bf16x2(m[0], m[1]), pack_bf16x2(m[2], m[3])};
     if (!R.final_state) return;
     if (nseg > 0) {
@@ -209,9 +257,8 @@ __global__ void __launch_bounds__(256) decay_scan_kernel(const DecayArgs g) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) m[q] = __builtin_fmaf(m[q], ln, last[q]);
     }
-    float* out = R.final_state + ((int64_t)seq * g.heads + head) * matrix;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) out[(a + j) * R.dc + c] = m[j];
+    for (int j = 0; j < 4; ++j) R.final_state[of_seq + (a + j) * R.dc + c] = m[j];
 }
 
 // A pair of 64-row tiles straight into LDS, as PackedDma, for tokens walked in either direction (reverse: row i is token nv - 1 - i from the base; the rows behind
@@ -363,6 +410,20 @@ __global__ void __launch_bounds__(256, DH <= 64 ? DECAY_OUT_WPE64 : 2) decay_out
 // 0.4 % of that.  A thread owns four columns of every RP-th row; eight rows are in flight per thread; the rows' partial sums of o meet in LDS.  Heads of
 // small batches are cut into column slices so that the few states spread over more CUs.
 // ------------------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ f32x4_t decay_stream_load(const float* p) {
+#if STEP_NT & 1
+    return __builtin_nontemporal_load(reinterpret_cast<const f32x4_t*>(p));
+#else
+    return *reinterpret_cast<const f32x4_t*>(p);
+#endif
+}
+__device__ __forceinline__ void decay_stream_store(float* p, f32x4_t v) {
+#if STEP_NT & 2
+    __builtin_nontemporal_store(v, reinterpret_cast<f32x4_t*>(p));
+#else
+    *reinterpret_cast<f32x4_t*>(p) = v;
+#endif
+}
 struct DecayStepArgs {
     const bf16_t *q, *k, *v;
     bf16_t* out;
@@ -397,7 +458,7 @@ __global__ void __launch_bounds__(256) decay_step_kernel(const DecayStepArgs a) 
         for (int base = r0; base < a.dk; base += 8 * rp) {
             f32x4_t x[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const f32x4_t*>(src + (uint32_t)(min(base + i * rp, a.dk - 1) * a.dv));
+            for (int i = 0; i < 8; ++i) x[i] = decay_stream_load(src + (uint32_t)(min(base + i * rp, a.dk - 1) * a.dv));
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int row = base + i * rp;
@@ -407,7 +468,7 @@ __global__ void __launch_bounds__(256) decay_step_kernel(const DecayStepArgs a) 
                     x[i][e] = __builtin_fmaf(x[i][e], l, kk * v[e]);
                     o[e] = row < a.dk ? __builtin_fmaf(qq, x[i][e], o[e]) : o[e];
                 }
-                if (row < a.dk) *reinterpret_cast<f32x4_t*>(dst + (uint32_t)(row * a.dv)) = x[i];
+                if (row < a.dk) decay_stream_store(dst + (uint32_t)(row * a.dv), x[i]);
             }
         }
     *reinterpret_cast<f32x4_t*>(so + tid * 4) = o;
@@ -424,9 +485,9 @@ __global__ void __launch_bounds__(256) decay_step_kernel(const DecayStepArgs a) 
 // ------------------------------------------------------------------------------------------------------------------------------
 // C entry points
 // ------------------------------------------------------------------------------------------------------------------------------
-// matrix elements of a call's segment states (one bf16 operand and one fp32 sum each); none where every sequence is one segment and no state goes in or out
-extern "C" int64_t genie_decay_attention_state_elems(int nseq, int rows, int heads, int dk, int dv, int with_state) {
-    if (nseq <= 0 || rows <= 0 || heads <= 0 || dk <= 0 || dv <= 0 || (rows <= DECAY_SEG && !with_state)) return 0;
+// matrix elements of a call's segment states (one bf16 operand and one fp32 sum each); none where every sequence is one segment and starts from nothing
+extern "C" int64_t genie_decay_attention_state_elems(int nseq, int rows, int heads, int dk, int dv, int has_initial) {
+    if (nseq <= 0 || rows <= 0 || heads <= 0 || dk <= 0 || dv <= 0 || (rows <= DECAY_SEG && !has_initial)) return 0;
     return (int64_t)(rows / DECAY_SEG + nseq + 1) * heads * dk * dv;
 }
 
@@ -454,10 +515,14 @@ static int decay_run(const DecayArgs& g, int roles, void* stream) {
     const int64_t segs = (int64_t)(g.rows / DECAY_SEG + g.nseq + 1) * g.heads, blocks = (int64_t)(g.rows / 128 + g.nseq + 1) * g.heads;
     GENIE_CHECK_ARG(segs < (1ll << 31) && blocks < (1ll << 31), "decay attention: too many blocks");
     const DecayRole& r = g.r[0];
-    if (r.local && g.nseq > 0) {
-        hipLaunchKernelGGL(decay_state_kernel<DH>, dim3((unsigned)segs), dim3(DecayGeo<DH>::NT), 0, (hipStream_t)stream, g);
+    if (g.nseq > 0 && (r.local || r.final_state)) {
+        auto* kernel = !r.local ? decay_state_kernel<DH, 3, true> : roles == 1 ? decay_state_kernel<DH, 3, false> : decay_state_kernel<DH, 2, false>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)segs), dim3(DecayGeo<DH>::NT), 0, (hipStream_t)stream, g);
         GENIE_CHECK_LAUNCH();
-        hipLaunchKernelGGL(decay_scan_kernel, dim3((unsigned)(g.nseq * g.heads), (unsigned)((r.da * r.dc + 1023) / 1024)), dim3(256), 0, (hipStream_t)stream, g);
+    }
+    if (g.nseq > 0 && r.local) {
+        const dim3 grid((unsigned)(g.nseq * g.heads), (unsigned)((r.da * r.dc + 255) / 256));
+        hipLaunchKernelGGL(decay_scan_kernel, grid, dim3(256), 0, (hipStream_t)stream, g);
         GENIE_CHECK_LAUNCH();
     }
     hipLaunchKernelGGL(decay_out_kernel<DH>, dim3((unsigned)blocks, roles), dim3(256), 4 * PackedGeo<DH>::TILE, (hipStream_t)stream, g);
@@ -487,7 +552,7 @@ extern "C" int genie_decay_attention_fwd(const void* q, const void* k, const voi
     r.da = dk; r.dc = dv; r.states = (bf16_t*)states; r.local = ws; r.initial = initial_state; r.final_state = final_state;
     rc = decay_check_role(what, r);
     if (rc != GENIE_OK) return rc;
-    const int64_t need = genie_decay_attention_state_elems(nseq, rows, heads, dk, dv, initial_state || final_state);
+    const int64_t need = genie_decay_attention_state_elems(nseq, rows, heads, dk, dv, initial_state != nullptr);
     GENIE_CHECK_ARG(state_elems >= need && (need == 0 || (states && ws)), "%s: workspace too small", what);
     if (need == 0) { r.states = nullptr; r.local = nullptr; }
     return decay_run_any(g, 1, stream);

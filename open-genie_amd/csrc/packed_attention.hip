@@ -9,9 +9,6 @@
 // layout of the second product -- the transposed V / K / dO / Q fragments are read in that order by ds_read_b64_tr_b16, nothing is exchanged.
 // The sequences' lengths live on the device only: seq_common.h maps slots to (sequence, tile).
 #include "packed_common.h"
-#ifndef DQ_UNROLL
-#define DQ_UNROLL 2
-#endif
 
 // ------------------------------------------------------------------------------------------------------------------------------
 // A block of the forward and dQ kernels: 128 query rows, 4 row groups of 32 x NG key groups of waves.  With two key groups alternate 64-key tiles pass through LDS two
@@ -187,15 +184,26 @@ __global__ void __launch_bounds__(256 * NG, WPE) packed_fwd_kernel(const PackedA
     if (r.grp == 0 && a.lse && h == 0 && r.qi < r.s.len)
         a.lse[(int64_t)r.blk.head * a.rows_q + r.s.start + r.qi] = l == 0.f ? -INFINITY : mc * 0.6931471805599453f + __logf(l);
     __syncthreads();                                                            // tiles and exchange area become the waves' output regions
-    if (r.grp == 0 && r.q0 < r.s.len)
-        packed_write_rows<DH>(smem + r.rw * 32 * G::PITCH, oacc, l == 0.f ? 0.f : 1.f / l, a.out + ((int64_t)(r.s.start + r.q0) * a.hq + r.blk.head) * a.dim,
-                              (int64_t)a.hq * a.dim, min(32, r.s.len - r.q0), a.dim);
+    if (r.grp == 0 && r.q0 < r.s.len) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int64_t to = ((int64_t)(r.s.start + r.q0) * a.hq + r.blk.head) * a.dim;
+        packed_write_rows<DH>(smem + r.rw * 32 * G::PITCH, oacc, inv, a.out + to, (int64_t)a.hq * a.dim, min(32, r.s.len - r.q0), a.dim);
+        if (a.out_lo) {
+#pragma unroll
+            for (int d = 0; d < G::DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) oacc[d][e] = oacc[d][e] * inv - bf16_to_f32(f32_to_bf16(oacc[d][e] * inv));
+            packed_write_rows<DH>(smem + r.rw * 32 * G::PITCH, oacc, 1.f, a.out_lo + to, (int64_t)a.hq * a.dim, min(32, r.s.len - r.q0), a.dim);
+        }
+    }
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------
 // Backward, dQ: the forward's walk over the keys with P recomputed from the log-sum-exp.  delta = rowsum(dO o O) of the wave's rows is formed from the
 // operand fragments, written out for the other kernel, and fed negated as the accumulator INPUT of dP^T = V dO^T, so that dS = P o (dP - delta) costs
-// no subtraction.  dS is rounded to bf16 for the last product, like P in the forward.
+// no subtraction.  dS is rounded to bf16 for the last product, like P in the forward.  delta takes O with the 16 bits that its rounding left over: where a row sees few
+// keys, dP - delta is a small difference, and the rounding of O alone would be as large an error in it as that of dS (a 5720-row batch: dQ 0.0026 off in
+// norm with it, 0.0024 without; sequences of a few tokens 0.0035 and 0.0024).
 // ------------------------------------------------------------------------------------------------------------------------------
 template <int DH, int NG, int WPE>
 __global__ void __launch_bounds__(256 * NG, WPE) packed_dq_kernel(const PackedArgs a) {
@@ -210,12 +218,14 @@ __global__ void __launch_bounds__(256 * NG, WPE) packed_dq_kernel(const PackedAr
     packed_row_frags<DH>(gf, a.dout + qrow * a.g_row + r.blk.head * a.g_head, r.qi < r.s.len, a.dim);
     float delta = 0.f, lse2 = INFINITY;                                         // a row that sees nothing, or none at all: exp2(x - inf) = 0
     {
-        bf16x8_t of[G::KS];
+        bf16x8_t of[G::KS], ol[G::KS];
         packed_row_frags<DH>(of, a.o + (qrow * a.hq + r.blk.head) * a.dim, r.qi < r.s.len, a.dim);
+        packed_row_frags<DH>(ol, a.out_lo + (qrow * a.hq + r.blk.head) * a.dim, r.qi < r.s.len, a.dim);
 #pragma unroll
         for (int ks = 0; ks < G::KS; ++ks)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(bf16_to_f32((bf16_t)gf[ks][e]), bf16_to_f32((bf16_t)of[ks][e]), delta);
+            for (int e = 0; e < 8; ++e)
+                delta = __builtin_fmaf(bf16_to_f32((bf16_t)gf[ks][e]), bf16_to_f32((bf16_t)of[ks][e]) + bf16_to_f32((bf16_t)ol[ks][e]), delta);
         delta = seq_xsum32(delta);
         if (r.qi < r.s.len) {
             const float lse = a.lse[(int64_t)r.blk.head * a.rows_q + qrow];
@@ -251,7 +261,7 @@ __global__ void __launch_bounds__(256 * NG, WPE) packed_dq_kernel(const PackedAr
         const int k0 = (t * NG + r.grp) * 64;
         if (k0 >= r.w_end) continue;
         at.forget();
-#pragma unroll DQ_UNROLL
+#pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
             f32x16_t sacc = packed_splat(0.f), dp = packed_splat(-delta);
 #pragma unroll
@@ -317,35 +327,35 @@ static int packed_check(const char* what, const PackedArgs& a) {
     return GENIE_OK;
 }
 
-#ifndef FWD_NG
-#define FWD_NG 2
-#define FWD_WPE 4
-#endif
-#ifndef DQ_NG
-#define DQ_NG 1
-#define DQ_WPE 3
-#endif
+// Two key groups per block (half the chain of steps, but waves without work where a sequence has only a tile or two, and at head widths above 64 one coupled block per CU
+// instead of two independent ones) from an average of 512 rows per sequence on, and while the launch leaves CUs short of blocks.  Measured one / two groups, us,
+// 16 query heads over 4 key heads: forward at width 64, one sequence of 1024 / 4096 / 8192: 18.2 / 15.3, 61.5 / 52.3, 158.0 / 157.3, at 40 x 100 rows 11.2 / 16.1;
+// width 128: 28.2 / 22.6, 101.2 / 91.2, 292.7 / 290.5, 4 x 2048: 89.0 / 97.8.  Backward at width 64: 52.1 / 49.3, 174.5 / 162.3, 504 / 520.
+static bool packed_two_groups(const PackedArgs& a, int64_t most) { return a.rows_q >= 512ll * a.nseq && (int64_t)(a.rows_q / 128) * a.hq <= most; }
+
 template <int DH>
 static int packed_fwd_dispatch(PackedArgs& a, void* stream) {
-    constexpr int NG = DH <= 64 ? FWD_NG : 1, WPE = DH <= 64 ? FWD_WPE : 2;
     a.nslots = a.rows_q / 128 + a.nseq + 1;
-    return packed_launch(packed_fwd_kernel<DH, NG, WPE>, a, (int64_t)a.nslots * a.hq, 256 * NG, 4 * NG * PackedGeo<DH>::TILE, stream);
+    const int64_t blocks = (int64_t)a.nslots * a.hq;
+    if (packed_two_groups(a, DH <= 64 ? (1ll << 31) : 512)) return packed_launch(packed_fwd_kernel<DH, 2, DH <= 64 ? 4 : 2>, a, blocks, 512, 8 * PackedGeo<DH>::TILE, stream);
+    return packed_launch(packed_fwd_kernel<DH, 1, DH <= 64 ? 3 : 2>, a, blocks, 256, 4 * PackedGeo<DH>::TILE, stream);
 }
 
 template <int DH>
 static int packed_bwd_dispatch(PackedArgs& a, void* stream) {
-    constexpr int NG = DH <= 64 ? DQ_NG : 1, WPE = DH <= 64 ? DQ_WPE : 2;
     a.nslots = a.rows_q / 128 + a.nseq + 1;
-    const int rc = packed_launch(packed_dq_kernel<DH, NG, WPE>, a, (int64_t)a.nslots * a.hq, 256 * NG, 4 * NG * PackedGeo<DH>::TILE, stream);
+    const int64_t blocks = (int64_t)a.nslots * a.hq;
+    const int rc = packed_two_groups(a, 512) ? packed_launch(packed_dq_kernel<DH, 2, 2>, a, blocks, 512, 8 * PackedGeo<DH>::TILE, stream)
+                                             : packed_launch(packed_dq_kernel<DH, 1, DH <= 64 ? 3 : 2>, a, blocks, 256, 4 * PackedGeo<DH>::TILE, stream);
     return rc != GENIE_OK ? rc : packed_dkv_run(a, stream);
 }
 
-extern "C" int genie_packed_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const int32_t* cu_q, const int32_t* cu_k, int nseq,
+extern "C" int genie_packed_attention_fwd(const void* q, const void* k, const void* v, void* out, void* out_lo, float* lse, const int32_t* cu_q, const int32_t* cu_k, int nseq,
                                           int rows_q, int rows_k, int hq, int hkv, int dim, const int64_t* q_strides, const int64_t* k_strides,
                                           const int64_t* v_strides, float scale, void* stream) {
     GENIE_CHECK_ARG(q_strides && k_strides && v_strides, "genie_packed_attention_fwd: null strides");
     PackedArgs a = {};
-    a.q = (const bf16_t*)q; a.k = (const bf16_t*)k; a.v = (const bf16_t*)v; a.out = (bf16_t*)out; a.lse = lse;
+    a.q = (const bf16_t*)q; a.k = (const bf16_t*)k; a.v = (const bf16_t*)v; a.out = (bf16_t*)out; a.out_lo = (bf16_t*)out_lo; a.lse = lse;
     a.cu_q = cu_q; a.cu_k = cu_k; a.nseq = nseq; a.rows_q = rows_q; a.rows_k = rows_k; a.hq = hq; a.hkv = hkv; a.dim = dim; a.scale = scale;
     a.q_row = q_strides[0]; a.q_head = q_strides[1]; a.k_row = k_strides[0]; a.k_head = k_strides[1]; a.v_row = v_strides[0]; a.v_head = v_strides[1];
     a.g_row = a.q_row; a.g_head = a.q_head;
@@ -359,20 +369,20 @@ extern "C" int genie_packed_attention_fwd(const void* q, const void* k, const vo
     return packed_fwd_dispatch<128>(a, stream);
 }
 
-extern "C" int genie_packed_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse, float* ws, int64_t ws_floats, void* dq,
+extern "C" int genie_packed_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* out_lo, const void* dout, const float* lse, float* ws, int64_t ws_floats, void* dq,
                                           void* dk, void* dv, const int32_t* cu_q, const int32_t* cu_k, int nseq, int rows_q, int rows_k, int hq, int hkv, int dim,
                                           const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int64_t* dout_strides, float scale,
                                           void* stream) {
     GENIE_CHECK_ARG(q_strides && k_strides && v_strides && dout_strides, "genie_packed_attention_bwd: null strides");
     PackedArgs a = {};
-    a.q = (const bf16_t*)q; a.k = (const bf16_t*)k; a.v = (const bf16_t*)v; a.o = (const bf16_t*)out; a.dout = (const bf16_t*)dout;
+    a.q = (const bf16_t*)q; a.k = (const bf16_t*)k; a.v = (const bf16_t*)v; a.o = (const bf16_t*)out; a.out_lo = (bf16_t*)const_cast<void*>(out_lo); a.dout = (const bf16_t*)dout;
     a.dq = (bf16_t*)dq; a.dk = (bf16_t*)dk; a.dv = (bf16_t*)dv; a.lse = const_cast<float*>(lse); a.delta = ws;
     a.cu_q = cu_q; a.cu_k = cu_k; a.nseq = nseq; a.rows_q = rows_q; a.rows_k = rows_k; a.hq = hq; a.hkv = hkv; a.dim = dim; a.scale = scale;
     a.q_row = q_strides[0]; a.q_head = q_strides[1]; a.k_row = k_strides[0]; a.k_head = k_strides[1]; a.v_row = v_strides[0]; a.v_head = v_strides[1];
     a.g_row = dout_strides[0]; a.g_head = dout_strides[1];
     const int rc = packed_check("genie_packed_attention_bwd", a);
     if (rc != GENIE_OK) return rc;
-    GENIE_CHECK_ARG(out && dout && lse && ws && dq && dk && dv, "genie_packed_attention_bwd: null pointer");
+    GENIE_CHECK_ARG(out && out_lo && dout && lse && ws && dq && dk && dv, "genie_packed_attention_bwd: null pointer");
     GENIE_CHECK_ARG(ws_floats >= genie_packed_attention_bwd_ws_floats(nseq, rows_q, rows_k, hq, hkv, dim) && (uintptr_t)ws % 16 == 0,
                     "genie_packed_attention_bwd: workspace too small or not 16-byte aligned");
     if (dim <= 32) return packed_bwd_dispatch<32>(a, stream);

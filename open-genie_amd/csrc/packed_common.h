@@ -5,7 +5,7 @@
 
 struct PackedArgs {
     const bf16_t *q, *k, *v, *o, *dout;
-    bf16_t *out, *dq, *dk, *dv;
+    bf16_t *out, *out_lo, *dq, *dk, *dv;      // out_lo: what the rounding of out left over, bf16, for rowsum(dO o O) (or NULL)
     float* lse;                    // [Hq][rows_q]  log-sum-exp of the scaled scores, -inf where a row sees nothing
     float* delta;                  // [Hq][rows_q]  rowsum(dO o O), written by the dQ kernel for the dK / dV kernel
     float* part;                   // [nsplit][dK, dV][rows_k][Hkv][dim] where a key tile's rows are split over blocks

@@ -81,9 +81,11 @@ __device__ __forceinline__ SeqSlot seq_find_longest(const int32_t* cu, int nseq,
 // host refuses row strides whose tile does not fit 2^29 bytes.  SEQ_OOB marks a lane that never has data (columns behind the head's width).
 // ------------------------------------------------------------------------------------------------------------------------------
 #define SEQ_OOB 0x7ff00000u
+// STREAM: non-temporal, for data that is read once.
+template <bool STREAM = false>
 __device__ __forceinline__ u32x4_t seq_load16(const void* base, int bytes_left, uint32_t voff) {
     const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, bytes_left, 0x00020000);
-    return __builtin_amdgcn_raw_buffer_load_b128(r, voff, 0, 0);
+    return __builtin_amdgcn_raw_buffer_load_b128(r, voff, 0, STREAM ? 2 : 0);
 }
 // the same load with its destination in LDS: lane l's 16 B go to lds + 16 l (lds is wave-uniform)
 __device__ __forceinline__ void seq_dma16(const void* base, int bytes_left, char* lds, uint32_t voff) {

@@ -136,9 +136,9 @@ SIGNATURES = {
     'genie_attention_dropout_mask': (C.c_int, [_P, _I, _I, _I, _I, _F, C.c_uint64, _P]),
     'genie_attention_lean_mode': (C.c_int, [_I]),
     'genie_attention_lean_occupancy': (C.c_int, [_I]),
-    'genie_packed_attention_fwd': (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _PL, _PL, _PL, _F, _P]),
+    'genie_packed_attention_fwd': (C.c_int, [_P] * 8 + [_I] * 6 + [_PL] * 3 + [_F, _P]),
     'genie_packed_attention_bwd_ws_floats': (C.c_int64, [_I] * 6),
-    'genie_packed_attention_bwd': (C.c_int, [_P] * 7 + [_L] + [_P] * 5 + [_I] * 6 + [_PL] * 4 + [_F, _P]),
+    'genie_packed_attention_bwd': (C.c_int, [_P] * 8 + [_L] + [_P] * 5 + [_I] * 6 + [_PL] * 4 + [_F, _P]),
     'genie_cached_attention_ws_floats': (C.c_int64, [_I, _I, _I, _I, _I]),
     'genie_cached_attention_step': (C.c_int, [_P] * 8 + [_L] + [_I] * 5 + [_PL] * 5 + [_F, _P]),
     'genie_decay_attention_state_elems': (C.c_int64, [_I] * 6),

@@ -137,13 +137,14 @@ def _packed_forward(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Tensor,
     (q, sq), (k, sk), (v, sv) = _rows(q), _rows(k), _rows(v)
     out = torch.empty((rows, hq, d), dtype=torch.bfloat16, device=q.device)
     lse = torch.empty((hq, rows), dtype=torch.float32, device=q.device) if keep else None
+    out_lo = torch.empty_like(out) if keep else None
     if rows and rows_k:
         P = _hip.ptr
-        _launch('genie_packed_attention_fwd', q.device, P(q), P(k), P(v), P(out), P(lse), P(cu_q), P(cu_k), cu_q.shape[0] - 1, rows, rows_k, hq, hkv, d, _i64(sq),
-                _i64(sk), _i64(sv), scale)
+        _launch('genie_packed_attention_fwd', q.device, P(q), P(k), P(v), P(out), P(out_lo), P(lse), P(cu_q), P(cu_k), cu_q.shape[0] - 1, rows, rows_k, hq, hkv, d,
+                _i64(sq), _i64(sk), _i64(sv), scale)
     else:
         out.zero_()
-    return out, ((q, k, v, out, lse, cu_q, cu_k), (sq, sk, sv, scale)) if keep else None
+    return out, ((q, k, v, out, out_lo, lse, cu_q, cu_k), (sq, sk, sv, scale)) if keep else None
 
 
 class _PackedAttention(torch.autograd.Function):
@@ -156,7 +157,7 @@ class _PackedAttention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout: Tensor):
-        q, k, v, out, lse, cu_q, cu_k = ctx.saved_tensors
+        q, k, v, out, out_lo, lse, cu_q, cu_k = ctx.saved_tensors
         sq, sk, sv, scale = ctx.cfg
         rows, hq, d = q.shape
         rows_k, hkv, _ = k.shape
@@ -168,7 +169,7 @@ class _PackedAttention(torch.autograd.Function):
             P = _hip.ptr
             nws = _hip.load_library().genie_packed_attention_bwd_ws_floats(cu_q.shape[0] - 1, rows, rows_k, hq, hkv, d)
             ws = torch.empty(nws, dtype=torch.float32, device=q.device)
-            _launch('genie_packed_attention_bwd', q.device, P(q), P(k), P(v), P(out), P(dout), P(lse), P(ws), nws, P(dq), P(dk), P(dv), P(cu_q), P(cu_k),
+            _launch('genie_packed_attention_bwd', q.device, P(q), P(k), P(v), P(out), P(out_lo), P(dout), P(lse), P(ws), nws, P(dq), P(dk), P(dv), P(cu_q), P(cu_k),
                     cu_q.shape[0] - 1, rows, rows_k, hq, hkv, d, _i64(sq), _i64(sk), _i64(sv), _i64(sg), scale)
         else:
             for t in (dq, dk, dv):
@@ -294,7 +295,7 @@ def _decay_forward(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, cu: Tenso
     states = ws = None
     if rows:
         P = _hip.ptr
-        n = _hip.load_library().genie_decay_attention_state_elems(nseq, rows, h, dk, dv, initial_state is not None or return_state)
+        n = _hip.load_library().genie_decay_attention_state_elems(nseq, rows, h, dk, dv, initial_state is not None)
         if n:
             states, ws = torch.empty(n, dtype=torch.bfloat16, device=dev), torch.empty(n, dtype=torch.float32, device=dev)
         _launch('genie_decay_attention_fwd', dev, P(q), P(k), P(v), P(log_decay), P(cu), P(initial_state), P(out), P(final), P(states), P(ws), n, nseq, rows, h, dk, dv,

@@ -86,7 +86,7 @@ def test_c_entries_refuse_before_any_device_work():
     two = _hip.i64((512, 64))
 
     def packed(hq=8, hkv=2, dim=64, strides=two, q=16, scale=1.0):
-        rc = lib.genie_packed_attention_fwd(q, 16, 16, 16, None, 16, 16, 1, 4, 4, hq, hkv, dim, strides, two, two, scale, None)
+        rc = lib.genie_packed_attention_fwd(q, 16, 16, 16, None, None, 16, 16, 1, 4, 4, hq, hkv, dim, strides, two, two, scale, None)
         return rc, lib.genie_last_error()
 
     assert packed(hkv=3)[0] == -1 and b'no multiple' in packed(hkv=3)[1]
@@ -96,11 +96,11 @@ def test_c_entries_refuse_before_any_device_work():
     assert packed(strides=_hip.i64((1 << 21, 64)))[0] == -1 and b'row stride' in packed(strides=_hip.i64((1 << 21, 64)))[1]
     assert packed(q=None)[0] == -1 and b'null pointer' in packed(q=None)[1]
     assert packed(scale=0.0)[0] == -1 and packed(scale=float('nan'))[0] == -1
-    rc = lib.genie_packed_attention_bwd(*([16] * 7), 1 << 20, *([16] * 4), None, 1, 4, 4, 8, 2, 64, two, two, two, two, 1.0, None)
+    rc = lib.genie_packed_attention_bwd(*([16] * 8), 1 << 20, *([16] * 4), None, 1, 4, 4, 8, 2, 64, two, two, two, two, 1.0, None)
     assert rc == -1 and b'null pointer' in lib.genie_last_error()
     need = lib.genie_packed_attention_bwd_ws_floats(1, 4096, 4096, 8, 2, 64)
     assert need > 8 * 4096
-    rc = lib.genie_packed_attention_bwd(*([16] * 7), need - 1, *([16] * 5), 1, 4096, 4096, 8, 2, 64, two, two, two, two, 1.0, None)
+    rc = lib.genie_packed_attention_bwd(*([16] * 8), need - 1, *([16] * 5), 1, 4096, 4096, 8, 2, 64, two, two, two, two, 1.0, None)
     assert rc == -1 and b'workspace' in lib.genie_last_error()
     three = _hip.i64((8192, 512, 64))
     assert lib.genie_cached_attention_step(16, 16, None, 16, 16, 16, 16, None, 0, 1, 8, 2, 64, 16, two, two, two, three, three, 1.0, None) == -1
