@@ -4,14 +4,12 @@
 //
 // Bound by reading K and V once: 4 n Hkv D bytes against 4 n Hq D operations.  The query heads that share a key head are the 16 columns of one
 // 16x16x32 product, so a cache row is read once for all of them and the vector units do no dot products; a wave walks 32-key tiles on its own --
-// K straight into operand registers, V through its private LDS tile for the transposing read, the next tile's loads in flight meanwhile -- and there is
-// no barrier in the key loop.  Where batch x key heads do not fill the chip, short caches get blocks of more waves (their parts meet in LDS), long ones are
+// loaded as whole rows, K and then V through its private LDS tile into operand layout, the next tile's loads in flight from the first product on -- and there is
+// no barrier in the key loop.  (64 sequences of up to 8191 keys, 4 key heads of width 128, 512 MB: 91 us = 5.6 TB/s;
+// with K straight into operand registers, 64 B of each of 16 rows per load, 104; without the non-temporal hint 102; parts joined in another 5.)  Where batch x key heads do not fill the chip, short caches get blocks of more waves (their parts meet in LDS), long ones are
 // split over blocks, and a second small kernel joins the parts (maximum, sum, unnormalised fp32 output) in a fixed order.  Lengths are read on the device: a captured graph replays with the lengths of the day.
 #include "seq_common.h"
 #include "genie_hip.h"
-#ifndef CACHED_NT
-#define CACHED_NT true
-#endif
 
 struct CachedArgs {
     const bf16_t *q, *k_new, *v_new;
@@ -59,20 +57,22 @@ __global__ void __launch_bounds__(64 * NW, DH <= 64 ? 4 : 2) cached_step_kernel(
     }
     const float c2 = a.scale * 1.4426950408889634f;
     char* vt = smem + wave * WREG;
-    uint32_t koff[2][KS], voff[VP], vlds[VP];
+    // a tile's rows in 16-B pieces, 64 / CPR rows per load; K and V have their own row strides.  Where whole rows fill a load (EVEN) a lane's pieces lie in one column a
+    // constant number of rows apart, and one register of each kind is enough: the swizzle's key of row r + R i is that of r with the key of R i flipped in.
+    constexpr bool EVEN = 64 % CPR == 0;
+    constexpr int R = 64 / CPR, NO = EVEN ? 1 : VP;
+    uint32_t koff[NO], voff[NO], lds[NO];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-            const int d = ks * 32 + g * 8;
-            koff[kt][ks] = d < a.dim ? (uint32_t)((kt * 16 + col) * a.k_t * 2) + d * 2 : SEQ_OOB;
-        }
-#pragma unroll
-    for (int i = 0; i < VP; ++i) {
+    for (int i = 0; i < NO; ++i) {
         const int idx = i * 64 + lane, row = idx / CPR, c = idx % CPR;
+        koff[i] = c * 8 < a.dim ? (uint32_t)(row * a.k_t * 2) + c * 16 : SEQ_OOB;
         voff[i] = c * 8 < a.dim ? (uint32_t)(row * a.v_t * 2) + c * 16 : SEQ_OOB;
-        vlds[i] = (uint32_t)(row * PITCH + (attn_swz<SW>(row, c) << 4));
+        lds[i] = (uint32_t)(row * PITCH + (attn_swz<SW>(row, c) << 4));
     }
+    auto lds_at = [&](int i) { return EVEN ? (lds[0] ^ (uint32_t)(attn_swz<SW>(i * R, 0) << 4)) + i * R * PITCH : lds[EVEN ? 0 : i]; };
+    auto koff_at = [&](int i) { return EVEN ? koff[0] + (uint32_t)(i * R * (int)a.k_t * 2) : koff[EVEN ? 0 : i]; };      // (SEQ_OOB plus a tile stays out of range)
+    auto voff_at = [&](int i) { return EVEN ? voff[0] + (uint32_t)(i * R * (int)a.v_t * 2) : voff[EVEN ? 0 : i]; };
+    const uint32_t roff = (uint32_t)(col * PITCH + (attn_swz<SW>(col, g) << 4));   // operand fragment of a row: chunk 4 ks + g is this with bits 6.. flipped
     uint32_t toff[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
@@ -85,21 +85,33 @@ __global__ void __launch_bounds__(64 * NW, DH <= 64 ? 4 : 2) cached_step_kernel(
     for (int d = 0; d < DT; ++d) acc[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     float m_run = -INFINITY, mc = 0.f, l_run = 0.f;
 
-    // one tile of up to 32 keys: K in kr, V in vr; `live` keys exist
-    auto tile = [&](const u32x4_t (&kr)[2][KS], const u32x4_t (&vr)[VP], int live) {
+    u32x4_t kr[VP], vr[VP];
+    // scores of the up to 32 keys in kr (`live` of them exist); V to LDS behind them: kr and vr are free then.  (LDS serves a wave's accesses in order: K's
+    // fragments are read before V overwrites them.)
+    auto scores = [&](f32x4_t (&s)[2], int live) {
 #pragma unroll
-        for (int i = 0; i < VP; ++i) *reinterpret_cast<u32x4_t*>(vt + vlds[i]) = vr[i];
-        f32x4_t s[2] = {f32x4_t{0.f, 0.f, 0.f, 0.f}, f32x4_t{0.f, 0.f, 0.f, 0.f}};
+        for (int i = 0; i < VP; ++i) *reinterpret_cast<u32x4_t*>(vt + lds_at(i)) = kr[i];
+        bf16x8_t kf[2][KS];
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt) s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kr[kt][ks]), qf[ks], s[kt], 0, 0, 0);
+            for (int kt = 0; kt < 2; ++kt) kf[kt][ks] = *reinterpret_cast<const bf16x8_t*>(vt + kt * 16 * PITCH + (roff ^ (uint32_t)(ks * 64)));
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int i = 0; i < VP; ++i) *reinterpret_cast<u32x4_t*>(vt + lds_at(i)) = vr[i];
+        s[0] = s[1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[kt][ks], qf[ks], s[kt], 0, 0, 0);
         if (live < 32) {
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[kt][e] = kt * 16 + 4 * g + e < live ? s[kt][e] : -INFINITY;
         }
+    };
+    auto weigh = [&](const f32x4_t (&s)[2]) {
         float p[8], ps;
         bool with_max = m_run == -INFINITY;                                     // (the same in the four lanes of a column; decided for the wave below)
         for (;;) {
@@ -138,17 +150,16 @@ __global__ void __launch_bounds__(64 * NW, DH <= 64 ? 4 : 2) cached_step_kernel(
     const int tiles = (n + 31) >> 5, per = (tiles + a.nsplit - 1) / a.nsplit, t_end = min(tiles, (split + 1) * per);
     const bf16_t* kb = a.kc + b * a.k_b + kvh * a.k_h;
     const bf16_t* vb = a.vc + b * a.v_b + kvh * a.v_h;
-    u32x4_t kr[2][KS], vr[VP];
     auto load = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < NO; ++i) asm volatile("" : "+v"(koff[i]), "+v"(voff[i]), "+v"(lds[i]));      // (derived offsets are formed anew)
         const bf16_t* kp = kb + (int64_t)t * 32 * a.k_t;
         const bf16_t* vp = vb + (int64_t)t * 32 * a.v_t;
         const int kl = seq_bytes_left(n - t * 32, a.k_t * 2, a.dim), vl = seq_bytes_left(n - t * 32, a.v_t * 2, a.dim);
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+        for (int i = 0; i < VP; ++i) kr[i] = seq_load16<true>(kp, kl, koff_at(i));
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) kr[kt][ks] = seq_load16<CACHED_NT>(kp, kl, koff[kt][ks]);
-#pragma unroll
-        for (int i = 0; i < VP; ++i) vr[i] = seq_load16<CACHED_NT>(vp, vl, voff[i]);
+        for (int i = 0; i < VP; ++i) vr[i] = seq_load16<true>(vp, vl, voff_at(i));
     };
     if (append && split == 0 && wave == NW - 1 && !bad && !idle) {
         // the new token, in the wave with the fewest tiles: a tile of one key, taken from the arguments and put into the cache by the same lanes (no other lane of this launch reads that row)
@@ -157,37 +168,30 @@ __global__ void __launch_bounds__(64 * NW, DH <= 64 ? 4 : 2) cached_step_kernel(
         bf16_t* kd = a.kc + b * a.k_b + kvh * a.k_h + (int64_t)n * a.k_t;
         bf16_t* vd = a.vc + b * a.v_b + kvh * a.v_h + (int64_t)n * a.v_t;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            kr[0][ks] = kr[1][ks] = u32x4_t{0, 0, 0, 0};
-            const int d = ks * 32 + g * 8;
-            if (col == 0 && d < a.dim) {
-                kr[0][ks] = *reinterpret_cast<const u32x4_t*>(kp + d);
-                if (hg == 0) *reinterpret_cast<u32x4_t*>(kd + d) = kr[0][ks];
-            }
-        }
-#pragma unroll
         for (int i = 0; i < VP; ++i) {
             const int idx = i * 64 + lane, row = idx / CPR, c = idx % CPR;
-            vr[i] = u32x4_t{0, 0, 0, 0};
+            kr[i] = vr[i] = u32x4_t{0, 0, 0, 0};
             if (row == 0 && c * 8 < a.dim) {
+                kr[i] = *reinterpret_cast<const u32x4_t*>(kp + c * 8);
                 vr[i] = *reinterpret_cast<const u32x4_t*>(vp + c * 8);
-                if (hg == 0) *reinterpret_cast<u32x4_t*>(vd + c * 8) = vr[i];
+                if (hg == 0) {
+                    *reinterpret_cast<u32x4_t*>(kd + c * 8) = kr[i];
+                    *reinterpret_cast<u32x4_t*>(vd + c * 8) = vr[i];
+                }
             }
         }
-        tile(kr, vr, 1);
+        f32x4_t s[2];
+        scores(s, 1);
+        weigh(s);
     }
     int t = split * per + wave;
     if (t < t_end) load(t);
     while (t < t_end) {
-        u32x4_t kc[2][KS], vc[VP];
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) { kc[0][ks] = kr[0][ks]; kc[1][ks] = kr[1][ks]; }
-#pragma unroll
-        for (int i = 0; i < VP; ++i) vc[i] = vr[i];
-        const int live = min(32, n - t * 32);
+        f32x4_t s[2];
+        scores(s, min(32, n - t * 32));
         t += NW;
-        if (t < t_end) load(t);
-        tile(kc, vc, live);
+        if (t < t_end) load(t);                                                 // in flight under the exponentials and the second product
+        weigh(s);
     }
     // the waves' parts: maxima, sums, outputs through LDS
     l_run += __shfl_xor(l_run, 16);
@@ -279,16 +283,13 @@ __global__ void __launch_bounds__(256) cached_join_kernel(const CachedArgs a) {
     }
 }
 
-#ifndef CACHED_BLOCKS
-#define CACHED_BLOCKS 2048
-#endif
 // waves of a block that takes a whole short cache, four tiles of 32 keys each
 static int cached_wide(int dim) { return dim <= 64 ? 16 : 8; }
 // parts of the key axis (0: one part, a wide block)
 static int cached_splits(int batch, int hq, int hkv, int dim, int cap) {
     const int64_t base = (int64_t)batch * hkv * ((hq / hkv + 15) / 16);
     if (base < 512 && cap <= 128 * cached_wide(dim)) return 0;
-    int64_t n = base > 0 ? (CACHED_BLOCKS + base - 1) / base : 1;
+    int64_t n = base > 0 ? (2048 + base - 1) / base : 1;
     const int64_t most = (cap + 127) / 128;
     n = n < most ? n : most;
     return (int)(n < 1 ? 1 : n > 128 ? 128 : n);
