@@ -258,36 +258,59 @@ __global__ void __launch_bounds__(256) decay_scan_kernel(const DecayArgs g) {
     for (int j = 0; j < 4; ++j) R.final_state[of_seq + (a + j) * R.dc + c] = m[j];
 }
 
-// A pair of 64-row tiles straight into LDS, as PackedDma, for tokens walked in either direction (reverse: row i is token nv - 1 - i from the base; the rows behind
-// the nv-th wrap past any range).
+// 32 rows straight into LDS, as PackedDma, for tokens walked in either direction (last >= 0: row i is token last - i from the base; rows behind the walk's end wrap
+// past any range).
 template <int DH>
 struct DecayDma {
     using G = PackedGeo<DH>;
-    static constexpr int SLABS = G::TILE / 1024 / 4, ROWS = 1024 / G::PITCH;
+    static constexpr int SLABS = 32 * G::PITCH / 1024 / 4, ROWS = 1024 / G::PITCH;
     int row0, slot;
     __device__ __forceinline__ void init(int wave, int lane) { row0 = wave * SLABS * ROWS + lane / G::SW; slot = lane % G::SW; }
-    __device__ __forceinline__ void load(int wave, char* tile, const bf16_t* base, int64_t stride, int rows, int dim, int rev_last) {
+    __device__ __forceinline__ void load(int wave, char* tile, const bf16_t* base, int64_t stride, int rows, int dim, int last) {
         asm volatile("" : "+v"(row0), "+v"(slot));                              // (offsets are formed anew: registers are short)
         const int left = seq_bytes_left(rows, stride * 2, dim);
         const uint32_t pitch = (uint32_t)(stride * 2);
 #pragma unroll
         for (int i = 0; i < SLABS; ++i) {
             const int row = row0 + i * ROWS, c = attn_swz<G::SW>(row, slot);
-            const uint32_t o = (uint32_t)(rev_last >= 0 ? rev_last - row : row) * pitch + c * 16;
+            const uint32_t o = (uint32_t)(last >= 0 ? last - row : row) * pitch + c * 16;
             seq_dma16(base, left, tile + (wave * SLABS + i) * 1024, c * 8 < dim ? o : SEQ_OOB);
         }
     }
 };
 
-#ifndef DECAY_OUT_WPE64
-#define DECAY_OUT_WPE64 3
-#endif
-// All outputs of one role: four waves of 32 rows, the state in front of the segment as tile pair 0 of the walk, the segment's keys after it.
+// acc[d] += (transposed 32-row tile, columns 32 d ..) x p, d = 0 ..: the reads and their wait in asm blocks where two columns make one (the loads in flight stay there)
 template <int DH>
-__global__ void __launch_bounds__(256, DH <= 64 ? DECAY_OUT_WPE64 : 2) decay_out_kernel(const DecayArgs g) {
+__device__ __forceinline__ void decay_tr_product(f32x16_t (&acc)[PackedGeo<DH>::DT], const PackedLane<DH>& at, const char* tile, const bf16x8_t (&p)[2]) {
     using G = PackedGeo<DH>;
-    constexpr int BM = 128;
-    extern __shared__ __attribute__((aligned(16))) char smem[];
+    if constexpr (G::DT % 2 == 0) {
+        const uint32_t base = attn_lds_offset(tile);
+#pragma unroll
+        for (int d = 0; d < G::DT; d += 2) {
+            bf16x8_t f[4];
+            seq_tr16x4<0, 16 * G::PITCH>(f, base + (at.tr0 ^ (uint32_t)(d * 64)), base + (at.tr1 ^ (uint32_t)(d * 64)), base + (at.tr0 ^ (uint32_t)(d * 64 + 64)),
+                                         base + (at.tr1 ^ (uint32_t)(d * 64 + 64)));
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) acc[d + e] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[2 * s2 + e], p[s2], acc[d + e], 0, 0, 0);
+        }
+    } else {
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+            for (int d = 0; d < G::DT; ++d) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at.tr_frag(tile + s2 * 16 * G::PITCH, d), p[s2], acc[d], 0, 0, 0);
+    }
+}
+
+// All outputs of one role: four waves of 32 rows; the state in front of the segment, then the segment's keys, 32 at a time, pass through a ring of three LDS stages,
+// two ahead (counted waits).  A block is short -- 4 or 8 key tiles -- and lives on memory latency: stages of 32 keys and the fade table in LDS make three blocks
+// fit a CU (48 KB, 168 registers) at head width 128.
+template <int DH>
+__global__ void __launch_bounds__(256, DH <= 64 ? 4 : 3) decay_out_kernel(const DecayArgs g) {
+    using G = PackedGeo<DH>;
+    constexpr int BM = 128, STAGE = 64 * G::PITCH, MINE = 2 * DecayDma<DH>::SLABS;      // MINE: loads of a wave per stage
+    __shared__ __attribute__((aligned(16))) char smem[3 * STAGE + 128];
     const DecayRole& R = g.r[blockIdx.y];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int head = (int)blockIdx.x % g.heads, slot = (int)blockIdx.x / g.heads;
@@ -301,41 +324,40 @@ __global__ void __launch_bounds__(256, DH <= 64 ? DECAY_OUT_WPE64 : 2) decay_out
     const int q0 = r0 + wave * 32, qi = q0 + (lane & 31);                        // rows in the order of the walk
     const float log2_l = g.log_decay[head] * 1.4426950408889634f;
     const bool carried = R.states && (seg > 0 || R.initial);                     // M is not zero
-    const int tiles = (end - seg0 + 63) >> 6;
+    const int tiles = (end - seg0 + 31) >> 5;
 
     const bf16_t* arow = R.a + (int64_t)(s.start + (rev ? s.len - 1 - qi : qi)) * R.a_row + head * R.a_head;
     const bf16_t* bp = R.b + (int64_t)s.start * R.b_row + head * R.b_head;
     const bf16_t* cp = R.c + (int64_t)s.start * R.c_row + head * R.c_head;
     DecayDma<DH> st;
     st.init(wave, lane);
-    auto load = [&](int t) {                                                     // t = -1: the state; 0 ..: keys
-        char* to = smem + ((t + 1) & 1) * 2 * G::TILE;
-        if (t < 0) {
-            const int mr = R.m_rows_a ? R.da : R.dc, mc = R.m_rows_a ? R.dc : R.da;
-            const bf16_t* m = R.states + ((int64_t)(s.start / DECAY_SEG + s.seq + seg) * g.heads + head) * mr * mc;
-            st.load(wave, to, m, mc, min(64, mr), mc, -1);
-            if (DH > 64) st.load(wave, to + G::TILE, m + 64 * mc, mc, mr - 64, mc, -1);
-            return;
-        }
-        const int p = seg0 + t * 64, nv = min(64, s.len - p), from = rev ? s.len - p - nv : p;
+    auto stage = [&](int t) { return smem + (t + 2) % 3 * STAGE; };
+    auto load = [&](int t) {
+        char* to = stage(t);
+        const int p = seg0 + t * 32, nv = min(32, s.len - p), from = rev ? s.len - p - nv : p;
         st.load(wave, to, bp + (int64_t)from * R.b_row, R.b_row, nv, R.da, rev ? nv - 1 : -1);
-        st.load(wave, to + G::TILE, cp + (int64_t)from * R.c_row, R.c_row, nv, R.dc, rev ? nv - 1 : -1);
+        st.load(wave, to + STAGE / 2, cp + (int64_t)from * R.c_row, R.c_row, nv, R.dc, rev ? nv - 1 : -1);
     };
-    if (carried) load(-1);
-    load(0);                                                                    // both buffers are free
-    bf16x8_t af[G::KS];
+    bf16x8_t af[G::KS];                                                          // (in front of the tiles' loads: the counted waits below count what is younger)
     packed_row_frags<DH>(af, arow, qi < s.len, R.da);
+    if (carried) {                                                               // the state: stages 0 and 1
+        const int mr = R.m_rows_a ? R.da : R.dc, mc = R.m_rows_a ? R.dc : R.da;
+        const bf16_t* m = R.states + ((int64_t)(s.start / DECAY_SEG + s.seq + seg) * g.heads + head) * mr * mc;
+#pragma unroll
+        for (int i = 0; i < G::DT; ++i) st.load(wave, smem + i * 32 * G::PITCH, m + i * 32 * mc, mc, mr - i * 32, mc, -1);
+    }
+    load(0);
+    if (!carried && tiles > 1) load(1);
     PackedLane<DH> at;
     at.init(lane);
-    float fade[16];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) fade[r] = decay_pow(log2_l, 31 - (seq_crow(r) + 4 * h));
+    float* fade = reinterpret_cast<float*>(smem + 3 * STAGE);                     // [h][r]: l^(31 - row r of a 32-row half)
+    if (tid < 32) fade[tid] = decay_pow(log2_l, 31 - ((tid & 3) + 8 * (tid >> 2 & 3) + 4 * (tid >> 4)));
     f32x16_t y[G::DT];
 #pragma unroll
     for (int d = 0; d < G::DT; ++d) y[d] = packed_splat(0.f);
 
     if (carried) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(MINE) : "memory");
         __syncthreads();
         if (!R.m_rows_a) {
 #pragma unroll
@@ -345,14 +367,17 @@ __global__ void __launch_bounds__(256, DH <= 64 ? DECAY_OUT_WPE64 : 2) decay_out
         } else {
             // the transposing read delivers columns of a in the accumulator order: this lane's row again, 4 + 4 values at a time
 #pragma unroll
-            for (int ks = 0; ks < G::KS; ++ks) {
-                u32x2_t lo = {0, 0}, hi = {0, 0};
-                const int col = ks * 16 + 4 * h;
-                if (qi < s.len && col < R.da) lo = *reinterpret_cast<const u32x2_t*>(arow + col);
-                if (qi < s.len && col + 8 < R.da) hi = *reinterpret_cast<const u32x2_t*>(arow + col + 8);
-                const bf16x8_t ap = __builtin_bit_cast(bf16x8_t, u32x4_t{lo[0], lo[1], hi[0], hi[1]});
+            for (int k2 = 0; k2 < G::KS; k2 += 2) {
+                bf16x8_t ap[2];
 #pragma unroll
-                for (int d = 0; d < G::DT; ++d) y[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at.tr_frag(smem + ks * 16 * G::PITCH, d), ap, y[d], 0, 0, 0);
+                for (int e = 0; e < 2; ++e) {
+                    u32x2_t lo = {0, 0}, hi = {0, 0};
+                    const int col = (k2 + e) * 16 + 4 * h;
+                    if (qi < s.len && col < R.da) lo = *reinterpret_cast<const u32x2_t*>(arow + col);
+                    if (qi < s.len && col + 8 < R.da) hi = *reinterpret_cast<const u32x2_t*>(arow + col + 8);
+                    ap[e] = __builtin_bit_cast(bf16x8_t, u32x4_t{lo[0], lo[1], hi[0], hi[1]});
+                }
+                decay_tr_product<DH>(y, at, smem + k2 * 16 * G::PITCH, ap);
             }
         }
         const float lead = decay_pow(log2_l, qi - seg0 + 1);
@@ -360,56 +385,44 @@ __global__ void __launch_bounds__(256, DH <= 64 ? DECAY_OUT_WPE64 : 2) decay_out
         for (int d = 0; d < G::DT; ++d)
 #pragma unroll
             for (int r = 0; r < 16; ++r) y[d][r] *= lead;
+        if (tiles > 1) {
+            __syncthreads();                                                     // everybody is done with the state
+            load(1);
+        }
     }
     for (int t = 0; t < tiles; ++t) {
-        char* bt = smem + ((t + 1) & 1) * 2 * G::TILE;
-        char* ct = bt + G::TILE;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        char* bt = stage(t);
+        char* ct = bt + STAGE / 2;
+        if (t + 1 < tiles) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(MINE) : "memory");      // tile t has landed, t + 1 is in flight
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (t + 1 < tiles) load(t + 1);
+        if (t + 2 < tiles) load(t + 2);
+        const int k0 = seg0 + t * 32;
+        if (k0 > q0) continue;                                                   // (wave-uniform) behind this wave's rows
         at.forget();
-#pragma unroll 1
-        for (int kt = 0; kt < 2; ++kt) {
-            const int k0 = seg0 + t * 64 + kt * 32;
-            if (k0 > q0) break;                                                  // (wave-uniform) behind this wave's rows
-            f32x16_t x = packed_splat(0.f);
+        f32x16_t x = packed_splat(0.f);
 #pragma unroll
-            for (int ks = 0; ks < G::KS; ++ks) x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at.row_frag(bt + kt * 32 * G::PITCH, ks), af[ks], x, 0, 0, 0);
-            if (k0 == q0) {                                                      // the diagonal: l^(t-s) for s <= t
+        for (int ks = 0; ks < G::KS; ++ks) x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at.row_frag(bt, ks), af[ks], x, 0, 0, 0);
+        if (k0 == q0) {                                                          // the diagonal: l^(t-s) for s <= t
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int d = (lane & 31) - (seq_crow(r) + 4 * h);
-                    x[r] = d >= 0 ? x[r] * decay_pow(log2_l, max(0, d)) : 0.f;
-                }
-            } else {                                                             // l^(t-s) = l^(31 - s) l^(t + 1 + distance of the tiles - 32)
-                const float f = decay_pow(log2_l, (lane & 31) + 1 + q0 - k0 - 32);
-#pragma unroll
-                for (int r = 0; r < 16; ++r) x[r] *= fade[r] * f;
+            for (int r = 0; r < 16; ++r) {
+                const int d = (lane & 31) - (seq_crow(r) + 4 * h);
+                x[r] = d >= 0 ? x[r] * decay_pow(log2_l, max(0, d)) : 0.f;
             }
-            bf16x8_t pf[2];
+        } else {                                                                 // l^(t-s) = l^(31 - s) l^(t + 1 + distance of the tiles - 32)
+            const float f = decay_pow(log2_l, (lane & 31) + 1 + q0 - k0 - 32);
 #pragma unroll
-            for (int s2 = 0; s2 < 2; ++s2)
-                pf[s2] = seq_pack8(x[8 * s2], x[8 * s2 + 1], x[8 * s2 + 2], x[8 * s2 + 3], x[8 * s2 + 4], x[8 * s2 + 5], x[8 * s2 + 6], x[8 * s2 + 7]);
-            const char* ck = ct + kt * 32 * G::PITCH;
-            if constexpr (G::DT % 2 == 0) {                                      // (the next tiles' DMA stays in flight)
-                const uint32_t base = attn_lds_offset(ck);
+            for (int q = 0; q < 4; ++q) {
+                const f32x4_t w = *reinterpret_cast<const f32x4_t*>(fade + 16 * h + 4 * q);
 #pragma unroll
-                for (int d = 0; d < G::DT; d += 2) {
-                    bf16x8_t f[4];
-                    seq_tr16x4<0, 16 * G::PITCH>(f, base + (at.tr0 ^ (uint32_t)(d * 64)), base + (at.tr1 ^ (uint32_t)(d * 64)), base + (at.tr0 ^ (uint32_t)(d * 64 + 64)),
-                                                 base + (at.tr1 ^ (uint32_t)(d * 64 + 64)));
-#pragma unroll
-                    for (int s2 = 0; s2 < 2; ++s2)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) y[d + e] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[2 * s2 + e], pf[s2], y[d + e], 0, 0, 0);
-                }
-            } else {
-#pragma unroll
-                for (int s2 = 0; s2 < 2; ++s2)
-#pragma unroll
-                    for (int d = 0; d < G::DT; ++d) y[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at.tr_frag(ck + s2 * 16 * G::PITCH, d), pf[s2], y[d], 0, 0, 0);
+                for (int e = 0; e < 4; ++e) x[4 * q + e] *= w[e] * f;
             }
         }
+        bf16x8_t pf[2];
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2)
+            pf[s2] = seq_pack8(x[8 * s2], x[8 * s2 + 1], x[8 * s2 + 2], x[8 * s2 + 3], x[8 * s2 + 4], x[8 * s2 + 5], x[8 * s2 + 6], x[8 * s2 + 7]);
+        decay_tr_product<DH>(y, at, ct, pf);
     }
     __syncthreads();
     if (q0 < s.len) {
@@ -526,7 +539,7 @@ static int decay_run(const DecayArgs& g, int roles, void* stream) {
         hipLaunchKernelGGL(decay_scan_kernel, grid, dim3(256), 0, (hipStream_t)stream, g);
         GENIE_CHECK_LAUNCH();
     }
-    hipLaunchKernelGGL(decay_out_kernel<DH>, dim3((unsigned)blocks, roles), dim3(256), 4 * PackedGeo<DH>::TILE, (hipStream_t)stream, g);
+    hipLaunchKernelGGL(decay_out_kernel<DH>, dim3((unsigned)blocks, roles), dim3(256), 0, (hipStream_t)stream, g);
     GENIE_CHECK_LAUNCH();
     return GENIE_OK;
 }
