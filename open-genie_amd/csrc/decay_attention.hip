@@ -35,7 +35,7 @@ struct DecayArgs {
     DecayRole r[3];
     const int32_t* cu;
     const float* log_decay;
-    int nseq, rows, heads;
+    int nseq, rows, heads, roles;
     float scale;
 };
 
@@ -311,9 +311,10 @@ __global__ void __launch_bounds__(256, DH <= 64 ? 4 : 3) decay_out_kernel(const 
     using G = PackedGeo<DH>;
     constexpr int BM = 128, STAGE = 64 * G::PITCH, MINE = 2 * DecayDma<DH>::SLABS;      // MINE: loads of a wave per stage
     __shared__ __attribute__((aligned(16))) char smem[3 * STAGE + 128];
-    const DecayRole& R = g.r[blockIdx.y];
+    // heads fastest, then roles: the roles read the same tensors (and two of them the same tiles), and with a multiple of 8 heads those blocks share an XCD's L2
+    const int head = (int)blockIdx.x % g.heads, role = (int)blockIdx.x / g.heads % g.roles, slot = (int)blockIdx.x / g.heads / g.roles;
+    const DecayRole& R = g.r[role];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-    const int head = (int)blockIdx.x % g.heads, slot = (int)blockIdx.x / g.heads;
     const SeqSlot s = seq_find<BM>(g.cu, g.nseq, g.rows, slot);
     if (s.tile < 0 || s.tile * BM >= s.len) return;
     if (s.seq == g.nseq) {
@@ -525,12 +526,12 @@ static int decay_check_role(const char* what, const DecayRole& r) {
 
 // role 0's states, then all roles' outputs
 template <int DH>
-static int decay_run(const DecayArgs& g, int roles, void* stream) {
-    const int64_t segs = (int64_t)(g.rows / DECAY_SEG + g.nseq + 1) * g.heads, blocks = (int64_t)(g.rows / 128 + g.nseq + 1) * g.heads;
+static int decay_run(const DecayArgs& g, void* stream) {
+    const int64_t segs = (int64_t)(g.rows / DECAY_SEG + g.nseq + 1) * g.heads, blocks = (int64_t)(g.rows / 128 + g.nseq + 1) * g.heads * g.roles;
     GENIE_CHECK_ARG(segs < (1ll << 31) && blocks < (1ll << 31), "decay attention: too many blocks");
     const DecayRole& r = g.r[0];
     if (g.nseq > 0 && (r.local || r.final_state)) {
-        auto* kernel = !r.local ? decay_state_kernel<DH, 3, true> : roles == 1 ? decay_state_kernel<DH, 3, false> : decay_state_kernel<DH, 2, false>;
+        auto* kernel = !r.local ? decay_state_kernel<DH, 3, true> : g.roles == 1 ? decay_state_kernel<DH, 3, false> : decay_state_kernel<DH, 2, false>;
         hipLaunchKernelGGL(kernel, dim3((unsigned)segs), dim3(DecayGeo<DH>::NT), 0, (hipStream_t)stream, g);
         GENIE_CHECK_LAUNCH();
     }
@@ -539,16 +540,16 @@ static int decay_run(const DecayArgs& g, int roles, void* stream) {
         hipLaunchKernelGGL(decay_scan_kernel, grid, dim3(256), 0, (hipStream_t)stream, g);
         GENIE_CHECK_LAUNCH();
     }
-    hipLaunchKernelGGL(decay_out_kernel<DH>, dim3((unsigned)blocks, roles), dim3(256), 0, (hipStream_t)stream, g);
+    hipLaunchKernelGGL(decay_out_kernel<DH>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, g);
     GENIE_CHECK_LAUNCH();
     return GENIE_OK;
 }
-static int decay_run_any(const DecayArgs& g, int roles, void* stream) {
+static int decay_run_any(const DecayArgs& g, void* stream) {
     const int d = g.r[0].da > g.r[0].dc ? g.r[0].da : g.r[0].dc;
-    if (d <= 32) return decay_run<32>(g, roles, stream);
-    if (d <= 64) return decay_run<64>(g, roles, stream);
-    if (d <= 96) return decay_run<96>(g, roles, stream);
-    return decay_run<128>(g, roles, stream);
+    if (d <= 32) return decay_run<32>(g, stream);
+    if (d <= 64) return decay_run<64>(g, stream);
+    if (d <= 96) return decay_run<96>(g, stream);
+    return decay_run<128>(g, stream);
 }
 
 extern "C" int genie_decay_attention_fwd(const void* q, const void* k, const void* v, const float* log_decay, const int32_t* cu, const float* initial_state, void* out,
@@ -569,7 +570,8 @@ extern "C" int genie_decay_attention_fwd(const void* q, const void* k, const voi
     const int64_t need = genie_decay_attention_state_elems(nseq, rows, heads, dk, dv, initial_state != nullptr);
     GENIE_CHECK_ARG(state_elems >= need && (need == 0 || (states && ws)), "%s: workspace too small", what);
     if (need == 0) { r.states = nullptr; r.local = nullptr; }
-    return decay_run_any(g, 1, stream);
+    g.roles = 1;
+    return decay_run_any(g, stream);
 }
 
 extern "C" int genie_decay_attention_bwd(const void* q, const void* k, const void* v, const void* dout, const float* log_decay, const int32_t* cu, int has_initial,
@@ -601,7 +603,8 @@ extern "C" int genie_decay_attention_bwd(const void* q, const void* k, const voi
     const int64_t need = genie_decay_attention_state_elems(nseq, rows, heads, dk, dv, 0);
     GENIE_CHECK_ARG(state_elems >= need && (need == 0 || (states && rev_states && ws)) && (!has_initial || states), "%s: workspace too small", what);
     if (need > 0) { rv.states = rk.states = (bf16_t*)rev_states; rv.local = ws; }
-    return decay_run_any(g, 3, stream);
+    g.roles = 3;
+    return decay_run_any(g, stream);
 }
 
 extern "C" int genie_decay_attention_step(const void* q, const void* k, const void* v, const float* log_decay, const float* state, float* new_state, void* out, int batch,
