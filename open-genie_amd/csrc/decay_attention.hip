@@ -366,17 +366,15 @@ __global__ void __launch_bounds__(256, DH <= 64 ? 4 : 3) decay_out_kernel(const 
 #pragma unroll
                 for (int d = 0; d < G::DT; ++d) y[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at.row_frag(smem + d * 32 * G::PITCH, ks), af[ks], y[d], 0, 0, 0);
         } else {
-            // the transposing read delivers columns of a in the accumulator order: this lane's row again, 4 + 4 values at a time
+            // the transposing read delivers columns of a in the accumulator order, 4 h .. + 3 and 8 + 4 h .. + 3 of 16; af holds 8 h .. + 7: the lanes of a row trade halves
 #pragma unroll
             for (int k2 = 0; k2 < G::KS; k2 += 2) {
                 bf16x8_t ap[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    u32x2_t lo = {0, 0}, hi = {0, 0};
-                    const int col = (k2 + e) * 16 + 4 * h;
-                    if (qi < s.len && col < R.da) lo = *reinterpret_cast<const u32x2_t*>(arow + col);
-                    if (qi < s.len && col + 8 < R.da) hi = *reinterpret_cast<const u32x2_t*>(arow + col + 8);
-                    ap[e] = __builtin_bit_cast(bf16x8_t, u32x4_t{lo[0], lo[1], hi[0], hi[1]});
+                    const u32x4_t f = __builtin_bit_cast(u32x4_t, af[k2 + e]);
+                    const auto x = __builtin_amdgcn_permlane32_swap(f[0], f[2], false, false), z = __builtin_amdgcn_permlane32_swap(f[1], f[3], false, false);
+                    ap[e] = __builtin_bit_cast(bf16x8_t, u32x4_t{x[0], z[0], x[1], z[1]});
                 }
                 decay_tr_product<DH>(y, at, smem + k2 * 16 * G::PITCH, ap);
             }
