@@ -139,11 +139,14 @@ __global__ void __launch_bounds__(64 * NW, DH <= 64 ? 4 : 2) cached_step_kernel(
             with_max = true;
         }
         l_run += ps;
-        const bf16x8_t pf = seq_pack8(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]);
+        // P and what its rounding left over: the second product hides behind the loads, and no rounding but the output's is left
+        const bf16x8_t pf = seq_pack8(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]), pr = seq_rest8(p, pf);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             const bf16x4_t lo = seq_tr16(vt + toff[d]), hi = seq_tr16(vt + toff[d] + 16 * PITCH);
-            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), pf, acc[d], 0, 0, 0);
+            const bf16x8_t vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pr, acc[d], 0, 0, 0);
+            acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf, acc[d], 0, 0, 0);
         }
     };
 

@@ -306,8 +306,8 @@ __device__ __forceinline__ void decay_tr_product(f32x16_t (&acc)[PackedGeo<DH>::
 // All outputs of one role: four waves of 32 rows; the state in front of the segment, then the segment's keys, 32 at a time, pass through a ring of three LDS stages,
 // two ahead (counted waits).  A block is short -- 4 or 8 key tiles -- and lives on memory latency: stages of 32 keys and the fade table in LDS make three blocks
 // fit a CU (48 KB, 168 registers) at head width 128.
-template <int DH>
-__global__ void __launch_bounds__(256, DH <= 64 ? 4 : 3) decay_out_kernel(const DecayArgs g) {
+template <int DH, bool REST>
+__global__ void __launch_bounds__(256, REST ? 1 : DH <= 64 ? 4 : 3) decay_out_kernel(const DecayArgs g) {
     using G = PackedGeo<DH>;
     constexpr int BM = 128, STAGE = 64 * G::PITCH, MINE = 2 * DecayDma<DH>::SLABS;      // MINE: loads of a wave per stage
     __shared__ __attribute__((aligned(16))) char smem[3 * STAGE + 128];
@@ -421,6 +421,15 @@ __global__ void __launch_bounds__(256, DH <= 64 ? 4 : 3) decay_out_kernel(const 
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2)
             pf[s2] = seq_pack8(x[8 * s2], x[8 * s2 + 1], x[8 * s2 + 2], x[8 * s2 + 3], x[8 * s2 + 4], x[8 * s2 + 5], x[8 * s2 + 6], x[8 * s2 + 7]);
+        if (REST) {
+            bf16x8_t pr[2];
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2) {
+                const float p[8] = {x[8 * s2], x[8 * s2 + 1], x[8 * s2 + 2], x[8 * s2 + 3], x[8 * s2 + 4], x[8 * s2 + 5], x[8 * s2 + 6], x[8 * s2 + 7]};
+                pr[s2] = seq_rest8(p, pf[s2]);
+            }
+            decay_tr_product<DH>(y, at, ct, pr);
+        }
         decay_tr_product<DH>(y, at, ct, pf);
     }
     __syncthreads();
@@ -538,7 +547,9 @@ static int decay_run(const DecayArgs& g, void* stream) {
         hipLaunchKernelGGL(decay_scan_kernel, grid, dim3(256), 0, (hipStream_t)stream, g);
         GENIE_CHECK_LAUNCH();
     }
-    hipLaunchKernelGGL(decay_out_kernel<DH>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, g);
+    // few rows: the weights with what their rounding left over, for the reason at packed_exact() (a 32768-token prompt would pay 38 us for 33)
+    if (g.rows <= 512) hipLaunchKernelGGL((decay_out_kernel<DH, true>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, g);
+    else hipLaunchKernelGGL((decay_out_kernel<DH, false>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, g);
     GENIE_CHECK_LAUNCH();
     return GENIE_OK;
 }

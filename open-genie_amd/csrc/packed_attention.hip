@@ -45,12 +45,12 @@ __device__ __forceinline__ bool packed_rows(const PackedArgs& a, PackedRows& r, 
 
 // ------------------------------------------------------------------------------------------------------------------------------
 // Forward.  Online softmax in the exp2 domain with fp32 maximum, sum and accumulator; P is rounded to bf16 (at most 2^-8 of a weight, the precision
-// of V itself) because the second product runs on the matrix cores.  The running maximum is "sum-triggered": a tile is exponentiated against the
+// of V itself) because the second product runs on the matrix cores; REST adds a product with what that left over.  The running maximum is "sum-triggered": a tile is exponentiated against the
 // maximum as it stands, and only a lane whose partial row sum passes 2^8 (inf and NaN too) has the tile redone with its exact maximum -- no
 // per-tile maximum tree in the steady state.  A wave's first tile always takes its maximum; a row that sees nothing of it (the second key group's first tile may lie
 // behind it) sees nothing after it either.
 // ------------------------------------------------------------------------------------------------------------------------------
-template <int DH, int NG, int WPE>
+template <int DH, int NG, int WPE, bool REST>
 __global__ void __launch_bounds__(256 * NG, WPE) packed_fwd_kernel(const PackedArgs a) {
     using G = PackedGeo<DH>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(256 * NG, WPE) packed_fwd_kernel(const PackedA
         if (k0 >= r.w_end) continue;                                            // (wave-uniform) nothing of this tile is visible to these 32 rows
         at.forget();
         bool with_max = t == 0;
-        bf16x8_t pf[4];
+        bf16x8_t pf[4], pr[REST ? 4 : 1];
         float psum;
         for (;;) {
             f32x16_t sacc[2] = {packed_splat(0.f), packed_splat(0.f)};
@@ -141,6 +141,7 @@ __global__ void __launch_bounds__(256 * NG, WPE) packed_fwd_kernel(const PackedA
                         ps[e & 3] += p[e];
                     }
                     pf[2 * kt + s2] = seq_pack8(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]);
+                    if (REST) pr[REST ? 2 * kt + s2 : 0] = seq_rest8(p, pf[2 * kt + s2]);
                 }
             psum = (ps[0] + ps[1]) + (ps[2] + ps[3]);
             if (with_max || __builtin_amdgcn_ballot_w64(!(psum <= 256.f)) == 0) break;
@@ -150,8 +151,11 @@ __global__ void __launch_bounds__(256 * NG, WPE) packed_fwd_kernel(const PackedA
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
-            for (int d = 0; d < G::DT; ++d)
-                oacc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at.tr_frag(vt_ + ks * 16 * G::PITCH, d), pf[ks], oacc[d], 0, 0, 0);
+            for (int d = 0; d < G::DT; ++d) {
+                const bf16x8_t vf = at.tr_frag(vt_ + ks * 16 * G::PITCH, d);
+                if (REST) oacc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pr[REST ? ks : 0], oacc[d], 0, 0, 0);
+                oacc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[ks], oacc[d], 0, 0, 0);
+            }
     }
     float l = 0.f;
     if constexpr (NG == 1) {
@@ -201,11 +205,11 @@ __global__ void __launch_bounds__(256 * NG, WPE) packed_fwd_kernel(const PackedA
 // ------------------------------------------------------------------------------------------------------------------------------
 // Backward, dQ: the forward's walk over the keys with P recomputed from the log-sum-exp.  delta = rowsum(dO o O) of the wave's rows is formed from the
 // operand fragments, written out for the other kernel, and fed negated as the accumulator INPUT of dP^T = V dO^T, so that dS = P o (dP - delta) costs
-// no subtraction.  dS is rounded to bf16 for the last product, like P in the forward.  delta takes O with the 16 bits that its rounding left over: where a row sees few
+// no subtraction.  dS is rounded to bf16 for the last product (REST: and what that left over), like P in the forward.  delta takes O with the 16 bits that its rounding left over: where a row sees few
 // keys, dP - delta is a small difference, and the rounding of O alone would be as large an error in it as that of dS (a 5720-row batch: dQ 0.0026 off in
 // norm with it, 0.0024 without; sequences of a few tokens 0.0035 and 0.0024).
 // ------------------------------------------------------------------------------------------------------------------------------
-template <int DH, int NG, int WPE>
+template <int DH, int NG, int WPE, bool REST>
 __global__ void __launch_bounds__(256 * NG, WPE) packed_dq_kernel(const PackedArgs a) {
     using G = PackedGeo<DH>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -275,19 +279,23 @@ __global__ void __launch_bounds__(256 * NG, WPE) packed_dq_kernel(const PackedAr
 #pragma unroll
                 for (int e = 0; e < 16; ++e) sacc[e] = seq_crow(e) < lim ? sacc[e] : -INFINITY;
             }
-            bf16x8_t ds[2];
+            bf16x8_t ds[2], dr[REST ? 2 : 1];
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2) {
                 float x[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[8 * s2 + e], c2, -lse2)) * dp[8 * s2 + e];
                 ds[s2] = seq_pack8(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
+                if (REST) dr[REST ? s2 : 0] = seq_rest8(x, ds[s2]);
             }
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
-                for (int d = 0; d < G::DT; ++d)
-                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at.tr_frag(kt_ + (kt * 2 + s2) * 16 * G::PITCH, d), ds[s2], acc[d], 0, 0, 0);
+                for (int d = 0; d < G::DT; ++d) {
+                    const bf16x8_t kf = at.tr_frag(kt_ + (kt * 2 + s2) * 16 * G::PITCH, d);
+                    if (REST) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, dr[REST ? s2 : 0], acc[d], 0, 0, 0);
+                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, ds[s2], acc[d], 0, 0, 0);
+                }
         }
     }
     if constexpr (NG == 2) {
@@ -337,16 +345,18 @@ template <int DH>
 static int packed_fwd_dispatch(PackedArgs& a, void* stream) {
     a.nslots = a.rows_q / 128 + a.nseq + 1;
     const int64_t blocks = (int64_t)a.nslots * a.hq;
-    if (packed_two_groups(a, DH <= 64 ? (1ll << 31) : 512)) return packed_launch(packed_fwd_kernel<DH, 2, DH <= 64 ? 4 : 2>, a, blocks, 512, 8 * PackedGeo<DH>::TILE, stream);
-    return packed_launch(packed_fwd_kernel<DH, 1, DH <= 64 ? 3 : 2>, a, blocks, 256, 4 * PackedGeo<DH>::TILE, stream);
+    if (packed_exact(a)) return packed_launch(packed_fwd_kernel<DH, 1, 1, true>, a, blocks, 256, 4 * PackedGeo<DH>::TILE, stream);
+    if (packed_two_groups(a, DH <= 64 ? (1ll << 31) : 512)) return packed_launch(packed_fwd_kernel<DH, 2, DH <= 64 ? 4 : 2, false>, a, blocks, 512, 8 * PackedGeo<DH>::TILE, stream);
+    return packed_launch(packed_fwd_kernel<DH, 1, DH <= 64 ? 3 : 2, false>, a, blocks, 256, 4 * PackedGeo<DH>::TILE, stream);
 }
 
 template <int DH>
 static int packed_bwd_dispatch(PackedArgs& a, void* stream) {
     a.nslots = a.rows_q / 128 + a.nseq + 1;
     const int64_t blocks = (int64_t)a.nslots * a.hq;
-    const int rc = packed_two_groups(a, 512) ? packed_launch(packed_dq_kernel<DH, 2, 2>, a, blocks, 512, 8 * PackedGeo<DH>::TILE, stream)
-                                             : packed_launch(packed_dq_kernel<DH, 1, DH <= 64 ? 3 : 2>, a, blocks, 256, 4 * PackedGeo<DH>::TILE, stream);
+    const int rc = packed_exact(a)             ? packed_launch(packed_dq_kernel<DH, 1, 1, true>, a, blocks, 256, 4 * PackedGeo<DH>::TILE, stream)
+                   : packed_two_groups(a, 512) ? packed_launch(packed_dq_kernel<DH, 2, 2, false>, a, blocks, 512, 8 * PackedGeo<DH>::TILE, stream)
+                                               : packed_launch(packed_dq_kernel<DH, 1, DH <= 64 ? 3 : 2, false>, a, blocks, 256, 4 * PackedGeo<DH>::TILE, stream);
     return rc != GENIE_OK ? rc : packed_dkv_run(a, stream);
 }
 

@@ -11,7 +11,7 @@
 // Head widths up to 64: KT = 1, three waves per SIMD hide each other's latencies.
 #include "packed_common.h"
 
-template <int DH, int KT, int WPE, bool VLDS>
+template <int DH, int KT, int WPE, bool VLDS, bool REST>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) packed_dkv_kernel(const PackedArgs a) {
     using G = PackedGeo<DH>;
     constexpr int NW = 4, BN = 32 * KT * NW, NT = 64 * NW, STAGE = 2 * G::TILE + 512;
@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, W
                 for (int r = 0; r < 16; ++r) sacc[kt][r] = seq_crow(r) >= lim ? sacc[kt][r] : -INFINITY;
             }
         }
-        bf16x8_t pf[KT][2], ds[KT][2];
+        bf16x8_t pf[KT][2], ds[KT][2], pr[REST ? KT : 1][2], dr[REST ? KT : 1][2];
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
 #pragma unroll
@@ -118,6 +118,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, W
                 }
                 pf[kt][s2] = seq_pack8(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]);
                 ds[kt][s2] = seq_pack8(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
+                if (REST) {
+                    pr[REST ? kt : 0][s2] = seq_rest8(p, pf[kt][s2]);
+                    dr[REST ? kt : 0][s2] = seq_rest8(x, ds[kt][s2]);
+                }
             }
         }
 #pragma unroll
@@ -127,6 +131,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, W
                 const bf16x8_t gt = at.tr_frag(gt_ + s2 * 16 * G::PITCH, d), qt = at.tr_frag(qt_ + s2 * 16 * G::PITCH, d);
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) {
+                    if (REST) {
+                        dv[kt][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(gt, pr[REST ? kt : 0][s2], dv[kt][d], 0, 0, 0);
+                        dk[kt][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qt, dr[REST ? kt : 0][s2], dk[kt][d], 0, 0, 0);
+                    }
                     dv[kt][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(gt, pf[kt][s2], dv[kt][d], 0, 0, 0);
                     dk[kt][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qt, ds[kt][s2], dk[kt][d], 0, 0, 0);
                 }
@@ -203,16 +211,11 @@ __global__ void __launch_bounds__(256) packed_dkv_sum_kernel(const PackedArgs a)
     }
 }
 
-#ifndef PACKED_DKV_BLOCKS
-#define PACKED_DKV_BLOCKS 1024
-#endif
-#ifndef PACKED_DKV_BLOCKS_WIDE
-#define PACKED_DKV_BLOCKS_WIDE 512
-#endif
-// parts a tile's (head, row tile) steps are cut into: as many as bring the launch to about PACKED_DKV_BLOCKS blocks, at most 8 and no more than there can be steps
+// parts a tile's (head, row tile) steps are cut into: as many as bring the launch to about 1024 blocks (three of them on a CU; head widths above 64, one on a CU: 512), at most 8
+// and no more than there can be steps
 static int packed_dkv_splits(int nseq, int rows_q, int rows_k, int hq, int hkv, int dim) {
     const int64_t blocks = (int64_t)(rows_k / (dim > 64 ? 256 : 128) + (nseq < rows_k ? nseq : rows_k)) * hkv, steps = (int64_t)(rows_q / 64 + 1) * (hq / hkv);
-    int64_t n = blocks > 0 ? ((dim > 64 ? PACKED_DKV_BLOCKS_WIDE : PACKED_DKV_BLOCKS) + blocks / 2) / blocks : 1;
+    int64_t n = blocks > 0 ? ((dim > 64 ? 512 : 1024) + blocks / 2) / blocks : 1;
     n = n < steps ? n : steps;
     return (int)(n < 1 ? 1 : n > 8 ? 8 : n);
 }
@@ -222,11 +225,11 @@ extern "C" int64_t genie_packed_attention_bwd_ws_floats(int nseq, int rows_q, in
     return (int64_t)hq * rows_q + 4 + (n > 1 ? (int64_t)2 * n * rows_k * hkv * dim : 0);      // delta (rounded up to 16 B), parts
 }
 
-template <int DH, int KT, int WPE>
+template <int DH, int KT, int WPE, bool REST = false>
 static int packed_dkv_dispatch(PackedArgs& a, void* stream) {
     constexpr bool VLDS = KT > 1;
     a.nslots = a.rows_k / (128 * KT) + a.nseq + 1;
-    const int rc = packed_launch(packed_dkv_kernel<DH, KT, WPE, VLDS>, a, (int64_t)a.nslots * a.hkv * a.nsplit, 256,
+    const int rc = packed_launch(packed_dkv_kernel<DH, KT, WPE, VLDS, REST>, a, (int64_t)a.nslots * a.hkv * a.nsplit, 256,
                                  4 * PackedGeo<DH>::TILE + 1024 + (VLDS ? 128 * KT * PackedGeo<DH>::PITCH : 0), stream);
     if (rc != GENIE_OK || a.nsplit == 1) return rc;
     return packed_launch(packed_dkv_sum_kernel, a, ((int64_t)a.rows_k * a.hkv * a.dim / 8 + 255) / 256, 256, 0, stream);
@@ -234,6 +237,12 @@ static int packed_dkv_dispatch(PackedArgs& a, void* stream) {
 int packed_dkv_run(PackedArgs& a, void* stream) {
     a.nsplit = packed_dkv_splits(a.nseq, a.rows_q, a.rows_k, a.hq, a.hkv, a.dim);
     a.part = a.delta + ((int64_t)a.hq * a.rows_q + 3) / 4 * 4;
+    if (packed_exact(a)) {
+        if (a.dim <= 32) return packed_dkv_dispatch<32, 1, 1, true>(a, stream);
+        if (a.dim <= 64) return packed_dkv_dispatch<64, 1, 1, true>(a, stream);
+        if (a.dim <= 96) return packed_dkv_dispatch<96, 1, 1, true>(a, stream);
+        return packed_dkv_dispatch<128, 1, 1, true>(a, stream);
+    }
     if (a.dim <= 32) return packed_dkv_dispatch<32, 1, 3>(a, stream);
     if (a.dim <= 64) return packed_dkv_dispatch<64, 1, 3>(a, stream);
     if (a.dim <= 96) return packed_dkv_dispatch<96, 2, 1>(a, stream);

@@ -125,6 +125,13 @@ __device__ __forceinline__ bf16x8_t seq_pack8(const float a0, const float a1, co
     const u32x4_t v = {pack_bf16x2(a0, a1), pack_bf16x2(a2, a3), pack_bf16x2(a4, a5), pack_bf16x2(a6, a7)};
     return __builtin_bit_cast(bf16x8_t, v);
 }
+// what rounding to bf16 left over of x, rounded in its turn: x = hi + rest within 2^-17 of x
+__device__ __forceinline__ bf16x8_t seq_rest8(const float (&x)[8], bf16x8_t hi) {
+    float r[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = x[e] - bf16_to_f32((bf16_t)hi[e]);
+    return seq_pack8(r[0], r[1], r[2], r[3], r[4], r[5], r[6], r[7]);
+}
 
 // value of the partner lane (lane ^ 32) combined with this lane's.  Inline asm as in the other attention kernels: given two copies of one value the
 // builtin is folded as if the swap were the identity; no memory is involved, `s_nop 1` covers the VALU-write -> permlane-read hazard.

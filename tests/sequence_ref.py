@@ -17,8 +17,9 @@ def bounds(lens):
     return out
 
 
-def packed_reference(q, k, v, lens, scale, dout=None, lens_k=None):
-    """out, dq, dk, dv and the largest error each may have (dicts by name)."""
+def packed_reference(q, k, v, lens, scale, dout=None, lens_k=None, w=U):
+    """out, dq, dk, dv and the largest error each may have (dicts by name).  w: what the roundings of the weights (P, dS) and of the output in delta move them by:
+    U, or U^2 where the kernels carry a second bf16 value for what the first left over."""
     q, k, v = q.double(), k.double(), v.double()
     g = None if dout is None else dout.double()
     hq, hkv = q.shape[1], k.shape[1]
@@ -39,7 +40,7 @@ def packed_reference(q, k, v, lens, scale, dout=None, lens_k=None):
             p = p / p.sum(1, keepdim=True).clamp(min=1e-300)
             o = p @ V
             val['out'][a:b, h] = o
-            t_o = U * o.abs() + (U + SLACK) * (p @ V.abs())                      # own rounding; weights' rounding
+            t_o = U * o.abs() + (w + SLACK) * (p @ V.abs())                      # own rounding; weights' rounding
             tol['out'][a:b, h] = t_o
             if g is None:
                 continue
@@ -50,16 +51,16 @@ def packed_reference(q, k, v, lens, scale, dout=None, lens_k=None):
             val['dk'][ka:kb, j] += scale * (ds.T @ Q)
             val['dv'][ka:kb, j] += p.T @ G
             # dS is rounded; delta comes from the rounded output; SLACK of the magnitudes that dP and delta are sums of
-            e_ds = U * ds.abs() + p * (G.abs() * t_o).sum(1, keepdim=True) + SLACK * p * (G.abs() @ V.abs().T + (G * o).abs().sum(1, keepdim=True))
+            e_ds = w * ds.abs() + p * (G.abs() * (t_o - (U - w) * o.abs())).sum(1, keepdim=True) + SLACK * p * (G.abs() @ V.abs().T + (G * o).abs().sum(1, keepdim=True))
             tol['dq'][a:b, h] = scale * (e_ds @ K.abs())
             tol['dk'][ka:kb, j] += scale * (e_ds.T @ Q.abs())
-            tol['dv'][ka:kb, j] += (U + SLACK) * (p.T @ G.abs())
+            tol['dv'][ka:kb, j] += (w + SLACK) * (p.T @ G.abs())
     for n in names[1:]:
         tol[n] += U * val[n].abs()
     return val, tol
 
 
-def step_reference(q, k_cache, v_cache, lengths, scale):
+def step_reference(q, k_cache, v_cache, lengths, scale, w=U):
     """One query per sequence against the first lengths[b] places of its cache."""
     val, tol = torch.zeros_like(q, dtype=torch.float64), torch.zeros_like(q, dtype=torch.float64)
     for b, n in enumerate(lengths):
@@ -69,13 +70,13 @@ def step_reference(q, k_cache, v_cache, lengths, scale):
                 p = torch.softmax(scale * (k_cache[b, :n, j].double() @ q[b, h].double()), 0)
                 V = v_cache[b, :n, j].double()
                 val[b, h] = p @ V
-                tol[b, h] = U * val[b, h].abs() + (U + SLACK) * (p @ V.abs())
+                tol[b, h] = U * val[b, h].abs() + (w + SLACK) * (p @ V.abs())
     return val, tol
 
 
-def decay_form(a, b, c, log_decay, lens, scale, reverse=False, state=None):
+def decay_form(a, b, c, log_decay, lens, scale, reverse=False, state=None, w=U):
     """y_t = scale sum_{s <= t} l^(t-s) (a_t . b_s) c_s + scale l^(t+1) a_t S, and its bound: the scores (or the state they are summed into) are rounded to
-    bf16 as operands, the result is rounded once."""
+    bf16 as operands (w: by how much), the result is rounded once."""
     a, b, c = a.double(), b.double(), c.double()
     val = torch.zeros(a.shape[:2] + c.shape[2:], dtype=torch.float64, device=a.device)
     tol = torch.zeros_like(val)
@@ -93,7 +94,7 @@ def decay_form(a, b, c, log_decay, lens, scale, reverse=False, state=None):
                 y = y + lead * (A @ state[i, h].double())
                 mag = mag + lead * (A.abs() @ state[i, h].double().abs())
             val[lo:hi, h] = scale * y
-            tol[lo:hi, h] = scale * (U * y.abs() + (U + SLACK) * mag)
+            tol[lo:hi, h] = scale * (U * y.abs() + (w + SLACK) * mag)
     return val, tol
 
 

@@ -557,3 +557,33 @@ def test_offsets_past_32_bits_in_a_long_cache():
     assert torch.equal(gf.packed_attention(wide, wide, wide, _cu([rows])), gf.packed_attention(dense, dense, dense, _cu([rows])))
     ld = _decays(hkv)
     assert torch.equal(gf.decay_attention(wide, wide, wide, ld, _cu([rows])), gf.decay_attention(dense, dense, dense, ld, _cu([rows])))
+
+
+@pytest.mark.parametrize('lens, spare', [([2, 2, 3], 0), ([1, 0, 31], 5), ([70, 130, 57, 255], 0)], ids=str)
+@pytest.mark.parametrize('d', [32, 64, 80, 128])
+def test_few_rows_round_nothing_but_their_results(lens, spare, d):
+    """Up to 512 rows the weights go into the products with their rounding's remainder (U^2 of them is left), in the cached form always."""
+    gf, w = _gf(), R.U ** 2
+    q, k, v, g = _packed_inputs(lens, spare, 4, 2, d, 700)
+    cu, rows, tiny = _cu(lens), sum(lens), 2.0 ** -100
+    val, tol = R.packed_reference(q, k, v, lens, d ** -0.5, g, w=w)
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    out = gf.packed_attention(q, k, v, cu)
+    grads = torch.autograd.grad(out, (q, k, v), g)
+    for name, t in zip(('out', 'dq', 'dk', 'dv'), (out, *grads)):
+        R.assert_within(t, val[name], tol[name] + tiny, name)
+    decay = -torch.linspace(0.01, 0.5, 2, device='cuda')
+    a, b, c = (x.detach()[:, :2].clone().requires_grad_(True) for x in (q, k, v))
+    out = gf.decay_attention(a, b, c, decay, cu)
+    da, db, dc = torch.autograd.grad(out, (a, b, c), g[:, :2])
+    z, (a, b, c) = g[:, :2], (x.detach() for x in (a, b, c))       # (no sequence passes 256 tokens: no rounded state in front of a segment)
+    for name, got, (ref, tol) in (('decay out', out, R.decay_form(a, b, c, decay, lens, d ** -0.5, w=w)),
+                                  ('decay dq', da, R.decay_form(z, c, b, decay, lens, d ** -0.5, w=w)),
+                                  ('decay dk', db, R.decay_form(c, z, a, decay, lens, d ** -0.5, reverse=True, w=w)),
+                                  ('decay dv', dc, R.decay_form(b, a, z, decay, lens, d ** -0.5, reverse=True, w=w))):
+        R.assert_within(got[:rows], ref[:rows], tol[:rows] + tiny, name)
+    cache = [_randn(2, 600, 2, d, seed=710 + i) for i in range(2)]
+    n = torch.tensor([600, 3], dtype=torch.int32, device='cuda')
+    val, tol = R.step_reference(g[:2], cache[0], cache[1], [600, 3], d ** -0.5, w=w)
+    R.assert_within(gf.cached_attention_step(g[:2].contiguous(), cache[0], cache[1], n), val, tol + tiny, 'step')
