@@ -548,7 +548,7 @@ static int decay_run(const DecayArgs& g, void* stream) {
         GENIE_CHECK_LAUNCH();
     }
     // few rows: the weights with what their rounding left over, for the reason at packed_exact() (a 32768-token prompt would pay 38 us for 33)
-    if (g.rows <= 512) hipLaunchKernelGGL((decay_out_kernel<DH, true>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, g);
+    if (g.rows <= 256) hipLaunchKernelGGL((decay_out_kernel<DH, true>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, g);
     else hipLaunchKernelGGL((decay_out_kernel<DH, false>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, g);
     GENIE_CHECK_LAUNCH();
     return GENIE_OK;

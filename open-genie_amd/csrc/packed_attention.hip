@@ -20,24 +20,25 @@ struct PackedRows {
     PackedBlock blk;
     int kstart, klen, shift, q0, qi, nstep, w_end, grp, rw;
 };
-template <int NG>
+template <int RW, int NG>
 __device__ __forceinline__ bool packed_rows(const PackedArgs& a, PackedRows& r, bf16_t* out) {
+    constexpr int BM = 32 * RW;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    r.grp = wave >> 2;
-    r.rw = wave & 3;
+    r.grp = wave / RW;
+    r.rw = wave % RW;
     r.blk = packed_block(a, a.hq);
-    r.s = seq_find_longest<128, false>(a.cu_q, a.nseq, a.rows_q, r.blk.slot, a.nslots);
-    if (r.s.tile < 0 || r.s.tile * 128 >= r.s.len) return false;
+    r.s = seq_find_longest<BM, false>(a.cu_q, a.nseq, a.rows_q, r.blk.slot, a.nslots);
+    if (r.s.tile < 0 || r.s.tile * BM >= r.s.len) return false;
     if (r.s.seq == a.nseq) {
-        packed_zero_rows<128, 256 * NG>(out, a.hq, a.dim, r.s, r.blk.head);
+        packed_zero_rows<BM, 64 * RW * NG>(out, a.hq, a.dim, r.s, r.blk.head);
         return false;
     }
     r.kstart = seq_cu(a.cu_k, r.s.seq, a.rows_k);
     r.klen = max(0, seq_cu(a.cu_k, r.s.seq + 1, a.rows_k) - r.kstart);
     r.shift = r.klen - r.s.len;                                                 // query i sees keys 0 .. i + shift
-    r.q0 = r.s.tile * 128 + r.rw * 32;
+    r.q0 = r.s.tile * BM + r.rw * 32;
     r.qi = r.q0 + (lane & 31);
-    const int k_end = min(r.klen, min(r.s.tile * 128 + 128, r.s.len) + r.shift);     // of the block (<= 0: nothing to see)
+    const int k_end = min(r.klen, min(r.s.tile * BM + BM, r.s.len) + r.shift);     // of the block (<= 0: nothing to see)
     r.w_end = min(r.klen, min(r.q0 + 32, r.s.len) + r.shift);                   // of this wave
     r.nstep = (max(k_end, 0) + 64 * NG - 1) / (64 * NG);
     return true;
@@ -50,13 +51,13 @@ __device__ __forceinline__ bool packed_rows(const PackedArgs& a, PackedRows& r, 
 // per-tile maximum tree in the steady state.  A wave's first tile always takes its maximum; a row that sees nothing of it (the second key group's first tile may lie
 // behind it) sees nothing after it either.
 // ------------------------------------------------------------------------------------------------------------------------------
-template <int DH, int NG, int WPE, bool REST>
-__global__ void __launch_bounds__(256 * NG, WPE) packed_fwd_kernel(const PackedArgs a) {
+template <int DH, int RW, int NG, int WPE, bool REST>
+__global__ void __launch_bounds__(64 * RW * NG, WPE) packed_fwd_kernel(const PackedArgs a) {
     using G = PackedGeo<DH>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     PackedRows r;
-    if (!packed_rows<NG>(a, r, a.out)) return;
+    if (!packed_rows<RW, NG>(a, r, a.out)) return;
     bf16x8_t qf[G::KS];
     packed_row_frags<DH>(qf, a.q + (int64_t)(r.s.start + r.qi) * a.q_row + r.blk.head * a.q_head, r.qi < r.s.len, a.dim);
     f32x16_t oacc[G::DT];
@@ -68,7 +69,7 @@ __global__ void __launch_bounds__(256 * NG, WPE) packed_fwd_kernel(const PackedA
     const bf16_t* kp = a.k + (int64_t)r.kstart * a.k_row + r.blk.kvh * a.k_head;
     const bf16_t* vp = a.v + (int64_t)r.kstart * a.v_row + r.blk.kvh * a.v_head;
     const int64_t k_step = 64 * NG * a.k_row, v_step = 64 * NG * a.v_row;
-    PackedDma<DH, 4 * NG, NG, (DH <= 64)> st;
+    PackedDma<DH, RW * NG, NG, (DH <= 64)> st;
     st.init(wave, lane, a.dim, a.k_row, a.v_row);
     auto load = [&](int t) {                                                    // (called for t = 0, 1, 2 ..)
         char* to = smem + (t & 1) * 2 * NG * G::TILE;
@@ -209,13 +210,13 @@ __global__ void __launch_bounds__(256 * NG, WPE) packed_fwd_kernel(const PackedA
 // keys, dP - delta is a small difference, and the rounding of O alone would be as large an error in it as that of dS (a 5720-row batch: dQ 0.0026 off in
 // norm with it, 0.0024 without; sequences of a few tokens 0.0035 and 0.0024).
 // ------------------------------------------------------------------------------------------------------------------------------
-template <int DH, int NG, int WPE, bool REST>
-__global__ void __launch_bounds__(256 * NG, WPE) packed_dq_kernel(const PackedArgs a) {
+template <int DH, int RW, int NG, int WPE, bool REST>
+__global__ void __launch_bounds__(64 * RW * NG, WPE) packed_dq_kernel(const PackedArgs a) {
     using G = PackedGeo<DH>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     PackedRows r;
-    if (!packed_rows<NG>(a, r, a.dq)) return;
+    if (!packed_rows<RW, NG>(a, r, a.dq)) return;
     bf16x8_t qf[G::KS], gf[G::KS];
     const int64_t qrow = r.s.start + r.qi;
     packed_row_frags<DH>(qf, a.q + qrow * a.q_row + r.blk.head * a.q_head, r.qi < r.s.len, a.dim);
@@ -244,7 +245,7 @@ __global__ void __launch_bounds__(256 * NG, WPE) packed_dq_kernel(const PackedAr
     const bf16_t* kp = a.k + (int64_t)r.kstart * a.k_row + r.blk.kvh * a.k_head;
     const bf16_t* vp = a.v + (int64_t)r.kstart * a.v_row + r.blk.kvh * a.v_head;
     const int64_t k_step = 64 * NG * a.k_row, v_step = 64 * NG * a.v_row;
-    PackedDma<DH, 4 * NG, NG, (DH <= 64)> st;
+    PackedDma<DH, RW * NG, NG, (DH <= 64)> st;
     st.init(wave, lane, a.dim, a.k_row, a.v_row);
     auto load = [&](int t) {                                                    // (called for t = 0, 1, 2 ..)
         char* to = smem + (t & 1) * 2 * NG * G::TILE;
@@ -339,24 +340,36 @@ static int packed_check(const char* what, const PackedArgs& a) {
 // instead of two independent ones) from an average of 512 rows per sequence on, and while the launch leaves CUs short of blocks.  Measured one / two groups, us,
 // 16 query heads over 4 key heads: forward at width 64, one sequence of 1024 / 4096 / 8192: 18.2 / 15.3, 61.5 / 52.3, 158.0 / 157.3, at 40 x 100 rows 11.2 / 16.1;
 // width 128: 28.2 / 22.6, 101.2 / 91.2, 292.7 / 290.5, 4 x 2048: 89.0 / 97.8.  Backward at width 64: 52.1 / 49.3, 174.5 / 162.3, 504 / 520.
-static bool packed_two_groups(const PackedArgs& a, int64_t most) { return a.rows_q >= 512ll * a.nseq && (int64_t)(a.rows_q / 128) * a.hq <= most; }
+// At widths up to 64 these blocks hold 64 rows instead of 128 while there are few of them: forward, 128 / 64 rows, 8 heads, one sequence of 1024 / 4096 / 8192:
+// 15.1 / 12.4, 43.2 / 38.6, 94.4 / 99.9; 5720 ragged rows 30.6 / 26.6 (dQ 33.2 / 30.5); 4 x 2048 31.0 / 34.7.
+static bool packed_two_groups(const PackedArgs& a, int64_t most) { return a.rows_q >= 512ll * a.nseq && packed_few(a.rows_q, a.hq, most); }
+
+template <int DH, int RW, int NG, int WPE, bool REST>
+static int packed_fwd_run(PackedArgs& a, void* stream) {
+    a.nslots = a.rows_q / (32 * RW) + a.nseq + 1;
+    return packed_launch(packed_fwd_kernel<DH, RW, NG, WPE, REST>, a, (int64_t)a.nslots * a.hq, 64 * RW * NG, 4 * NG * PackedGeo<DH>::TILE, stream);
+}
+template <int DH, int RW, int NG, int WPE, bool REST>
+static int packed_dq_run(PackedArgs& a, void* stream) {
+    a.nslots = a.rows_q / (32 * RW) + a.nseq + 1;
+    return packed_launch(packed_dq_kernel<DH, RW, NG, WPE, REST>, a, (int64_t)a.nslots * a.hq, 64 * RW * NG, 4 * NG * PackedGeo<DH>::TILE, stream);
+}
 
 template <int DH>
 static int packed_fwd_dispatch(PackedArgs& a, void* stream) {
-    a.nslots = a.rows_q / 128 + a.nseq + 1;
-    const int64_t blocks = (int64_t)a.nslots * a.hq;
-    if (packed_exact(a)) return packed_launch(packed_fwd_kernel<DH, 1, 1, true>, a, blocks, 256, 4 * PackedGeo<DH>::TILE, stream);
-    if (packed_two_groups(a, DH <= 64 ? (1ll << 31) : 512)) return packed_launch(packed_fwd_kernel<DH, 2, DH <= 64 ? 4 : 2, false>, a, blocks, 512, 8 * PackedGeo<DH>::TILE, stream);
-    return packed_launch(packed_fwd_kernel<DH, 1, DH <= 64 ? 3 : 2, false>, a, blocks, 256, 4 * PackedGeo<DH>::TILE, stream);
+    if (packed_exact(a)) return packed_fwd_run<DH, 4, 1, 1, true>(a, stream);
+    if (DH <= 64 && packed_two_groups(a, 448)) return packed_fwd_run<DH <= 64 ? DH : 64, 2, 2, 2, false>(a, stream);
+    if (packed_two_groups(a, DH <= 64 ? (1ll << 31) : 512)) return packed_fwd_run<DH, 4, 2, DH <= 64 ? 4 : 2, false>(a, stream);
+    return packed_fwd_run<DH, 4, 1, DH <= 64 ? 3 : 2, false>(a, stream);
 }
 
 template <int DH>
 static int packed_bwd_dispatch(PackedArgs& a, void* stream) {
-    a.nslots = a.rows_q / 128 + a.nseq + 1;
-    const int64_t blocks = (int64_t)a.nslots * a.hq;
-    const int rc = packed_exact(a)             ? packed_launch(packed_dq_kernel<DH, 1, 1, true>, a, blocks, 256, 4 * PackedGeo<DH>::TILE, stream)
-                   : packed_two_groups(a, 512) ? packed_launch(packed_dq_kernel<DH, 2, 2, false>, a, blocks, 512, 8 * PackedGeo<DH>::TILE, stream)
-                                               : packed_launch(packed_dq_kernel<DH, 1, DH <= 64 ? 3 : 2, false>, a, blocks, 256, 4 * PackedGeo<DH>::TILE, stream);
+    int rc;
+    if (packed_exact(a)) rc = packed_dq_run<DH, 4, 1, 1, true>(a, stream);
+    else if (DH <= 64 && packed_two_groups(a, 448)) rc = packed_dq_run<DH <= 64 ? DH : 64, 2, 2, 2, false>(a, stream);
+    else if (packed_two_groups(a, 512)) rc = packed_dq_run<DH, 4, 2, 2, false>(a, stream);
+    else rc = packed_dq_run<DH, 4, 1, DH <= 64 ? 3 : 2, false>(a, stream);
     return rc != GENIE_OK ? rc : packed_dkv_run(a, stream);
 }
 

@@ -11,10 +11,10 @@
 // Head widths up to 64: KT = 1, three waves per SIMD hide each other's latencies.
 #include "packed_common.h"
 
-template <int DH, int KT, int WPE, bool VLDS, bool REST>
+template <int DH, int KT, int RG, int WPE, bool VLDS, bool REST>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) packed_dkv_kernel(const PackedArgs a) {
     using G = PackedGeo<DH>;
-    constexpr int NW = 4, BN = 32 * KT * NW, NT = 64 * NW, STAGE = 2 * G::TILE + 512;
+    constexpr int NW = 4, KG = NW / RG, BN = 32 * KT * KG, NT = 64 * NW, STAGE = 2 * G::TILE + 512;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int kvh = (int)blockIdx.x % a.hkv, part = (int)blockIdx.x / a.hkv % a.nsplit, slot = (int)blockIdx.x / a.hkv / a.nsplit, group = a.hq / a.hkv;
@@ -28,7 +28,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, W
     }
     const int qstart = seq_cu(a.cu_q, s.seq, a.rows_q), qlen = max(0, seq_cu(a.cu_q, s.seq + 1, a.rows_q) - qstart);
     const int shift = s.len - qlen;                                             // key j is seen by rows i >= j - shift
-    const int j0 = s.tile * BN + wave * 32 * KT, kj = j0 + (lane & 31);
+    const int kg = wave % KG, rg = wave / KG;                                   // this wave's keys and, RG = 2, its half of each tile's rows
+    const int j0 = s.tile * BN + kg * 32 * KT, kj = j0 + (lane & 31);
     const int first = max(0, s.tile * BN - shift) & ~63;                        // first query row the block needs, on a tile border
     const int w_first = j0 - shift;
     const int tiles = max(0, (qlen - first + 63) >> 6);
@@ -151,12 +152,35 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, W
         __syncthreads();
         if (i + 1 < i1) load(i + 1);
         const int r0 = first + (i % tiles) * 64;
-        if (r0 + 63 < w_first) continue;                                        // (wave-uniform) no row of these 64 sees this wave's keys
+        if (r0 + (RG == 2 ? rg * 32 + 31 : 63) < w_first) continue;             // (wave-uniform) none of these rows sees this wave's keys
         at.forget();
 #pragma unroll 1
-        for (int qt = 0; qt < 2; ++qt) rows32(qt_ + qt * 32 * G::PITCH, gt_ + qt * 32 * G::PITCH, stats + qt * 32, r0 + qt * 32);
+        for (int qt = RG == 2 ? rg : 0; qt < (RG == 2 ? rg + 1 : 2); ++qt) rows32(qt_ + qt * 32 * G::PITCH, gt_ + qt * 32 * G::PITCH, stats + qt * 32, r0 + qt * 32);
+    }
+    if constexpr (RG == 2) {                                                    // the row halves' sums meet in LDS, register by register
+        static_assert(KT == 1, "one set of accumulators");
+        __syncthreads();
+        float* xs = reinterpret_cast<float*>(smem) + kg * 2 * G::DT * 16 * 64 + lane;
+        if (rg == 1)
+#pragma unroll
+            for (int d = 0; d < G::DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    xs[(d * 32 + e) * 64] = dk[0][d][e];
+                    xs[(d * 32 + 16 + e) * 64] = dv[0][d][e];
+                }
+        __syncthreads();
+        if (rg == 0)
+#pragma unroll
+            for (int d = 0; d < G::DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    dk[0][d][e] += xs[(d * 32 + e) * 64];
+                    dv[0][d][e] += xs[(d * 32 + 16 + e) * 64];
+                }
     }
     if (a.nsplit > 1) {                                                         // fp32 parts, 16 B per lane and store
+        if (rg != 0) return;
         float* pk = a.part + (((int64_t)part * 2 * a.rows_k + s.start) * a.hkv + kvh) * a.dim;
         float* pv = pk + (int64_t)a.rows_k * a.hkv * a.dim;
 #pragma unroll
@@ -178,6 +202,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, W
         return;
     }
     __syncthreads();
+    if (rg != 0) return;
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
         const int j = j0 + 32 * kt;
@@ -211,13 +236,26 @@ __global__ void __launch_bounds__(256) packed_dkv_sum_kernel(const PackedArgs a)
     }
 }
 
-// parts a tile's (head, row tile) steps are cut into: as many as bring the launch to about 1024 blocks (three of them on a CU; head widths above 64, one on a CU: 512), at most 8
-// and no more than there can be steps
+// Parts that a key tile's (head, row tile) steps are cut into.  A launch takes the longest chain of steps (all sequences taken as equally long), or the time that all pairs take on a
+// full chip, whichever is longer; parts shorten the chain and cost a second launch and their fp32 sums written and read.  The rates are
+// measured: a step 1 us (64 keys per block), 2 us (128) or 4.7 us (256, width 128), 0.56 or 1.14 us per million pairs, 5 us, 6 TB/s.  The model's order of n = 1 .. 8 was the measured one
+// for every batch tried, e.g. 4 x 700 rows, 8 / 8 heads of width 64, n = 1, 2, 3: 33 / 40 / 44 us the whole backward; 16 / 4 heads, n = 3, 4, 5, 8: 57 / 55 / 56 / 64.
 static int packed_dkv_splits(int nseq, int rows_q, int rows_k, int hq, int hkv, int dim) {
-    const int64_t blocks = (int64_t)(rows_k / (dim > 64 ? 256 : 128) + (nseq < rows_k ? nseq : rows_k)) * hkv, steps = (int64_t)(rows_q / 64 + 1) * (hq / hkv);
-    int64_t n = blocks > 0 ? ((dim > 64 ? 512 : 1024) + blocks / 2) / blocks : 1;
-    n = n < steps ? n : steps;
-    return (int)(n < 1 ? 1 : n > 8 ? 8 : n);
+    const float length = (float)rows_q / (float)(nseq > 0 ? nseq : 1);
+    const float step = dim > 64 ? 4.7f * (float)dim / 128.f : packed_few(rows_q, hq, 512) ? 1.f : 2.f;
+    const float chain = (length / 64.f + 1.f) * (float)(hq / hkv) * step;
+    const float all = (float)rows_q * length * 0.5f * (float)hq * (dim > 64 ? 1.14e-6f : 0.56e-6f);
+    const float part = (float)rows_k * (float)hkv * (float)dim * 16.f / 6e6f;
+    int best = 1;
+    float least = 0.f;
+    for (int n = 1; n <= 8; ++n) {
+        const float t = (chain / (float)n > all ? chain / (float)n : all) + (n > 1 ? 5.f + (float)n * part : 0.f);
+        if (n == 1 || t < least) {
+            least = t;
+            best = n;
+        }
+    }
+    return best;
 }
 extern "C" int64_t genie_packed_attention_bwd_ws_floats(int nseq, int rows_q, int rows_k, int hq, int hkv, int dim) {
     if (nseq < 0 || rows_q <= 0 || rows_k <= 0 || hkv <= 0 || hq <= 0 || hq % hkv != 0 || dim <= 0) return 0;
@@ -225,11 +263,11 @@ extern "C" int64_t genie_packed_attention_bwd_ws_floats(int nseq, int rows_q, in
     return (int64_t)hq * rows_q + 4 + (n > 1 ? (int64_t)2 * n * rows_k * hkv * dim : 0);      // delta (rounded up to 16 B), parts
 }
 
-template <int DH, int KT, int WPE, bool REST = false>
+template <int DH, int KT, int RG, int WPE, bool REST = false>
 static int packed_dkv_dispatch(PackedArgs& a, void* stream) {
     constexpr bool VLDS = KT > 1;
-    a.nslots = a.rows_k / (128 * KT) + a.nseq + 1;
-    const int rc = packed_launch(packed_dkv_kernel<DH, KT, WPE, VLDS, REST>, a, (int64_t)a.nslots * a.hkv * a.nsplit, 256,
+    a.nslots = a.rows_k / (128 * KT / RG) + a.nseq + 1;
+    const int rc = packed_launch(packed_dkv_kernel<DH, KT, RG, WPE, VLDS, REST>, a, (int64_t)a.nslots * a.hkv * a.nsplit, 256,
                                  4 * PackedGeo<DH>::TILE + 1024 + (VLDS ? 128 * KT * PackedGeo<DH>::PITCH : 0), stream);
     if (rc != GENIE_OK || a.nsplit == 1) return rc;
     return packed_launch(packed_dkv_sum_kernel, a, ((int64_t)a.rows_k * a.hkv * a.dim / 8 + 255) / 256, 256, 0, stream);
@@ -238,13 +276,17 @@ int packed_dkv_run(PackedArgs& a, void* stream) {
     a.nsplit = packed_dkv_splits(a.nseq, a.rows_q, a.rows_k, a.hq, a.hkv, a.dim);
     a.part = a.delta + ((int64_t)a.hq * a.rows_q + 3) / 4 * 4;
     if (packed_exact(a)) {
-        if (a.dim <= 32) return packed_dkv_dispatch<32, 1, 1, true>(a, stream);
-        if (a.dim <= 64) return packed_dkv_dispatch<64, 1, 1, true>(a, stream);
-        if (a.dim <= 96) return packed_dkv_dispatch<96, 1, 1, true>(a, stream);
-        return packed_dkv_dispatch<128, 1, 1, true>(a, stream);
+        if (a.dim <= 32) return packed_dkv_dispatch<32, 1, 2, 1, true>(a, stream);
+        if (a.dim <= 64) return packed_dkv_dispatch<64, 1, 2, 1, true>(a, stream);
+        if (a.dim <= 96) return packed_dkv_dispatch<96, 1, 1, 1, true>(a, stream);
+        return packed_dkv_dispatch<128, 1, 1, 1, true>(a, stream);
     }
-    if (a.dim <= 32) return packed_dkv_dispatch<32, 1, 3>(a, stream);
-    if (a.dim <= 64) return packed_dkv_dispatch<64, 1, 3>(a, stream);
-    if (a.dim <= 96) return packed_dkv_dispatch<96, 2, 1>(a, stream);
-    return packed_dkv_dispatch<128, 2, 1>(a, stream);
+    if (packed_few(a.rows_q, a.hq, 512)) {
+        if (a.dim <= 32) return packed_dkv_dispatch<32, 1, 2, 3>(a, stream);
+        if (a.dim <= 64) return packed_dkv_dispatch<64, 1, 2, 3>(a, stream);
+    }
+    if (a.dim <= 32) return packed_dkv_dispatch<32, 1, 1, 3>(a, stream);
+    if (a.dim <= 64) return packed_dkv_dispatch<64, 1, 1, 3>(a, stream);
+    if (a.dim <= 96) return packed_dkv_dispatch<96, 2, 1, 1>(a, stream);
+    return packed_dkv_dispatch<128, 2, 1, 1>(a, stream);
 }

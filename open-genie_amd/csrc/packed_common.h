@@ -171,6 +171,9 @@ static inline int packed_launch(K kernel, const PackedArgs& a, int64_t blocks, i
 // Few rows: P and dS go into their products with what their rounding left over, too (variants with REST).  Over many rows that rounding makes the error sqrt(2) times that of
 // rounding the result alone; over a handful of values it can be any value's worst.  Measured with / without: sequences of 2, 2 and 2 tokens dQ 0.0018 / 0.0026 off in
 // norm (the best bf16 result: 0.0018); three snippets of 33 tokens together 5.3 / 5.2 us; a batch of 5720 tokens would pay (forward 43 / 31, dQ 48 / 34, dK and dV 62 / 42 us).
-static inline bool packed_exact(const PackedArgs& a) { return a.rows_q <= 512 && a.rows_k <= 512; }
+static inline bool packed_exact(const PackedArgs& a) { return a.rows_q <= 256 && a.rows_k <= 256; }
+
+// few enough blocks of 128 rows that blocks half as tall (head widths up to 64), whose chain of steps takes half as long, pay: see the rules where it is called
+static inline bool packed_few(int rows, int heads, int64_t most) { return (int64_t)(rows / 128) * heads <= most; }
 
 int packed_dkv_run(PackedArgs& a, void* stream);     // packed_attention_dkv.hip

@@ -559,10 +559,10 @@ def test_offsets_past_32_bits_in_a_long_cache():
     assert torch.equal(gf.decay_attention(wide, wide, wide, ld, _cu([rows])), gf.decay_attention(dense, dense, dense, ld, _cu([rows])))
 
 
-@pytest.mark.parametrize('lens, spare', [([2, 2, 3], 0), ([1, 0, 31], 5), ([70, 130, 57, 255], 0)], ids=str)
+@pytest.mark.parametrize('lens, spare', [([2, 2, 3], 0), ([1, 0, 31], 5), ([70, 130, 56], 0), ([256], 0)], ids=str)
 @pytest.mark.parametrize('d', [32, 64, 80, 128])
 def test_few_rows_round_nothing_but_their_results(lens, spare, d):
-    """Up to 512 rows the weights go into the products with their rounding's remainder (U^2 of them is left), in the cached form always."""
+    """Up to 256 rows the weights go into the products with their rounding's remainder (U^2 of them is left), in the cached form always."""
     gf, w = _gf(), R.U ** 2
     q, k, v, g = _packed_inputs(lens, spare, 4, 2, d, 700)
     cu, rows, tiny = _cu(lens), sum(lens), 2.0 ** -100
