@@ -189,11 +189,13 @@ __global__ void __launch_bounds__(64 * (DH / 32), 2) decay_state_kernel(const De
 }
 
 // States in front of the segments: M_0 = initial or 0, M_{i+1} = l^256 M_i + local_i, elementwise in fp32; each M_i is stored rounded to bf16 as the operand that it
-// becomes, the last sum is the final state.  A lane owns four elements, the block's four waves take eight segments each of 32 at a time: all 32 loads of a
-// step are in flight together, the waves' sums meet in LDS, and each wave walks its own eight from there.  (One wave walking all of them, eight loads ahead: 18 us
-// for 128 segments of 8 heads of width 64 -- a chain of store and load latencies.)
-__global__ void __launch_bounds__(256) decay_scan_kernel(const DecayArgs g) {
-    __shared__ __attribute__((aligned(16))) f32x4_t part[2][4][64];
+// becomes, the last sum is the final state.  A lane owns four elements, the block's NW waves take eight segments each: all loads of a step are in flight
+// together, the waves' sums meet in LDS, and each wave walks its own eight from there.  128 segments of 8 heads of width 64: 16 waves 8.2 us, 4 waves 9.8, one wave walking all
+// of them, eight loads ahead, 18 -- a chain of store and load latencies.  Up to 32 segments a sequence four waves do it in one step: 100 MB of 63 segments of 16 heads of
+// width 128 in 21 us = 4.8 TB/s.
+template <int NW>
+__global__ void __launch_bounds__(64 * NW) decay_scan_kernel(const DecayArgs g) {
+    __shared__ __attribute__((aligned(16))) f32x4_t part[2][NW][64];
     const DecayRole& R = g.r[0];
     const int seq = (int)blockIdx.x / g.heads, head = (int)blockIdx.x % g.heads, matrix = R.da * R.dc;
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -212,7 +214,7 @@ __global__ void __launch_bounds__(256) decay_scan_kernel(const DecayArgs g) {
     bf16_t* dst = R.states + first;
     const int full = nseg - 1;                                                  // segments whose sum is followed by another segment
     const float l8 = decay_pow(log2_l, 8 * DECAY_SEG);
-    for (int base = 0, flip = 0; base < full; base += 32, flip ^= 1) {
+    for (int base = 0, flip = 0; base < full; base += 8 * NW, flip ^= 1) {
         const int i0 = base + wave * 8, n = min(8, full - i0);
         f32x4_t x[8], sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -227,7 +229,7 @@ __global__ void __launch_bounds__(256) decay_scan_kernel(const DecayArgs g) {
         __syncthreads();
         f32x4_t mine = m;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < NW; ++w) {
             if (w == wave) mine = m;
             const int nw = min(8, full - base - w * 8);
             if (nw > 0) {
@@ -544,7 +546,8 @@ static int decay_run(const DecayArgs& g, void* stream) {
     }
     if (g.nseq > 0 && r.local) {
         const dim3 grid((unsigned)(g.nseq * g.heads), (unsigned)((r.da * r.dc + 255) / 256));
-        hipLaunchKernelGGL(decay_scan_kernel, grid, dim3(256), 0, (hipStream_t)stream, g);
+        if (g.rows > 32ll * DECAY_SEG * g.nseq) hipLaunchKernelGGL((decay_scan_kernel<16>), grid, dim3(1024), 0, (hipStream_t)stream, g);
+        else hipLaunchKernelGGL((decay_scan_kernel<4>), grid, dim3(256), 0, (hipStream_t)stream, g);
         GENIE_CHECK_LAUNCH();
     }
     // few rows: the weights with what their rounding left over, for the reason at packed_exact() (a 32768-token prompt would pay 38 us for 33)

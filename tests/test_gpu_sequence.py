@@ -340,6 +340,12 @@ def test_decay_attention_long():
     _check_decay([3000, 17], 0, 2, 64, 64, 40, False)
 
 
+@pytest.mark.parametrize('lens', [[33100], [17000, 40], [8193]], ids=str)
+def test_decay_attention_many_segments(lens):
+    """More segments of 256 tokens than one step of the state scan takes (32, or 128 in sequences that long)."""
+    _check_decay(lens, 0, 1, 16, 16, 45, True)
+
+
 def test_decay_attention_layouts():
     gf, lens, d, h = _gf(), [70, 230], 64, 4
     fused = _randn(300, 3, h, d, seed=50).requires_grad_(True)
