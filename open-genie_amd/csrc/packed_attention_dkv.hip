@@ -87,59 +87,128 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, W
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) { sacc[kt][4 * g + e] = x[e]; dp[kt][4 * g + e] = y[e]; }
         }
+        if constexpr (VLDS) {
+            // Four runs of products -- S, dP with the exponentials, dV with dS, dK -- as one chain of stages of KT products.  A stage's LDS fragments are requested in the stage
+            // before, and the compiler may not move them back behind its products: with one wave per SIMD nobody else hides their latency (4 x 4096 rows, 16 / 4 heads:
+            // 600 us; in the order below 700; requested two stages ahead 605).
+            static_assert(!REST, "weights are one bf16 value here");
+            constexpr int KS = G::KS, DT = G::DT, NS = 2 * KS + 4 * DT, N = 16 * KT;
+            bf16x8_t fr[NS], vr[KT][KS], pf[KT][2], ds[KT][2];
+            auto fetch = [&](int n) __attribute__((always_inline)) {
+                if (n < KS) fr[n] = at.row_frag(qt_, n);
+                else if (n < 2 * KS) {
+                    fr[n] = at.row_frag(gt_, n - KS);
 #pragma unroll
-        for (int ks = 0; ks < G::KS; ++ks) {
-            const bf16x8_t qa = at.row_frag(qt_, ks), ga = at.row_frag(gt_, ks);
+                    for (int kt = 0; kt < KT; ++kt) vr[kt][n - KS] = at.row_frag(vt_ + kt * 32 * G::PITCH, n - KS);
+                } else if (n < 2 * KS + 2 * DT) fr[n] = at.tr_frag(gt_ + (n - 2 * KS) / DT * 16 * G::PITCH, (n - 2 * KS) % DT);
+                else if (n < NS) fr[n] = at.tr_frag(qt_ + (n - 2 * KS - 2 * DT) / DT * 16 * G::PITCH, (n - 2 * KS) % DT);
+            };
+            fetch(0);
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-                sacc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qa, kf[kt][ks], sacc[kt], 0, 0, 0);
-                dp[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ga, VLDS ? at.row_frag(vt_ + kt * 32 * G::PITCH, ks) : vf[VLDS ? 0 : kt][ks], dp[kt], 0, 0, 0);
-            }
-        }
-        if (rbase < w_first + 32 * KT - 1) {                                    // some of these rows do not see all of the wave's keys
+            for (int n = 0; n < NS; ++n) {
+                fetch(n + 1);
+                __builtin_amdgcn_sched_barrier(0);
+                if (n < KS) {
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt) {
-                int lim = kj + 32 * kt - shift - rbase - 4 * h;                 // rows below do not see this lane's key
-                asm volatile("" : "+v"(lim));
+                    for (int kt = 0; kt < KT; ++kt) sacc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr[n], kf[kt][n], sacc[kt], 0, 0, 0);
+                    if (n == KS - 1 && rbase < w_first + 32 * KT - 1) {             // some of these rows do not see all of the wave's keys
 #pragma unroll
-                for (int r = 0; r < 16; ++r) sacc[kt][r] = seq_crow(r) >= lim ? sacc[kt][r] : -INFINITY;
-            }
-        }
-        bf16x8_t pf[KT][2], ds[KT][2], pr[REST ? KT : 1][2], dr[REST ? KT : 1][2];
+                        for (int kt = 0; kt < KT; ++kt) {
+                            int lim = kj + 32 * kt - shift - rbase - 4 * h;         // rows below do not see this lane's key
+                            asm volatile("" : "+v"(lim));
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
+                            for (int r = 0; r < 16; ++r) sacc[kt][r] = seq_crow(r) >= lim ? sacc[kt][r] : -INFINITY;
+                        }
+                    }
+                } else if (n < 2 * KS) {
+                    const int ks = n - KS;
 #pragma unroll
-            for (int s2 = 0; s2 < 2; ++s2) {
-                float p[8], x[8];
+                    for (int kt = 0; kt < KT; ++kt) dp[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr[n], vr[kt][ks], dp[kt], 0, 0, 0);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int r = 8 * s2 + e;
-                    p[e] = __builtin_amdgcn_exp2f(sacc[kt][r] * c2);
-                    x[e] = p[e] * dp[kt][r];
+                    for (int e = ks * N / KS; e < (ks + 1) * N / KS; ++e) {
+                        sacc[e / 16][e % 16] = __builtin_amdgcn_exp2f(sacc[e / 16][e % 16] * c2);
+                        if (e % 8 == 7) {
+                            const int kt = e / 16, s2 = e / 8 % 2;
+                            const float p[8] = {sacc[kt][8 * s2], sacc[kt][8 * s2 + 1], sacc[kt][8 * s2 + 2], sacc[kt][8 * s2 + 3], sacc[kt][8 * s2 + 4], sacc[kt][8 * s2 + 5],
+                                                sacc[kt][8 * s2 + 6], sacc[kt][8 * s2 + 7]};
+                            pf[kt][s2] = seq_pack8(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]);
+                        }
+                    }
+                } else if (n < 2 * KS + 2 * DT) {
+                    const int i = n - 2 * KS, s2 = i / DT, d = i % DT;
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) dv[kt][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr[n], pf[kt][s2], dv[kt][d], 0, 0, 0);
+#pragma unroll
+                    for (int e = i * N / (2 * DT); e < (i + 1) * N / (2 * DT); ++e) {
+                        dp[e / 16][e % 16] *= sacc[e / 16][e % 16];
+                        if (e % 8 == 7) {
+                            const int kt = e / 16, s2 = e / 8 % 2;
+                            const float x[8] = {dp[kt][8 * s2], dp[kt][8 * s2 + 1], dp[kt][8 * s2 + 2], dp[kt][8 * s2 + 3], dp[kt][8 * s2 + 4], dp[kt][8 * s2 + 5],
+                                                dp[kt][8 * s2 + 6], dp[kt][8 * s2 + 7]};
+                            ds[kt][s2] = seq_pack8(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
+                        }
+                    }
+                } else {
+                    const int i = n - 2 * KS - 2 * DT, s2 = i / DT, d = i % DT;
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) dk[kt][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr[n], ds[kt][s2], dk[kt][d], 0, 0, 0);
                 }
-                pf[kt][s2] = seq_pack8(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]);
-                ds[kt][s2] = seq_pack8(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
-                if (REST) {
-                    pr[REST ? kt : 0][s2] = seq_rest8(p, pf[kt][s2]);
-                    dr[REST ? kt : 0][s2] = seq_rest8(x, ds[kt][s2]);
-                }
             }
-        }
+        } else {
 #pragma unroll
-        for (int s2 = 0; s2 < 2; ++s2)
-#pragma unroll
-            for (int d = 0; d < G::DT; ++d) {
-                const bf16x8_t gt = at.tr_frag(gt_ + s2 * 16 * G::PITCH, d), qt = at.tr_frag(qt_ + s2 * 16 * G::PITCH, d);
+            for (int ks = 0; ks < G::KS; ++ks) {
+                const bf16x8_t qa = at.row_frag(qt_, ks), ga = at.row_frag(gt_, ks);
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) {
-                    if (REST) {
-                        dv[kt][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(gt, pr[REST ? kt : 0][s2], dv[kt][d], 0, 0, 0);
-                        dk[kt][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qt, dr[REST ? kt : 0][s2], dk[kt][d], 0, 0, 0);
-                    }
-                    dv[kt][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(gt, pf[kt][s2], dv[kt][d], 0, 0, 0);
-                    dk[kt][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qt, ds[kt][s2], dk[kt][d], 0, 0, 0);
+                    sacc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qa, kf[kt][ks], sacc[kt], 0, 0, 0);
+                    dp[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ga, vf[kt][ks], dp[kt], 0, 0, 0);
                 }
             }
+            if (rbase < w_first + 32 * KT - 1) {                                    // some of these rows do not see all of the wave's keys
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt) {
+                    int lim = kj + 32 * kt - shift - rbase - 4 * h;                 // rows below do not see this lane's key
+                    asm volatile("" : "+v"(lim));
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sacc[kt][r] = seq_crow(r) >= lim ? sacc[kt][r] : -INFINITY;
+                }
+            }
+            bf16x8_t pf[KT][2], ds[KT][2], pr[REST ? KT : 1][2], dr[REST ? KT : 1][2];
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt) {
+#pragma unroll
+                for (int s2 = 0; s2 < 2; ++s2) {
+                    float p[8], x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int r = 8 * s2 + e;
+                        p[e] = __builtin_amdgcn_exp2f(sacc[kt][r] * c2);
+                        x[e] = p[e] * dp[kt][r];
+                    }
+                    pf[kt][s2] = seq_pack8(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]);
+                    ds[kt][s2] = seq_pack8(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
+                    if (REST) {
+                        pr[REST ? kt : 0][s2] = seq_rest8(p, pf[kt][s2]);
+                        dr[REST ? kt : 0][s2] = seq_rest8(x, ds[kt][s2]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+                for (int d = 0; d < G::DT; ++d) {
+                    const bf16x8_t gt = at.tr_frag(gt_ + s2 * 16 * G::PITCH, d), qt = at.tr_frag(qt_ + s2 * 16 * G::PITCH, d);
+#pragma unroll
+                    for (int kt = 0; kt < KT; ++kt) {
+                        if (REST) {
+                            dv[kt][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(gt, pr[REST ? kt : 0][s2], dv[kt][d], 0, 0, 0);
+                            dk[kt][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qt, dr[REST ? kt : 0][s2], dk[kt][d], 0, 0, 0);
+                        }
+                        dv[kt][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(gt, pf[kt][s2], dv[kt][d], 0, 0, 0);
+                        dk[kt][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qt, ds[kt][s2], dk[kt][d], 0, 0, 0);
+                    }
+                }
+        }
     };
 
     if (i0 < i1) load(i0);
