@@ -269,10 +269,18 @@ __global__ void __launch_bounds__(64 * RW * NG, WPE) packed_dq_kernel(const Pack
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
             f32x16_t sacc = packed_splat(0.f), dp = packed_splat(-delta);
+            bf16x8_t ka[G::KS], va[G::KS];                                      // (a product's fragments are requested one product ahead: 4 x 4096 rows 397 us, else 408)
+            ka[0] = at.row_frag(kt_ + kt * 32 * G::PITCH, 0);
+            va[0] = at.row_frag(vt_ + kt * 32 * G::PITCH, 0);
 #pragma unroll
             for (int ks = 0; ks < G::KS; ++ks) {
-                sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at.row_frag(kt_ + kt * 32 * G::PITCH, ks), qf[ks], sacc, 0, 0, 0);
-                dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at.row_frag(vt_ + kt * 32 * G::PITCH, ks), gf[ks], dp, 0, 0, 0);
+                if (ks + 1 < G::KS) {
+                    ka[ks + 1] = at.row_frag(kt_ + kt * 32 * G::PITCH, ks + 1);
+                    va[ks + 1] = at.row_frag(vt_ + kt * 32 * G::PITCH, ks + 1);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[ks], qf[ks], sacc, 0, 0, 0);
+                dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[ks], gf[ks], dp, 0, 0, 0);
             }
             if (k0 + 64 > r.klen || k0 + 63 > r.q0 + r.shift) {
                 int lim = min(r.klen, r.qi + r.shift + 1) - k0 - 32 * kt - 4 * h;
@@ -289,11 +297,16 @@ __global__ void __launch_bounds__(64 * RW * NG, WPE) packed_dq_kernel(const Pack
                 ds[s2] = seq_pack8(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
                 if (REST) dr[REST ? s2 : 0] = seq_rest8(x, ds[s2]);
             }
+            bf16x8_t kfr[2 * G::DT];
+            kfr[0] = at.tr_frag(kt_ + kt * 32 * G::PITCH, 0);
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
                 for (int d = 0; d < G::DT; ++d) {
-                    const bf16x8_t kf = at.tr_frag(kt_ + (kt * 2 + s2) * 16 * G::PITCH, d);
+                    const int n = s2 * G::DT + d;
+                    if (n + 1 < 2 * G::DT) kfr[n + 1] = at.tr_frag(kt_ + (kt * 2 + (n + 1) / G::DT) * 16 * G::PITCH, (n + 1) % G::DT);
+                    __builtin_amdgcn_sched_barrier(0);
+                    const bf16x8_t kf = kfr[n];
                     if (REST) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, dr[REST ? s2 : 0], acc[d], 0, 0, 0);
                     acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, ds[s2], acc[d], 0, 0, 0);
                 }
