@@ -307,13 +307,13 @@ __global__ void __launch_bounds__(256) packed_dkv_sum_kernel(const PackedArgs a)
 
 // Parts that a key tile's (head, row tile) steps are cut into.  A launch takes the longest chain of steps (all sequences taken as equally long), or the time that all pairs take on a
 // full chip, whichever is longer; parts shorten the chain and cost a second launch and their fp32 sums written and read.  The rates are
-// measured: a step 1 us (64 keys per block), 2 us (128) or 4.7 us (256, width 128), 0.56 or 1.14 us per million pairs, 5 us, 6 TB/s.  The model's order of n = 1 .. 8 was the measured one
-// for every batch tried, e.g. 4 x 700 rows, 8 / 8 heads of width 64, n = 1, 2, 3: 33 / 40 / 44 us the whole backward; 16 / 4 heads, n = 3, 4, 5, 8: 57 / 55 / 56 / 64.
+// measured: a step 1 us (64 keys per block), 2 us (128) or 4.2 us (256, width 128), 0.56 or 1 us per million pairs, 5 us, 6 TB/s.  The model agreed with the measured order
+// of n = 1 .. 8 on ten batches, e.g. 4 x 700 rows, 8 / 8 heads of width 64, n = 1, 2, 3: 33 / 40 / 44 us the whole backward; 16 / 4 heads, n = 3, 4, 5, 8: 57 / 55 / 56 / 64.
 static int packed_dkv_splits(int nseq, int rows_q, int rows_k, int hq, int hkv, int dim) {
     const float length = (float)rows_q / (float)(nseq > 0 ? nseq : 1);
-    const float step = dim > 64 ? 4.7f * (float)dim / 128.f : packed_few(rows_q, hq, 512) ? 1.f : 2.f;
+    const float step = dim > 64 ? 4.2f * (float)dim / 128.f : packed_few(rows_q, hq, 512) ? 1.f : 2.f;
     const float chain = (length / 64.f + 1.f) * (float)(hq / hkv) * step;
-    const float all = (float)rows_q * length * 0.5f * (float)hq * (dim > 64 ? 1.14e-6f : 0.56e-6f);
+    const float all = (float)rows_q * length * 0.5f * (float)hq * (dim > 64 ? 1e-6f : 0.56e-6f);
     const float part = (float)rows_k * (float)hkv * (float)dim * 16.f / 6e6f;
     int best = 1;
     float least = 0.f;

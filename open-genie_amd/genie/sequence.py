@@ -127,6 +127,16 @@ def _no_grad_wanted(what: str, *tensors: Optional[Tensor]) -> None:
         raise RuntimeError(f'{what} has no backward pass: call it under torch.no_grad(), or on tensors that do not require gradients')
 
 
+def _first_order(backward):
+    """``once_differentiable``, whose bookkeeping (3 us of a small training call's 120) only runs where a graph of the backward pass is asked for."""
+    recorded = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
 # ------------------------------------------------------------------------------------------------------------------------------------
 # causal attention over packed sequences
 # ------------------------------------------------------------------------------------------------------------------------------------
@@ -136,15 +146,16 @@ def _packed_forward(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Tensor,
     rows_k, hkv, _ = k.shape
     (q, sq), (k, sk), (v, sv) = _rows(q), _rows(k), _rows(v)
     out = torch.empty((rows, hq, d), dtype=torch.bfloat16, device=q.device)
-    lse = torch.empty((hq, rows), dtype=torch.float32, device=q.device) if keep else None
-    out_lo = torch.empty_like(out) if keep else None
+    # for the backward pass, in one buffer: what out's rounding left over (bf16, rows x hq x d), then the log-sum-exps (fp32, hq x rows)
+    rest = torch.empty(rows * hq * (d // 2 + 1), dtype=torch.float32, device=q.device) if keep else None
     if rows and rows_k:
         P = _hip.ptr
-        _launch('genie_packed_attention_fwd', q.device, P(q), P(k), P(v), P(out), P(out_lo), P(lse), P(cu_q), P(cu_k), cu_q.shape[0] - 1, rows, rows_k, hq, hkv, d,
+        lo = P(rest)
+        _launch('genie_packed_attention_fwd', q.device, P(q), P(k), P(v), P(out), lo, lo + rows * hq * d * 2 if keep else None, P(cu_q), P(cu_k), cu_q.shape[0] - 1, rows, rows_k, hq, hkv, d,
                 _i64(sq), _i64(sk), _i64(sv), scale)
     else:
         out.zero_()
-    return out, ((q, k, v, out, out_lo, lse, cu_q, cu_k), (sq, sk, sv, scale)) if keep else None
+    return out, ((q, k, v, out, rest, cu_q, cu_k), (sq, sk, sv, scale)) if keep else None
 
 
 class _PackedAttention(torch.autograd.Function):
@@ -155,9 +166,9 @@ class _PackedAttention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dout: Tensor):
-        q, k, v, out, out_lo, lse, cu_q, cu_k = ctx.saved_tensors
+        q, k, v, out, rest, cu_q, cu_k = ctx.saved_tensors
         sq, sk, sv, scale = ctx.cfg
         rows, hq, d = q.shape
         rows_k, hkv, _ = k.shape
@@ -167,9 +178,10 @@ class _PackedAttention(torch.autograd.Function):
         dv = torch.empty_like(dk)
         if rows and rows_k:
             P = _hip.ptr
+            lo = P(rest)
             nws = _hip.load_library().genie_packed_attention_bwd_ws_floats(cu_q.shape[0] - 1, rows, rows_k, hq, hkv, d)
             ws = torch.empty(nws, dtype=torch.float32, device=q.device)
-            _launch('genie_packed_attention_bwd', q.device, P(q), P(k), P(v), P(out), P(out_lo), P(dout), P(lse), P(ws), nws, P(dq), P(dk), P(dv), P(cu_q), P(cu_k),
+            _launch('genie_packed_attention_bwd', q.device, P(q), P(k), P(v), P(out), lo, P(dout), lo + rows * hq * d * 2, P(ws), nws, P(dq), P(dk), P(dv), P(cu_q), P(cu_k),
                     cu_q.shape[0] - 1, rows, rows_k, hq, hkv, d, _i64(sq), _i64(sk), _i64(sv), _i64(sg), scale)
         else:
             for t in (dq, dk, dv):
@@ -316,7 +328,7 @@ class _DecayAttention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dout: Tensor, *_):
         q, k, v, log_decay, cu, states = ctx.saved_tensors
         sq, sk, sv, scale, has_initial = ctx.cfg

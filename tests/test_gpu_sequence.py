@@ -593,3 +593,16 @@ def test_few_rows_round_nothing_but_their_results(lens, spare, d):
     n = torch.tensor([600, 3], dtype=torch.int32, device='cuda')
     val, tol = R.step_reference(g[:2], cache[0], cache[1], [600, 3], d ** -0.5, w=w)
     R.assert_within(gf.cached_attention_step(g[:2].contiguous(), cache[0], cache[1], n), val, tol + tiny, 'step')
+
+
+def test_gradients_of_gradients_are_refused():
+    """A recorded backward pass gives the same gradients, and says so when they are differentiated in their turn."""
+    gf = _gf()
+    q, k, v, g = (_randn(40, 2, 32, seed=800 + i).requires_grad_(i < 3) for i in range(4))
+    decay = torch.full((2,), -0.1, device='cuda')
+    for call in (lambda: gf.packed_attention(q, k, v, _cu([30, 10])), lambda: gf.decay_attention(q, k, v, decay, _cu([30, 10]))):
+        plain = torch.autograd.grad(call(), (q, k, v), g)
+        recorded = torch.autograd.grad(call(), (q, k, v), g, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(plain, recorded))
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(recorded[0].float().sum(), q)
