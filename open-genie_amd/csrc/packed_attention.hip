@@ -3,11 +3,16 @@
 //   o_i = sum_{j <= i + Lk - Lq} softmax_j(scale q_i . k_j) v_j          per sequence and head; key head = head / (Hq / Hkv)
 //   dV = P^T dO,  dS = P o (dO V^T - rowsum(dO o O)),  dQ = scale dS K,  dK = scale dS^T Q
 //
-// One wave owns 32 query rows (forward, dQ) or 32 key rows (dK / dV); the 64-row tiles of the other side pass through LDS, double-buffered, staged
-// through registers (global load of tile t + 1 in flight under the products of tile t).  "Swapped" products: S^T = K Q^T puts one query into one
+// One wave owns 32 query rows (forward, dQ) or 32 or 64 key rows (dK / dV); the 64-row tiles of the other side pass through LDS, double-buffered and written there by the
+// loads themselves (tile t + 1 in flight under the products of tile t).  "Swapped" products: S^T = K Q^T puts one query into one
 // lane's column, so that softmax is lane-local, and the accumulator layout of P^T is, up to a fixed order of the contraction index, the operand
 // layout of the second product -- the transposed V / K / dO / Q fragments are read in that order by ds_read_b64_tr_b16, nothing is exchanged.
 // The sequences' lengths live on the device only: seq_common.h maps slots to (sequence, tile).
+//
+// Bound by the matrix cores on long sequences: 16384 rows, 8 heads of width 64, forward 297 us = 925 TFLOP/s of the products it needs; 4 x 4096 rows, 16 heads of width 128 over 4
+// key heads: forward 295 us = 930, dQ 388 us = 1060, dK / dV 570 us + 25 us for the parts' sums = 920 TFLOP/s of the products they do (bf16 library products of 8192^3 and
+// more reach 1340 here).  On short ones by the chain of a sequence's tiles (7 ragged sequences of up to 2048 rows: 27, 30 and 42 + 6 us against 21 us of products in all), and under
+// 256 rows by the launch.
 #include "packed_common.h"
 
 // ------------------------------------------------------------------------------------------------------------------------------
