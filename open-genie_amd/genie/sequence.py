@@ -20,6 +20,9 @@ Common conventions
   * a tensor whose rows are not 16-byte aligned, or whose last axis is not contiguous, is copied first; slices of a fused projection are taken as they are.
   * the kernels run on the current stream of the tensors' device; scratch memory is allocated per call (a captured graph owns its own).
   * bitwise reproducible: no atomics, every sum has a fixed order.
+  * capture of a backward pass into a graph: with no eager autograd graph of the same leaves alive (torch ends the process where it meets a leaf's node of another
+    stream inside a capture; this holds for every differentiable operator).
+  * weights (P, dS, decayed scores) are bf16 operands; up to 256 rows, and in the cached form, a second bf16 value carries what that left over.
   * a non-finite value in a token is not masked out: it may reach any row of its own sequence.
 """
 from __future__ import annotations

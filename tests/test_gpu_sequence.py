@@ -606,3 +606,57 @@ def test_gradients_of_gradients_are_refused():
         assert all(torch.equal(a, b) for a, b in zip(plain, recorded))
         with pytest.raises(RuntimeError):
             torch.autograd.grad(recorded[0].float().sum(), q)
+
+
+@pytest.mark.parametrize('rows', [200, 900])
+def test_two_captured_graphs_at_once(rows):
+    """Two captures of the same calls replayed at the same time on two streams: nothing is shared between them."""
+    cu = _cu([rows // 3, 1, rows - rows // 3 - 1])
+    inputs = [_everything_inputs(rows, 3, seed=900 + 10 * i) for i in range(2)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _everything(**inputs[0], cu=cu)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs, got = [], []
+    for x in inputs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            got.append(_everything(**x, cu=cu))
+    streams = [torch.cuda.Stream() for _ in inputs]
+    for _ in range(3):
+        for t in (t for each in got for t in each):
+            t.fill_(7.0)
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        kept = [[t.clone() for t in each] for each in got]
+        for each, x in zip(kept, inputs):
+            for a, b in zip(each, _everything(**x, cu=cu)):
+                assert torch.equal(a, b)
+
+
+def test_calls_from_two_threads():
+    """Two host threads, each on its own stream, through the same operators."""
+    import threading
+    cu = _cu([300, 1, 599])
+    inputs = [_everything_inputs(900, 3, seed=950 + 10 * i) for i in range(2)]
+    want = [[t.clone() for t in _everything(**x, cu=cu)] for x in inputs]
+    torch.cuda.synchronize()
+    same = [False, False]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            runs = [_everything(**inputs[i], cu=cu) for _ in range(5)]
+            torch.cuda.current_stream().synchronize()
+            same[i] = all(torch.equal(a, b) for r in runs for a, b in zip(r, want[i]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert same == [True, True]
