@@ -75,10 +75,10 @@ def _check_cu(what: str, cu: Tensor, name: str, device: torch.device) -> None:
 
 
 def _strides(t: Tensor) -> Optional[Tuple[int, ...]]:
-    """Element strides of all axes but the last as the kernels take them, or None where the layout has to be copied.  An axis of one entry takes the stride it
-    would have in a dense tensor."""
+    """Element strides of all axes but the last as the kernels take them, or None where the layout (alignment of the first element aside) has to be copied.  An axis
+    of one entry takes the stride it would have in a dense tensor."""
     *lead, last = t.stride()
-    if last != 1 or t.data_ptr() % 16:
+    if last != 1:
         return None
     shape = t.shape
     if 1 in shape:
@@ -93,16 +93,21 @@ def _strides(t: Tensor) -> Optional[Tuple[int, ...]]:
     return tuple(lead)
 
 
+def _direct(t: Tensor) -> Optional[Tuple[int, ...]]:
+    """Strides of (rows, heads, d) or (batch, heads, d) if the kernels can take it as it is, its alignment aside."""
+    st = _strides(t)
+    # (a row stride under the head width -- rows that overlap or repeat -- would let a tile's last rows be read past its sequence)
+    return st if st is not None and t.shape[2] <= st[0] < _MAX_STRIDE else None
+
+
 def _rows(t: Tensor) -> Tuple[Tensor, Tuple[int, ...]]:
     """(rows, heads, d) or (batch, heads, d) ready for the kernels: the tensor itself where its layout allows, else a contiguous copy."""
-    st = _strides(t)
-    if st is None or not t.shape[2] <= st[0] < _MAX_STRIDE:
-        # (a row stride under the head width -- rows that overlap or repeat -- would let a tile's last rows be read past its sequence)
-        t = t.contiguous()
+    st = _direct(t)
+    if st is None or t.data_ptr() % 16:
+        t = t.contiguous() if st is None else t.clone(memory_format=torch.contiguous_format)
+        if t.data_ptr() % 16:                                     # contiguous all along, but its storage offset is not 16-byte aligned
+            t = t.clone()
         st = _strides(t)
-        if st is None:                                            # contiguous, but its storage offset is not 16-byte aligned
-            t = t.clone(memory_format=torch.contiguous_format)
-            st = _strides(t)
         if st[0] >= _MAX_STRIDE:
             raise ValueError(f'rows of {st[0]} elements are too long (limit {_MAX_STRIDE})')
     return t, st
@@ -123,6 +128,29 @@ def _launch(name: str, device: torch.device, *args) -> None:
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _hip.check(rc, name)
+
+
+def _sig(t: Optional[Tensor]):
+    return None if t is None else (t.dtype, t.get_device(), t.shape, t.stride())
+
+
+_PLANS: dict = {}
+
+
+def _planned(make, tensors, *rest):
+    """``make(*tensors, *rest)``: all checks of a call that its types, devices, shapes and strides decide, and what follows from them for the launch.  Kept for the calls
+    that look the same (a token's call: 18 us with the checks, 11 without); nothing in it depends on a tensor's address or contents."""
+    try:
+        key = (make, *map(_sig, tensors), *rest)
+    except AttributeError:                                        # not a tensor: the checks say so
+        return make(*tensors, *rest)
+    plan = _PLANS.get(key)
+    if plan is None:
+        plan = make(*tensors, *rest)
+        if len(_PLANS) >= 4096:
+            _PLANS.clear()
+        _PLANS[key] = plan
+    return plan
 
 
 def _no_grad_wanted(what: str, *tensors: Optional[Tensor]) -> None:
@@ -193,14 +221,8 @@ class _PackedAttention(torch.autograd.Function):
         return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None
 
 
-def packed_attention(q: Tensor, k: Tensor, v: Tensor, cu_seqlens: Tensor, scale: Optional[float] = None, cu_seqlens_k: Optional[Tensor] = None) -> Tensor:
-    """Causal softmax attention inside each packed sequence.
-
-    ``q`` (rows, Hq, d), ``k`` / ``v`` (rows_k, Hkv, d) bf16 with ``Hq`` a multiple of ``Hkv`` (query head h reads key head ``h // (Hq // Hkv)``), d a multiple of 8 up
-    to 128; ``scale`` defaults to ``d ** -0.5``.  Returns (rows, Hq, d) bf16; differentiable in q, k and v.
-
-    ``cu_seqlens_k``: the keys' own packing, where a sequence has other keys than queries -- a prompt that continues a context.  The last query then sees the
-    last key: query i of n sees keys ``0 .. i + n_k - n``.  A query that sees no key (``n_k < n``) returns zeros and has zero gradients."""
+def _packed_plan(q, k, v, cu_seqlens, cu_seqlens_k, scale):
+    """(scale, None or what a call takes whose tensors need no copy)"""
     what = 'packed_attention'
     _check(what, q, 'q', 3, torch.bfloat16)
     _check(what, k, 'k', 3, torch.bfloat16, q.device)
@@ -220,27 +242,42 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, cu_seqlens: Tensor, scale:
     if cu_seqlens_k is None:
         if rows != rows_k:
             raise ValueError(f'{what}: q and k have {q.shape[0]} and {k.shape[0]} rows (pass cu_seqlens_k for keys packed differently)')
-        cu_seqlens_k = cu_seqlens
     else:
         _check_cu(what, cu_seqlens_k, 'cu_seqlens_k', q.device)
         if cu_seqlens_k.shape != cu_seqlens.shape:
             raise ValueError(f'{what}: cu_seqlens and cu_seqlens_k describe different numbers of sequences')
     scale = _scale(what, scale, d)
+    strides = [_direct(t) for t in (q, k, v)]
+    if None in strides or not (rows and rows_k):
+        return scale, None
+    return scale, ((rows, hq, d), q.device, (cu_seqlens.shape[0] - 1, rows, rows_k, hq, hkv, d, *map(_i64, strides), scale))
+
+
+def packed_attention(q: Tensor, k: Tensor, v: Tensor, cu_seqlens: Tensor, scale: Optional[float] = None, cu_seqlens_k: Optional[Tensor] = None) -> Tensor:
+    """Causal softmax attention inside each packed sequence.
+
+    ``q`` (rows, Hq, d), ``k`` / ``v`` (rows_k, Hkv, d) bf16 with ``Hq`` a multiple of ``Hkv`` (query head h reads key head ``h // (Hq // Hkv)``), d a multiple of 8 up
+    to 128; ``scale`` defaults to ``d ** -0.5``.  Returns (rows, Hq, d) bf16; differentiable in q, k and v.
+
+    ``cu_seqlens_k``: the keys' own packing, where a sequence has other keys than queries -- a prompt that continues a context.  The last query then sees the
+    last key: query i of n sees keys ``0 .. i + n_k - n``.  A query that sees no key (``n_k < n``) returns zeros and has zero gradients."""
+    scale, direct = _planned(_packed_plan, (q, k, v, cu_seqlens, cu_seqlens_k), None if scale is None else float(scale))
+    if cu_seqlens_k is None:
+        cu_seqlens_k = cu_seqlens
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _PackedAttention.apply(q, k, v, cu_seqlens, cu_seqlens_k, scale)
+    if direct is not None:
+        shape, device, sizes = direct
+        ptrs = q.data_ptr(), k.data_ptr(), v.data_ptr()
+        if not (ptrs[0] | ptrs[1] | ptrs[2]) % 16:
+            out = torch.empty(shape, dtype=torch.bfloat16, device=device)
+            _launch('genie_packed_attention_fwd', device, *ptrs, out.data_ptr(), None, None, cu_seqlens.data_ptr(), cu_seqlens_k.data_ptr(), *sizes)
+            return out
     return _packed_forward(q, k, v, cu_seqlens, cu_seqlens_k, scale, False)[0]
 
 
-def cached_attention_step(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: Tensor, k_new: Optional[Tensor] = None, v_new: Optional[Tensor] = None,
-                          scale: Optional[float] = None) -> Tensor:
-    """Softmax attention of one new token per sequence against its cache.
-
-    ``q`` (B, Hq, d); ``k_cache`` / ``v_cache`` (B, capacity, Hkv, d) bf16, any strides with a contiguous last axis; ``lengths`` (B,) int32: tokens already in each cache.
-    With ``k_new`` / ``v_new`` (B, Hkv, d) the token is written to place ``lengths[b]`` of the caches and attended to as well -- ``lengths`` itself is left alone (the
-    caller advances it once for all layers).  Rows of the caches from the length on are not read.  Returns (B, Hq, d) bf16; no backward pass.
-
-    An unused row of the batch has a negative length (without a new token: or zero): it returns zeros and its caches stay as they are.  A length that leaves no room
-    in the cache returns NaN and writes nothing -- the lengths live on the device, so a full cache cannot raise here."""
+def _cached_plan(q, k_cache, v_cache, lengths, k_new, v_new, scale):
+    """(device, the output's shape, floats of workspace, None or the strides of tensors that need no copy, (sizes, caches' strides, scale))"""
     what = 'cached_attention_step'
     _check(what, q, 'q', 3, torch.bfloat16)
     b, hq, d = q.shape
@@ -262,7 +299,6 @@ def cached_attention_step(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: 
         raise ValueError(f'{what}: lengths must be a contiguous tensor of {b} entries')
     if (k_new is None) != (v_new is None):
         raise ValueError(f'{what}: k_new and v_new come together')
-    _no_grad_wanted(what, q, k_cache, v_cache, k_new, v_new)
     scale = _scale(what, scale, d)
     cst = []
     for t, name in ((k_cache, 'k_cache'), (v_cache, 'v_cache')):
@@ -272,7 +308,7 @@ def cached_attention_step(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: 
         if not d <= st[1] < _MAX_STRIDE:
             raise ValueError(f'{what}: consecutive tokens of {name} are {st[1]} elements apart (from the head width up to {_MAX_STRIDE} is supported)')
         cst.append(st)
-    skn = svn = None
+    rows = [q]
     if k_new is not None:
         for t, name in ((k_new, 'k_new'), (v_new, 'v_new')):
             _check(what, t, name, 3, torch.bfloat16, dev)
@@ -281,30 +317,60 @@ def cached_attention_step(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: 
         for st, t, name in ((cst[0], k_cache, 'k_cache'), (cst[1], v_cache, 'v_cache')):
             if any(s == 0 and n > 1 for s, n in zip(st, t.shape)):
                 raise ValueError(f'{what}: {name} is an expanded view; a token cannot be appended to it')
-        if k_cache.data_ptr() == v_cache.data_ptr():
-            raise ValueError(f'{what}: k_cache and v_cache are the same memory')
-        (k_new, skn), (v_new, svn) = _rows(k_new), _rows(v_new)
-    q, sq = _rows(q)
-    out = torch.empty((b, hq, d), dtype=torch.bfloat16, device=dev)
-    if b == 0:
+        rows += [k_new, v_new]
+    direct = [_direct(t) for t in rows]
+    direct = None if None in direct else (*map(_i64, direct), None, None)[:3]
+    nws = _hip.load_library().genie_cached_attention_ws_floats(b, hq, hkv, d, cap)
+    return dev, (b, hq, d), nws, direct, ((b, hq, hkv, d, cap), (_i64(cst[0]), _i64(cst[1])), scale)
+
+
+def cached_attention_step(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: Tensor, k_new: Optional[Tensor] = None, v_new: Optional[Tensor] = None,
+                          scale: Optional[float] = None) -> Tensor:
+    """Softmax attention of one new token per sequence against its cache.
+
+    ``q`` (B, Hq, d); ``k_cache`` / ``v_cache`` (B, capacity, Hkv, d) bf16, any strides with a contiguous last axis; ``lengths`` (B,) int32: tokens already in each cache.
+    With ``k_new`` / ``v_new`` (B, Hkv, d) the token is written to place ``lengths[b]`` of the caches and attended to as well -- ``lengths`` itself is left alone (the
+    caller advances it once for all layers).  Rows of the caches from the length on are not read.  Returns (B, Hq, d) bf16; no backward pass.
+
+    An unused row of the batch has a negative length (without a new token: or zero): it returns zeros and its caches stay as they are.  A length that leaves no room
+    in the cache returns NaN and writes nothing -- the lengths live on the device, so a full cache cannot raise here."""
+    what = 'cached_attention_step'
+    new = k_new is not None
+    device, shape, nws, direct, tail = _planned(_cached_plan, (q, k_cache, v_cache, lengths, k_new, v_new), None if scale is None else float(scale))
+    _no_grad_wanted(what, q, k_cache, v_cache, k_new, v_new)
+    kc, vc = k_cache.data_ptr(), v_cache.data_ptr()
+    if (kc | vc) % 16:
+        raise ValueError(f'{what}: {"k_cache" if kc % 16 else "v_cache"} must have a contiguous last axis and 16-byte aligned rows (it is updated in place and cannot be copied)')
+    if new and kc == vc:
+        raise ValueError(f'{what}: k_cache and v_cache are the same memory')
+    out = torch.empty(shape, dtype=torch.bfloat16, device=device)
+    if shape[0] == 0:
         return out
-    lib = _hip.load_library()
-    nws = lib.genie_cached_attention_ws_floats(b, hq, hkv, d, cap)
-    ws = torch.empty(nws, dtype=torch.float32, device=dev) if nws else None
+    ws = torch.empty(nws, dtype=torch.float32, device=device) if nws else None
     P = _hip.ptr
-    _launch('genie_cached_attention_step', dev, P(q), P(k_new), P(v_new), P(k_cache), P(v_cache), P(lengths), P(out), P(ws), nws, b, hq, hkv, d, cap, _i64(sq),
-            None if skn is None else _i64(skn), None if svn is None else _i64(svn), _i64(cst[0]), _i64(cst[1]), scale)
+    sizes, cst, scale = tail
+    if direct is None or (q.data_ptr() | (k_new.data_ptr() | v_new.data_ptr() if new else 0)) % 16:
+        q, sq = _rows(q)
+        direct = _i64(sq), None, None
+        if new:
+            (k_new, skn), (v_new, svn) = _rows(k_new), _rows(v_new)
+            direct = _i64(sq), _i64(skn), _i64(svn)
+    _launch('genie_cached_attention_step', device, P(q), P(k_new), P(v_new), kc, vc, P(lengths), P(out), P(ws), nws, *sizes, *direct, *cst, scale)
     return out
 
 
 # ------------------------------------------------------------------------------------------------------------------------------------
 # linear attention with a decay per head
 # ------------------------------------------------------------------------------------------------------------------------------------
-def _decay_forward(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, cu: Tensor, initial_state: Optional[Tensor], scale: float, return_state: bool):
-    """(out, final states or None, what the backward pass keeps)"""
+def _decay_forward(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, cu: Tensor, initial_state: Optional[Tensor], scale: float, return_state: bool,
+                   direct=None):
+    """(out, final states or None, what the backward pass keeps); direct: strides of q, k and v if only their alignment is open"""
     rows, h, dk = q.shape
     dv, nseq, dev = v.shape[2], cu.shape[0] - 1, q.device
-    (q, sq), (k, sk), (v, sv) = _rows(q), _rows(k), _rows(v)
+    if direct is not None and not (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
+        sq, sk, sv = direct
+    else:
+        (q, sq), (k, sk), (v, sv) = _rows(q), _rows(k), _rows(v)
     out = torch.empty((rows, h, dv), dtype=torch.bfloat16, device=dev)
     final = torch.empty((nseq, h, dk, dv), dtype=torch.float32, device=dev) if return_state else None
     states = ws = None
@@ -350,24 +416,22 @@ class _DecayAttention(torch.autograd.Function):
         return gq if need[0] else None, gk if need[1] else None, gv if need[2] else None, None, None, None, None, None
 
 
-def _check_decay(what: str, log_decay: Tensor, heads: int, device: torch.device) -> Tensor:
+def _check_decay(what: str, log_decay: Tensor, heads: int, device: torch.device) -> None:
     _check(what, log_decay, 'log_decay', 1, torch.float32, device)
     if log_decay.shape[0] != heads:
         raise ValueError(f'{what}: log_decay must hold one value for each of the {heads} heads, got {tuple(log_decay.shape)}')
-    if log_decay.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError(f'{what}: the decays are constants (no gradient): pass log_decay.detach()')
-    return log_decay.detach().contiguous()
 
 
-def decay_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, cu_seqlens: Tensor, initial_state: Optional[Tensor] = None, scale: Optional[float] = None,
-                    return_state: bool = False) -> Union[Tensor, Tuple[Tensor, Tensor]]:
-    """Linear attention with a decay for each head over packed sequences: ``S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T``, ``o_t = scale q_t S_t``.
+def _constant(what: str, why: str, t: Tensor) -> Tensor:
+    if t.requires_grad:
+        if torch.is_grad_enabled():
+            raise RuntimeError(f'{what}: {why}')
+        t = t.detach()
+    return t if t.is_contiguous() else t.contiguous()
 
-    ``q`` / ``k`` (rows, H, dk), ``v`` (rows, H, dv) bf16, widths multiples of 8 up to 128; ``log_decay`` (H,) fp32, <= 0 (``-inf``: no memory, 0: none is lost);
-    ``scale`` defaults to ``dk ** -0.5``.  Returns (rows, H, dv) bf16, differentiable in q, k and v.
 
-    ``initial_state`` (sequences, H, dk, dv) fp32: the state in front of each sequence's first token.  ``return_state``: also return the state behind each sequence's
-    last token, which ``decay_attention_step`` and a later call continue from.  States carry no gradient (truncated backpropagation)."""
+def _decay_plan(q, k, v, log_decay, cu_seqlens, initial_state, scale):
+    """(scale, None or the strides of q, k and v where they need no copy)"""
     what = 'decay_attention'
     _check(what, q, 'q', 3, torch.bfloat16)
     _check(what, k, 'k', 3, torch.bfloat16, q.device)
@@ -383,26 +447,39 @@ def decay_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, cu_seqle
         raise ValueError(f'{what}: at most {_MAX_ROWS} rows')
     _check_width(what, dk, 'q and k')
     _check_width(what, v.shape[2], 'v')
-    log_decay = _check_decay(what, log_decay, h, q.device)
+    _check_decay(what, log_decay, h, q.device)
     _check_cu(what, cu_seqlens, 'cu_seqlens', q.device)
     if initial_state is not None:
         _check(what, initial_state, 'initial_state', 4, torch.float32, q.device)
         want = (cu_seqlens.shape[0] - 1, h, dk, v.shape[2])
         if initial_state.shape != want:
             raise ValueError(f'{what}: initial_state must be {want}, got {tuple(initial_state.shape)}')
-        if initial_state.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError(f'{what}: no gradient flows into a state: pass initial_state.detach()')
-        initial_state = initial_state.detach().contiguous()
-    scale = _scale(what, scale, dk)
+    strides = tuple(_direct(t) for t in (q, k, v))
+    return _scale(what, scale, dk), None if None in strides else strides
+
+
+def decay_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, cu_seqlens: Tensor, initial_state: Optional[Tensor] = None, scale: Optional[float] = None,
+                    return_state: bool = False) -> Union[Tensor, Tuple[Tensor, Tensor]]:
+    """Linear attention with a decay for each head over packed sequences: ``S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T``, ``o_t = scale q_t S_t``.
+
+    ``q`` / ``k`` (rows, H, dk), ``v`` (rows, H, dv) bf16, widths multiples of 8 up to 128; ``log_decay`` (H,) fp32, <= 0 (``-inf``: no memory, 0: none is lost);
+    ``scale`` defaults to ``dk ** -0.5``.  Returns (rows, H, dv) bf16, differentiable in q, k and v.
+
+    ``initial_state`` (sequences, H, dk, dv) fp32: the state in front of each sequence's first token.  ``return_state``: also return the state behind each sequence's
+    last token, which ``decay_attention_step`` and a later call continue from.  States carry no gradient (truncated backpropagation)."""
+    what = 'decay_attention'
+    scale, direct = _planned(_decay_plan, (q, k, v, log_decay, cu_seqlens, initial_state), None if scale is None else float(scale))
+    log_decay = _constant(what, 'the decays are constants (no gradient): pass log_decay.detach()', log_decay)
+    if initial_state is not None:
+        initial_state = _constant(what, 'no gradient flows into a state: pass initial_state.detach()', initial_state)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _DecayAttention.apply(q, k, v, log_decay, cu_seqlens, initial_state, scale, bool(return_state))
-    out, final, _ = _decay_forward(q, k, v, log_decay, cu_seqlens, initial_state, scale, return_state)
+    out, final, _ = _decay_forward(q, k, v, log_decay, cu_seqlens, initial_state, scale, return_state, direct)
     return (out, final) if return_state else out
 
 
-def decay_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor, scale: Optional[float] = None, new_state: Optional[Tensor] = None) -> Tensor:
-    """``decay_attention`` for one token per sequence: ``q`` / ``k`` (B, H, dk), ``v`` (B, H, dv) bf16, ``state`` (B, H, dk, dv) fp32, contiguous.  The state is advanced in
-    place, or into ``new_state`` (the old one then stays).  Returns (B, H, dv) bf16; no backward pass."""
+def _decay_step_plan(q, k, v, log_decay, state, new_state, scale):
+    """(device, the output's shape, None or the strides of tensors that need no copy, sizes, scale)"""
     what = 'decay_attention_step'
     _check(what, q, 'q', 3, torch.bfloat16)
     _check(what, k, 'k', 3, torch.bfloat16, q.device)
@@ -417,23 +494,37 @@ def decay_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, sta
         raise ValueError(f'{what}: no heads')
     _check_width(what, dk, 'q and k')
     _check_width(what, dv, 'v')
-    log_decay = _check_decay(what, log_decay, h, q.device)
-    _no_grad_wanted(what, q, k, v, state, new_state)
-    new_state = state if new_state is None else new_state
+    _check_decay(what, log_decay, h, q.device)
     for t, name in ((state, 'state'), (new_state, 'new_state')):
+        if t is None and name == 'new_state':
+            continue
         _check(what, t, name, 4, torch.float32, q.device)
         if t.shape != (b, h, dk, dv):
             raise ValueError(f'{what}: {name} must be {(b, h, dk, dv)}, got {tuple(t.shape)}')
-        if not t.is_contiguous() or t.data_ptr() % 16:
+        if not t.is_contiguous():
             raise ValueError(f'{what}: {name} must be contiguous and 16-byte aligned')
-    lo, hi = sorted((state.data_ptr(), new_state.data_ptr()))
-    if lo != hi and hi - lo < state.numel() * 4:
+    direct = [_direct(t) for t in (q, k, v)]
+    return q.device, (b, h, dv), None if None in direct else tuple(map(_i64, direct)), (b, h, dk, dv), _scale(what, scale, dk)
+
+
+def decay_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor, scale: Optional[float] = None, new_state: Optional[Tensor] = None) -> Tensor:
+    """``decay_attention`` for one token per sequence: ``q`` / ``k`` (B, H, dk), ``v`` (B, H, dv) bf16, ``state`` (B, H, dk, dv) fp32, contiguous.  The state is advanced in
+    place, or into ``new_state`` (the old one then stays).  Returns (B, H, dv) bf16; no backward pass."""
+    what = 'decay_attention_step'
+    device, shape, direct, sizes, scale = _planned(_decay_step_plan, (q, k, v, log_decay, state, new_state), None if scale is None else float(scale))
+    log_decay = _constant(what, 'the decays are constants (no gradient): pass log_decay.detach()', log_decay)
+    _no_grad_wanted(what, q, k, v, state, new_state)
+    old = state.data_ptr()
+    new = old if new_state is None else new_state.data_ptr()
+    if (old | new) % 16:
+        raise ValueError(f'{what}: {"state" if old % 16 else "new_state"} must be contiguous and 16-byte aligned')
+    if old != new and abs(old - new) < state.numel() * 4:
         raise ValueError(f'{what}: new_state overlaps state without being it')
-    scale = _scale(what, scale, dk)
-    (q, sq), (k, sk), (v, sv) = _rows(q), _rows(k), _rows(v)
-    out = torch.empty((b, h, dv), dtype=torch.bfloat16, device=q.device)
-    if b == 0:
+    out = torch.empty(shape, dtype=torch.bfloat16, device=device)
+    if shape[0] == 0:
         return out
-    P = _hip.ptr
-    _launch('genie_decay_attention_step', q.device, P(q), P(k), P(v), P(log_decay), P(state), P(new_state), P(out), b, h, dk, dv, _i64(sq), _i64(sk), _i64(sv), scale)
+    if direct is None or (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
+        (q, sq), (k, sk), (v, sv) = _rows(q), _rows(k), _rows(v)
+        direct = _i64(sq), _i64(sk), _i64(sv)
+    _launch('genie_decay_attention_step', device, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), old, new, out.data_ptr(), *sizes, *direct, scale)
     return out

@@ -660,3 +660,61 @@ def test_calls_from_two_threads():
     for t in threads:
         t.join()
     assert same == [True, True]
+
+
+@pytest.mark.parametrize('lens', [[2200, 2100], [2048, 2048]], ids=str)
+@pytest.mark.parametrize('d', [32, 64, 128])
+def test_packed_attention_many_blocks(lens, d):
+    """Enough blocks that the kernels take their forms for a full chip: tall blocks, whole row tiles per wave."""
+    _check_packed(lens, 3, 16, 4, d, 960)
+
+
+@pytest.mark.parametrize('d', [32, 64, 96, 128])
+def test_cached_step_many_short_caches(d):
+    """Enough sequences that neither wide blocks nor splits are taken."""
+    b, cap, hkv = 300, 100, 2
+    q, kc, vc = _randn(b, 4, d, seed=970), _cache(b, cap, hkv, d, 971), _cache(b, cap, hkv, d, 972)
+    lengths = [(i * 37) % (cap + 1) for i in range(b)]
+    val, tol = R.step_reference(q, kc, vc, lengths, d ** -0.5)
+    out = _gf().cached_attention_step(q, kc, vc, torch.tensor(lengths, dtype=torch.int32, device='cuda'))
+    R.assert_within(out, val, tol, 'out')
+
+
+def test_calls_that_look_the_same_but_for_their_addresses():
+    """Same types, shapes and strides as an earlier call, other addresses: rows off 16 bytes are copied, a cache or state off 16 bytes or twice the same is refused."""
+    gf, d = _gf(), 64
+
+    def odd(t):
+        return torch.empty(t.numel() + 3, dtype=t.dtype, device='cuda')[3:].view(t.shape).copy_(t)
+
+    cu, ld = _cu([3, 5]), _decays(2)
+    q, k, v = (_randn(8, 2, d, seed=980 + i) for i in range(3))
+    kc, vc = _cache(8, 20, 2, d, 984), _cache(8, 20, 2, d, 985)
+    n, s = torch.arange(8, dtype=torch.int32, device='cuda'), torch.randn(8, 2, d, d, device='cuda')
+    new = torch.empty_like(s)
+    calls = (lambda q, k, v: gf.packed_attention(q, k, v, cu), lambda q, k, v: gf.decay_attention(q, k, v, ld, cu), lambda q, k, v: gf.cached_attention_step(q, kc, vc, n, k, v),
+             lambda q, k, v: gf.decay_attention_step(q, k, v, ld, s, new_state=new))
+    for call in calls:
+        want = call(q, k, v)
+        for moved in ((odd(q), k, v), (q, odd(k), v), (q, k, odd(v))):
+            assert torch.equal(call(*moved), want)
+        assert torch.equal(call(q.clone(), k, v), want)
+        assert not torch.equal(call(k, q, v), want)
+    with pytest.raises(ValueError, match='updated in place'):
+        gf.cached_attention_step(q, odd(kc), vc, n, k, v)
+    with pytest.raises(ValueError, match='updated in place'):
+        gf.cached_attention_step(q, kc, odd(vc), n, k, v)
+    with pytest.raises(ValueError, match='same memory'):
+        gf.cached_attention_step(q, kc, kc, n, k, v)
+    with pytest.raises(ValueError, match='aligned'):
+        gf.decay_attention_step(q, k, v, ld, odd(s), new_state=new)
+    with pytest.raises(ValueError, match='aligned'):
+        gf.decay_attention_step(q, k, v, ld, s, new_state=odd(new))
+    with pytest.raises(RuntimeError, match='no backward'):
+        gf.decay_attention_step(q.clone().requires_grad_(), k, v, ld, s, new_state=new)
+    with pytest.raises(RuntimeError, match='constants'):
+        gf.decay_attention(q, k, v, ld.clone().requires_grad_(), cu)
+    with torch.no_grad():
+        a = gf.decay_attention(q, k, v, ld.clone().requires_grad_(), cu)
+    assert torch.equal(a, gf.decay_attention(q, k, v, ld, cu))
+    assert not torch.equal(gf.packed_attention(q, k, v, cu, scale=0.5), gf.packed_attention(q, k, v, cu, scale=torch.tensor(0.25)))
