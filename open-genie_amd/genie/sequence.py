@@ -139,7 +139,8 @@ _PLANS: dict = {}
 
 def _planned(make, tensors, *rest):
     """``make(*tensors, *rest)``: all checks of a call that its types, devices, shapes and strides decide, and what follows from them for the launch.  Kept for the calls
-    that look the same (a token's call: 18 us with the checks, 11 without); nothing in it depends on a tensor's address or contents."""
+    that look the same (a token's call: 18 us with the checks, 11 without; a layout's first call
+    takes 3 us more than the checks alone); nothing in it depends on a tensor's address or contents."""
     try:
         key = (make, *map(_sig, tensors), *rest)
     except AttributeError:                                        # not a tensor: the checks say so
@@ -171,28 +172,31 @@ def _first_order(backward):
 # ------------------------------------------------------------------------------------------------------------------------------------
 # causal attention over packed sequences
 # ------------------------------------------------------------------------------------------------------------------------------------
-def _packed_forward(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Tensor, scale: float, keep: bool):
-    """(out, what the backward pass keeps)"""
+def _packed_forward(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Tensor, scale: float, direct, keep: bool):
+    """(out, tensors that the backward pass keeps, sizes and strides of the call); direct: those where no tensor needs a copy, their alignment aside"""
     rows, hq, d = q.shape
     rows_k, hkv, _ = k.shape
-    (q, sq), (k, sk), (v, sv) = _rows(q), _rows(k), _rows(v)
-    out = torch.empty((rows, hq, d), dtype=torch.bfloat16, device=q.device)
+    if direct is None or (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
+        (q, sq), (k, sk), (v, sv) = _rows(q), _rows(k), _rows(v)
+        direct = (cu_q.shape[0] - 1, rows, rows_k, hq, hkv, d, _i64(sq), _i64(sk), _i64(sv), scale)
+    out = q.new_empty((rows, hq, d))
     # for the backward pass, in one buffer: what out's rounding left over (bf16, rows x hq x d), then the log-sum-exps (fp32, hq x rows)
-    rest = torch.empty(rows * hq * (d // 2 + 1), dtype=torch.float32, device=q.device) if keep else None
+    rest, lo, lse = None, None, None
+    if keep:
+        rest = torch.empty(rows * hq * (d // 2 + 1), dtype=torch.float32, device=q.device)
+        lo = rest.data_ptr()
+        lse = lo + rows * hq * d * 2
     if rows and rows_k:
-        P = _hip.ptr
-        lo = P(rest)
-        _launch('genie_packed_attention_fwd', q.device, P(q), P(k), P(v), P(out), lo, lo + rows * hq * d * 2 if keep else None, P(cu_q), P(cu_k), cu_q.shape[0] - 1, rows, rows_k, hq, hkv, d,
-                _i64(sq), _i64(sk), _i64(sv), scale)
+        _launch('genie_packed_attention_fwd', q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lo, lse, cu_q.data_ptr(), cu_k.data_ptr(), *direct)
     else:
         out.zero_()
-    return out, ((q, k, v, out, rest, cu_q, cu_k), (sq, sk, sv, scale)) if keep else None
+    return out, (q, k, v, out, rest, cu_q, cu_k), direct
 
 
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Tensor, scale: float):
-        out, (saved, ctx.cfg) = _packed_forward(q, k, v, cu_q, cu_k, scale, True)
+    def forward(ctx, q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Tensor, scale: float, direct):
+        out, saved, ctx.call = _packed_forward(q, k, v, cu_q, cu_k, scale, direct, True)
         ctx.save_for_backward(*saved)
         return out
 
@@ -200,29 +204,24 @@ class _PackedAttention(torch.autograd.Function):
     @_first_order
     def backward(ctx, dout: Tensor):
         q, k, v, out, rest, cu_q, cu_k = ctx.saved_tensors
-        sq, sk, sv, scale = ctx.cfg
-        rows, hq, d = q.shape
-        rows_k, hkv, _ = k.shape
+        nseq, rows, rows_k, hq, hkv, d, sq, sk, sv, scale = ctx.call
         dout, sg = _rows(dout)
-        dq = torch.empty((rows, hq, d), dtype=torch.bfloat16, device=q.device)
-        dk = torch.empty((rows_k, hkv, d), dtype=torch.bfloat16, device=q.device)
-        dv = torch.empty_like(dk)
+        dq, dk, dv = q.new_empty((rows, hq, d)), q.new_empty((rows_k, hkv, d)), q.new_empty((rows_k, hkv, d))
         if rows and rows_k:
-            P = _hip.ptr
-            lo = P(rest)
-            nws = _hip.load_library().genie_packed_attention_bwd_ws_floats(cu_q.shape[0] - 1, rows, rows_k, hq, hkv, d)
+            lo = rest.data_ptr()
+            nws = _hip.load_library().genie_packed_attention_bwd_ws_floats(nseq, rows, rows_k, hq, hkv, d)
             ws = torch.empty(nws, dtype=torch.float32, device=q.device)
-            _launch('genie_packed_attention_bwd', q.device, P(q), P(k), P(v), P(out), lo, P(dout), lo + rows * hq * d * 2, P(ws), nws, P(dq), P(dk), P(dv), P(cu_q), P(cu_k),
-                    cu_q.shape[0] - 1, rows, rows_k, hq, hkv, d, _i64(sq), _i64(sk), _i64(sv), _i64(sg), scale)
+            _launch('genie_packed_attention_bwd', q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lo, dout.data_ptr(), lo + rows * hq * d * 2, ws.data_ptr(), nws,
+                    dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), nseq, rows, rows_k, hq, hkv, d, sq, sk, sv, _i64(sg), scale)
         else:
             for t in (dq, dk, dv):
                 t.zero_()
         need = ctx.needs_input_grad
-        return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None
+        return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None, None
 
 
 def _packed_plan(q, k, v, cu_seqlens, cu_seqlens_k, scale):
-    """(scale, None or what a call takes whose tensors need no copy)"""
+    """(scale, None or the sizes and strides of a call whose tensors need no copy)"""
     what = 'packed_attention'
     _check(what, q, 'q', 3, torch.bfloat16)
     _check(what, k, 'k', 3, torch.bfloat16, q.device)
@@ -248,9 +247,7 @@ def _packed_plan(q, k, v, cu_seqlens, cu_seqlens_k, scale):
             raise ValueError(f'{what}: cu_seqlens and cu_seqlens_k describe different numbers of sequences')
     scale = _scale(what, scale, d)
     strides = [_direct(t) for t in (q, k, v)]
-    if None in strides or not (rows and rows_k):
-        return scale, None
-    return scale, ((rows, hq, d), q.device, (cu_seqlens.shape[0] - 1, rows, rows_k, hq, hkv, d, *map(_i64, strides), scale))
+    return scale, None if None in strides else (cu_seqlens.shape[0] - 1, rows, rows_k, hq, hkv, d, *map(_i64, strides), scale)
 
 
 def packed_attention(q: Tensor, k: Tensor, v: Tensor, cu_seqlens: Tensor, scale: Optional[float] = None, cu_seqlens_k: Optional[Tensor] = None) -> Tensor:
@@ -265,15 +262,8 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, cu_seqlens: Tensor, scale:
     if cu_seqlens_k is None:
         cu_seqlens_k = cu_seqlens
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _PackedAttention.apply(q, k, v, cu_seqlens, cu_seqlens_k, scale)
-    if direct is not None:
-        shape, device, sizes = direct
-        ptrs = q.data_ptr(), k.data_ptr(), v.data_ptr()
-        if not (ptrs[0] | ptrs[1] | ptrs[2]) % 16:
-            out = torch.empty(shape, dtype=torch.bfloat16, device=device)
-            _launch('genie_packed_attention_fwd', device, *ptrs, out.data_ptr(), None, None, cu_seqlens.data_ptr(), cu_seqlens_k.data_ptr(), *sizes)
-            return out
-    return _packed_forward(q, k, v, cu_seqlens, cu_seqlens_k, scale, False)[0]
+        return _PackedAttention.apply(q, k, v, cu_seqlens, cu_seqlens_k, scale, direct)
+    return _packed_forward(q, k, v, cu_seqlens, cu_seqlens_k, scale, direct, False)[0]
 
 
 def _cached_plan(q, k_cache, v_cache, lengths, k_new, v_new, scale):
@@ -343,7 +333,7 @@ def cached_attention_step(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: 
         raise ValueError(f'{what}: {"k_cache" if kc % 16 else "v_cache"} must have a contiguous last axis and 16-byte aligned rows (it is updated in place and cannot be copied)')
     if new and kc == vc:
         raise ValueError(f'{what}: k_cache and v_cache are the same memory')
-    out = torch.empty(shape, dtype=torch.bfloat16, device=device)
+    out = q.new_empty(shape)
     if shape[0] == 0:
         return out
     ws = torch.empty(nws, dtype=torch.float32, device=device) if nws else None
@@ -363,7 +353,7 @@ def cached_attention_step(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: 
 # linear attention with a decay per head
 # ------------------------------------------------------------------------------------------------------------------------------------
 def _decay_forward(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, cu: Tensor, initial_state: Optional[Tensor], scale: float, return_state: bool,
-                   direct=None):
+                   direct):
     """(out, final states or None, what the backward pass keeps); direct: strides of q, k and v if only their alignment is open"""
     rows, h, dk = q.shape
     dv, nseq, dev = v.shape[2], cu.shape[0] - 1, q.device
@@ -371,7 +361,7 @@ def _decay_forward(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, cu: Tenso
         sq, sk, sv = direct
     else:
         (q, sq), (k, sk), (v, sv) = _rows(q), _rows(k), _rows(v)
-    out = torch.empty((rows, h, dv), dtype=torch.bfloat16, device=dev)
+    out = q.new_empty((rows, h, dv))
     final = torch.empty((nseq, h, dk, dv), dtype=torch.float32, device=dev) if return_state else None
     states = ws = None
     if rows:
@@ -388,8 +378,8 @@ def _decay_forward(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, cu: Tenso
 
 class _DecayAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, cu: Tensor, initial_state: Optional[Tensor], scale: float, return_state: bool):
-        out, final, (saved, ctx.cfg) = _decay_forward(q, k, v, log_decay, cu, initial_state, scale, return_state)
+    def forward(ctx, q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, cu: Tensor, initial_state: Optional[Tensor], scale: float, return_state: bool, direct):
+        out, final, (saved, ctx.cfg) = _decay_forward(q, k, v, log_decay, cu, initial_state, scale, return_state, direct)
         ctx.save_for_backward(*saved)
         if return_state:
             ctx.mark_non_differentiable(final)
@@ -404,8 +394,7 @@ class _DecayAttention(torch.autograd.Function):
         rows, h, dk = q.shape
         dv, nseq, dev = v.shape[2], cu.shape[0] - 1, q.device
         dout, sg = _rows(dout)
-        gq, gk = (torch.empty((rows, h, dk), dtype=torch.bfloat16, device=dev) for _ in range(2))
-        gv = torch.empty((rows, h, dv), dtype=torch.bfloat16, device=dev)
+        gq, gk, gv = q.new_empty((rows, h, dk)), q.new_empty((rows, h, dk)), q.new_empty((rows, h, dv))
         if rows:
             n, rev, ws, P = _hip.load_library().genie_decay_attention_state_elems(nseq, rows, h, dk, dv, 0), None, None, _hip.ptr
             if n:
@@ -413,7 +402,7 @@ class _DecayAttention(torch.autograd.Function):
             _launch('genie_decay_attention_bwd', dev, P(q), P(k), P(v), P(dout), P(log_decay), P(cu), int(has_initial), P(states), P(rev), P(ws), n, P(gq), P(gk), P(gv),
                     nseq, rows, h, dk, dv, _i64(sq), _i64(sk), _i64(sv), _i64(sg), scale)
         need = ctx.needs_input_grad
-        return gq if need[0] else None, gk if need[1] else None, gv if need[2] else None, None, None, None, None, None
+        return gq if need[0] else None, gk if need[1] else None, gv if need[2] else None, None, None, None, None, None, None
 
 
 def _check_decay(what: str, log_decay: Tensor, heads: int, device: torch.device) -> None:
@@ -473,7 +462,7 @@ def decay_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, cu_seqle
     if initial_state is not None:
         initial_state = _constant(what, 'no gradient flows into a state: pass initial_state.detach()', initial_state)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _DecayAttention.apply(q, k, v, log_decay, cu_seqlens, initial_state, scale, bool(return_state))
+        return _DecayAttention.apply(q, k, v, log_decay, cu_seqlens, initial_state, scale, bool(return_state), direct)
     out, final, _ = _decay_forward(q, k, v, log_decay, cu_seqlens, initial_state, scale, return_state, direct)
     return (out, final) if return_state else out
 
@@ -520,7 +509,7 @@ def decay_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, sta
         raise ValueError(f'{what}: {"state" if old % 16 else "new_state"} must be contiguous and 16-byte aligned')
     if old != new and abs(old - new) < state.numel() * 4:
         raise ValueError(f'{what}: new_state overlaps state without being it')
-    out = torch.empty(shape, dtype=torch.bfloat16, device=device)
+    out = q.new_empty(shape)
     if shape[0] == 0:
         return out
     if direct is None or (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
