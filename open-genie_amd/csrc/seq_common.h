@@ -98,7 +98,7 @@ __device__ __forceinline__ int seq_bytes_left(int rows, int64_t stride_bytes, in
 }
 
 // ds_read_b64_tr_b16: in each group of 16 lanes, lane i names 4 consecutive 16-bit values of row i / 4 (columns 4 (i % 4) ...) and receives column i of the
-// four rows.  The builtin: the compiler tracks the wait itself (tiles here are staged through registers, no LDS-DMA is in flight beside it).
+// four rows.  The builtin: the compiler tracks the wait itself, but waits for an LDS-DMA in flight as well.
 typedef __attribute__((address_space(3))) bf16x4_t seq_lds_b16x4;
 __device__ __forceinline__ bf16x4_t seq_tr16(const char* p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((seq_lds_b16x4*)p); }
 
