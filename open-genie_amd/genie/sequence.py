@@ -18,6 +18,7 @@ Common conventions
     every entry to the rows that exist, so a wrong one costs wrong results and no access out of bounds.  Rows behind ``cu[-1]`` are padding: never read
     (they may hold anything, NaN included), zero in every result and gradient.
   * a tensor whose rows are not 16-byte aligned, or whose last axis is not contiguous, is copied first; slices of a fused projection are taken as they are.
+    Tensors saved for a backward pass are looked at again as they come back from hooks on saved tensors (``torch.autograd.graph.save_on_cpu`` and its like).
   * the kernels run on the current stream of the tensors' device; scratch memory is allocated per call (a captured graph owns its own).
   * bitwise reproducible: no atomics, every sum has a fixed order.
   * capture of a backward pass into a graph: with no eager autograd graph of the same leaves alive (torch ends the process where it meets a leaf's node of another
@@ -154,6 +155,22 @@ def _planned(make, tensors, *rest):
     return plan
 
 
+def _came_back(what: str, t: Optional[Tensor], name: str, dtype: torch.dtype, shape: Tuple[int, ...], device: torch.device) -> None:
+    """A tensor that the forward pass saved: hooks on saved tensors (``torch.autograd.graph.save_on_cpu`` and its like) may bring it back with other strides, at
+    another address, or as something else altogether."""
+    if not isinstance(t, Tensor) or t.dtype != dtype or t.shape != shape or t.device != device:
+        got = f'{t.dtype} {tuple(t.shape)} on {t.device}' if isinstance(t, Tensor) else repr(t)
+        raise RuntimeError(f'{what}: {name} was saved for the backward pass as {dtype} {tuple(shape)} on {device} and came back as {got}')
+
+
+def _dense(t: Optional[Tensor]) -> Optional[Tensor]:
+    """The tensor itself if it is contiguous and 16-byte aligned, else a copy that is."""
+    if t is None:
+        return None
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
 def _no_grad_wanted(what: str, *tensors: Optional[Tensor]) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f'{what} has no backward pass: call it under torch.no_grad(), or on tensors that do not require gradients')
@@ -172,13 +189,12 @@ def _first_order(backward):
 # ------------------------------------------------------------------------------------------------------------------------------------
 # causal attention over packed sequences
 # ------------------------------------------------------------------------------------------------------------------------------------
-def _packed_forward(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Tensor, scale: float, direct, keep: bool):
-    """(out, tensors that the backward pass keeps, sizes and strides of the call); direct: those where no tensor needs a copy, their alignment aside"""
-    rows, hq, d = q.shape
-    rows_k, hkv, _ = k.shape
-    if direct is None or (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
+def _packed_forward(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Tensor, scale: float, sizes, strides, keep: bool):
+    """(out, tensors that the backward pass keeps); strides: those of q, k and v where no tensor needs a copy, their alignment aside"""
+    _, rows, rows_k, hq, _, d = sizes
+    if strides is None or (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
         (q, sq), (k, sk), (v, sv) = _rows(q), _rows(k), _rows(v)
-        direct = (cu_q.shape[0] - 1, rows, rows_k, hq, hkv, d, _i64(sq), _i64(sk), _i64(sv), scale)
+        strides = _i64(sq), _i64(sk), _i64(sv)
     out = q.new_empty((rows, hq, d))
     # for the backward pass, in one buffer: what out's rounding left over (bf16, rows x hq x d), then the log-sum-exps (fp32, hq x rows)
     rest, lo, lse = None, None, None
@@ -187,41 +203,59 @@ def _packed_forward(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Tensor,
         lo = rest.data_ptr()
         lse = lo + rows * hq * d * 2
     if rows and rows_k:
-        _launch('genie_packed_attention_fwd', q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lo, lse, cu_q.data_ptr(), cu_k.data_ptr(), *direct)
+        _launch('genie_packed_attention_fwd', q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lo, lse, cu_q.data_ptr(), cu_k.data_ptr(), *sizes, *strides, scale)
     else:
         out.zero_()
-    return out, (q, k, v, out, rest, cu_q, cu_k), direct
+    return out, (q, k, v, out, rest, cu_q, cu_k)
+
+
+def _packed_bwd_plan(q, k, v, out, rest, cu_q, cu_k, dout, sizes):
+    """(None or the strides of q, k, v and dout where no tensor needs a copy, floats of workspace), from the tensors as they came back"""
+    what, dev = 'packed_attention', dout.device
+    nseq, rows, rows_k, hq, hkv, d = sizes
+    for t, name, dtype, shape in ((q, 'q', torch.bfloat16, (rows, hq, d)), (k, 'k', torch.bfloat16, (rows_k, hkv, d)), (v, 'v', torch.bfloat16, (rows_k, hkv, d)),
+                                  (out, 'the output', torch.bfloat16, (rows, hq, d)), (rest, 'its remainder', torch.float32, (rows * hq * (d // 2 + 1),)),
+                                  (cu_q, 'cu_seqlens', torch.int32, (nseq + 1,)), (cu_k, 'cu_seqlens_k', torch.int32, (nseq + 1,))):
+        _came_back(what, t, name, dtype, shape, dev)
+    strides = [_direct(t) for t in (q, k, v, dout)]
+    direct = None not in strides and all(t.is_contiguous() for t in (out, rest, cu_q, cu_k))
+    return tuple(map(_i64, strides)) if direct else None, _hip.load_library().genie_packed_attention_bwd_ws_floats(*sizes)
 
 
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Tensor, scale: float, direct):
-        out, saved, ctx.call = _packed_forward(q, k, v, cu_q, cu_k, scale, direct, True)
+    def forward(ctx, q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Tensor, scale: float, sizes, strides):
+        out, saved = _packed_forward(q, k, v, cu_q, cu_k, scale, sizes, strides, True)
+        ctx.sizes, ctx.scale = sizes, scale
         ctx.save_for_backward(*saved)
         return out
 
     @staticmethod
     @_first_order
     def backward(ctx, dout: Tensor):
+        # nothing about the saved tensors' layout is taken over from the forward pass: they are looked at as they came back
         q, k, v, out, rest, cu_q, cu_k = ctx.saved_tensors
-        nseq, rows, rows_k, hq, hkv, d, sq, sk, sv, scale = ctx.call
-        dout, sg = _rows(dout)
+        _, rows, rows_k, hq, hkv, d = sizes = ctx.sizes
+        strides, nws = _planned(_packed_bwd_plan, (q, k, v, out, rest, cu_q, cu_k, dout), sizes)
         dq, dk, dv = q.new_empty((rows, hq, d)), q.new_empty((rows_k, hkv, d)), q.new_empty((rows_k, hkv, d))
         if rows and rows_k:
+            if strides is None or (q.data_ptr() | k.data_ptr() | v.data_ptr() | dout.data_ptr() | out.data_ptr() | rest.data_ptr()) % 16:
+                (q, sq), (k, sk), (v, sv), (dout, sg) = _rows(q), _rows(k), _rows(v), _rows(dout)
+                strides = _i64(sq), _i64(sk), _i64(sv), _i64(sg)
+                out, rest, cu_q, cu_k = _dense(out), _dense(rest), _dense(cu_q), _dense(cu_k)
             lo = rest.data_ptr()
-            nws = _hip.load_library().genie_packed_attention_bwd_ws_floats(nseq, rows, rows_k, hq, hkv, d)
             ws = torch.empty(nws, dtype=torch.float32, device=q.device)
             _launch('genie_packed_attention_bwd', q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lo, dout.data_ptr(), lo + rows * hq * d * 2, ws.data_ptr(), nws,
-                    dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), nseq, rows, rows_k, hq, hkv, d, sq, sk, sv, _i64(sg), scale)
+                    dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), *sizes, *strides, ctx.scale)
         else:
             for t in (dq, dk, dv):
                 t.zero_()
         need = ctx.needs_input_grad
-        return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None, None
+        return dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None, None, None
 
 
 def _packed_plan(q, k, v, cu_seqlens, cu_seqlens_k, scale):
-    """(scale, None or the sizes and strides of a call whose tensors need no copy)"""
+    """(scale, sizes, None or the strides of q, k and v where they need no copy)"""
     what = 'packed_attention'
     _check(what, q, 'q', 3, torch.bfloat16)
     _check(what, k, 'k', 3, torch.bfloat16, q.device)
@@ -247,7 +281,7 @@ def _packed_plan(q, k, v, cu_seqlens, cu_seqlens_k, scale):
             raise ValueError(f'{what}: cu_seqlens and cu_seqlens_k describe different numbers of sequences')
     scale = _scale(what, scale, d)
     strides = [_direct(t) for t in (q, k, v)]
-    return scale, None if None in strides else (cu_seqlens.shape[0] - 1, rows, rows_k, hq, hkv, d, *map(_i64, strides), scale)
+    return scale, (cu_seqlens.shape[0] - 1, rows, rows_k, hq, hkv, d), None if None in strides else tuple(map(_i64, strides))
 
 
 def packed_attention(q: Tensor, k: Tensor, v: Tensor, cu_seqlens: Tensor, scale: Optional[float] = None, cu_seqlens_k: Optional[Tensor] = None) -> Tensor:
@@ -258,12 +292,12 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, cu_seqlens: Tensor, scale:
 
     ``cu_seqlens_k``: the keys' own packing, where a sequence has other keys than queries -- a prompt that continues a context.  The last query then sees the
     last key: query i of n sees keys ``0 .. i + n_k - n``.  A query that sees no key (``n_k < n``) returns zeros and has zero gradients."""
-    scale, direct = _planned(_packed_plan, (q, k, v, cu_seqlens, cu_seqlens_k), None if scale is None else float(scale))
+    scale, sizes, strides = _planned(_packed_plan, (q, k, v, cu_seqlens, cu_seqlens_k), None if scale is None else float(scale))
     if cu_seqlens_k is None:
         cu_seqlens_k = cu_seqlens
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _PackedAttention.apply(q, k, v, cu_seqlens, cu_seqlens_k, scale, direct)
-    return _packed_forward(q, k, v, cu_seqlens, cu_seqlens_k, scale, direct, False)[0]
+        return _PackedAttention.apply(q, k, v, cu_seqlens, cu_seqlens_k, scale, sizes, strides)
+    return _packed_forward(q, k, v, cu_seqlens, cu_seqlens_k, scale, sizes, strides, False)[0]
 
 
 def _cached_plan(q, k_cache, v_cache, lengths, k_new, v_new, scale):
@@ -373,13 +407,29 @@ def _decay_forward(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, cu: Tenso
                 _i64(sq), _i64(sk), _i64(sv), scale)
     elif return_state:
         final.zero_() if initial_state is None else final.copy_(initial_state)
-    return out, final, ((q, k, v, log_decay, cu, states), (sq, sk, sv, scale, initial_state is not None))
+    return out, final, (q, k, v, log_decay, cu, states)
+
+
+def _decay_bwd_plan(q, k, v, log_decay, cu, states, dout, sizes, has_initial):
+    """(None or the strides of q, k, v and dout where no tensor needs a copy, elements of states and workspace), from the tensors as they came back"""
+    what, dev = 'decay_attention', dout.device
+    nseq, rows, h, dk, dv = sizes
+    elems = _hip.load_library().genie_decay_attention_state_elems
+    kept = elems(*sizes, has_initial) if rows else 0
+    for t, name, dtype, shape in ((q, 'q', torch.bfloat16, (rows, h, dk)), (k, 'k', torch.bfloat16, (rows, h, dk)), (v, 'v', torch.bfloat16, (rows, h, dv)),
+                                  (log_decay, 'log_decay', torch.float32, (h,)), (cu, 'cu_seqlens', torch.int32, (nseq + 1,)),
+                                  *(((states, 'the states', torch.bfloat16, (kept,)),) if kept else ())):
+        _came_back(what, t, name, dtype, shape, dev)
+    strides = [_direct(t) for t in (q, k, v, dout)]
+    direct = None not in strides and all(t is None or t.is_contiguous() for t in (log_decay, cu, states))
+    return tuple(map(_i64, strides)) if direct else None, elems(*sizes, 0) if rows else 0
 
 
 class _DecayAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, cu: Tensor, initial_state: Optional[Tensor], scale: float, return_state: bool, direct):
-        out, final, (saved, ctx.cfg) = _decay_forward(q, k, v, log_decay, cu, initial_state, scale, return_state, direct)
+        out, final, saved = _decay_forward(q, k, v, log_decay, cu, initial_state, scale, return_state, direct)
+        ctx.sizes, ctx.scale, ctx.has_initial = (cu.shape[0] - 1, *q.shape, v.shape[2]), scale, int(initial_state is not None)
         ctx.save_for_backward(*saved)
         if return_state:
             ctx.mark_non_differentiable(final)
@@ -390,17 +440,19 @@ class _DecayAttention(torch.autograd.Function):
     @_first_order
     def backward(ctx, dout: Tensor, *_):
         q, k, v, log_decay, cu, states = ctx.saved_tensors
-        sq, sk, sv, scale, has_initial = ctx.cfg
-        rows, h, dk = q.shape
-        dv, nseq, dev = v.shape[2], cu.shape[0] - 1, q.device
-        dout, sg = _rows(dout)
+        _, rows, h, dk, dv = sizes = ctx.sizes
+        strides, n = _planned(_decay_bwd_plan, (q, k, v, log_decay, cu, states, dout), sizes, ctx.has_initial)
         gq, gk, gv = q.new_empty((rows, h, dk)), q.new_empty((rows, h, dk)), q.new_empty((rows, h, dv))
         if rows:
-            n, rev, ws, P = _hip.load_library().genie_decay_attention_state_elems(nseq, rows, h, dk, dv, 0), None, None, _hip.ptr
+            rev, ws, P, dev = None, None, _hip.ptr, q.device
+            if strides is None or (q.data_ptr() | k.data_ptr() | v.data_ptr() | dout.data_ptr() | (P(states) or 0)) % 16:
+                (q, sq), (k, sk), (v, sv), (dout, sg) = _rows(q), _rows(k), _rows(v), _rows(dout)
+                strides = _i64(sq), _i64(sk), _i64(sv), _i64(sg)
+                log_decay, cu, states = _dense(log_decay), _dense(cu), _dense(states)
             if n:
                 rev, ws = torch.empty(n, dtype=torch.bfloat16, device=dev), torch.empty(n, dtype=torch.float32, device=dev)
-            _launch('genie_decay_attention_bwd', dev, P(q), P(k), P(v), P(dout), P(log_decay), P(cu), int(has_initial), P(states), P(rev), P(ws), n, P(gq), P(gk), P(gv),
-                    nseq, rows, h, dk, dv, _i64(sq), _i64(sk), _i64(sv), _i64(sg), scale)
+            _launch('genie_decay_attention_bwd', dev, P(q), P(k), P(v), P(dout), P(log_decay), P(cu), ctx.has_initial, P(states), P(rev), P(ws), n, P(gq), P(gk), P(gv),
+                    *sizes, *strides, ctx.scale)
         need = ctx.needs_input_grad
         return gq if need[0] else None, gk if need[1] else None, gv if need[2] else None, None, None, None, None, None, None
 

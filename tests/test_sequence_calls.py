@@ -1,0 +1,129 @@
+"""The host side of the sequence operators (genie/sequence.py) without a GPU: their checks, layouts, saved tensors and autograd nodes run as they do there, the kernels'
+launches are written down instead of made."""
+import pytest
+import torch
+
+import util  # noqa: F401  (paths)
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """CPU tensors pass the operators' device check; [(entry point, arguments)] of the launches they would make."""
+    from genie import _hip, sequence
+    made = []
+    monkeypatch.setattr(_hip, 'require_gpu', lambda *_: None)
+    monkeypatch.setattr(sequence, '_PLANS', {})
+    monkeypatch.setattr(sequence, '_launch', lambda name, device, *args: made.append((name, args)))
+    return made
+
+
+def _randn(*shape, seed=0):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(torch.bfloat16)
+
+
+def _cu(*lens):
+    return torch.tensor([0, *lens], dtype=torch.int32).cumsum(0).to(torch.int32)
+
+
+def _fused(rows, heads, d, seed):
+    """q, k and v as slices of one projection."""
+    x = _randn(rows, sum(heads), d, seed=seed).requires_grad_(True)
+    return x.split(heads, 1)
+
+
+class _Hooks:
+    """Hooks on saved tensors that bring every tensor back at another address, through `back`."""
+
+    def __init__(self, back):
+        self.back, self.returned = back, []
+
+    def unpack(self, t):
+        self.returned.append(self.back(t))
+        return self.returned[-1]
+
+    def __enter__(self):
+        self.context = torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), self.unpack)
+        self.context.__enter__()
+        return self
+
+    def __exit__(self, *what):
+        self.context.__exit__(*what)
+
+    def covers(self, pointer, strides, shape):
+        """Whether a (rows, heads, width) tensor of these strides at this address lies inside what was brought back."""
+        last = pointer + 2 * sum((n - 1) * st for n, st in zip(shape, (*strides, 1)))
+        for t in self.returned:
+            if t.dtype == torch.bfloat16 and pointer == t.data_ptr() and tuple(t.shape) == tuple(shape):
+                return tuple(t.stride()) == (*strides, 1) and last < t.data_ptr() + 2 * t.untyped_storage().nbytes()
+        return False
+
+
+def _dense(t):
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def test_packed_backward_takes_the_layout_its_saved_tensors_come_back_with(launches):
+    from genie import functional as GF
+    q, k, v = _fused(20, (4, 2, 2), 64, 1)
+    assert q.stride() == (512, 64, 1)
+    with _Hooks(_dense) as hooks:
+        out = GF.packed_attention(q, k, v, _cu(13, 7))
+        out.backward(_randn(20, 4, 64, seed=2))
+    name, args = launches[-1]
+    assert name == 'genie_packed_attention_bwd'
+    for at, strides, shape in ((0, 20, (20, 4, 64)), (1, 21, (20, 2, 64)), (2, 22, (20, 2, 64))):
+        assert hooks.covers(args[at], list(args[strides]), shape), (at, list(args[strides]))
+
+
+def test_decay_backward_takes_the_layout_its_saved_tensors_come_back_with(launches):
+    from genie import functional as GF
+    q, k, v = _fused(20, (2, 2, 2), 64, 1)
+    with _Hooks(_dense) as hooks:
+        out = GF.decay_attention(q, k, v, torch.full((2,), -0.1), _cu(13, 7))
+        out.backward(_randn(20, 2, 64, seed=2))
+    name, args = launches[-1]
+    assert name == 'genie_decay_attention_bwd'
+    for at, strides in ((0, 19), (1, 20), (2, 21)):
+        assert hooks.covers(args[at], list(args[strides]), (20, 2, 64)), (at, list(args[strides]))
+
+
+def _apart(t):
+    """The same values, nothing of them contiguous."""
+    wide = torch.empty((*t.shape, 2), dtype=t.dtype, device=t.device)
+    wide[..., 0] = t
+    return wide[..., 0]
+
+
+def _shifted(t):
+    """The same values at an address off 16 bytes."""
+    flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:].view(t.shape)
+    return flat.copy_(t)
+
+
+@pytest.mark.parametrize('back', [_dense, _apart, _shifted], ids=lambda f: f.__name__)
+def test_saved_tensors_that_come_back_in_any_layout_are_laid_out_for_the_kernels(launches, back):
+    """Every pointer of the backward launch that the kernels read as 16-byte pieces is aligned, every matrix has the strides given or is dense."""
+    from genie import functional as GF
+    rows = 300
+    q, k, v = _fused(rows, (2, 2, 2), 64, 1)
+    for call, bwd, aligned in ((lambda: GF.packed_attention(q, k, v, _cu(250, 50)), 'genie_packed_attention_bwd', (0, 1, 2, 3, 4, 5)),
+                               (lambda: GF.decay_attention(q, k, v, torch.full((2,), -0.1), _cu(250, 50)), 'genie_decay_attention_bwd', (0, 1, 2, 3, 7))):
+        with _Hooks(back):
+            call().backward(_randn(rows, 2, 64, seed=2))
+        name, args = launches[-1]
+        assert name == bwd and all(args[i] % 16 == 0 for i in aligned), args
+        strides = [tuple(a) for a in args if hasattr(a, '_length_')]
+        assert len(strides) == 4 and all(st == (128, 64) for st in strides), strides
+
+
+def test_saved_tensors_that_come_back_as_something_else_are_refused(launches):
+    from genie import functional as GF
+    q, k, v = _fused(20, (2, 2, 2), 64, 1)
+    for call in (lambda: GF.packed_attention(q, k, v, _cu(13, 7)), lambda: GF.decay_attention(q, k, v, torch.full((2,), -0.1), _cu(13, 7))):
+        for back in (lambda t: t.double(), lambda t: t[:-1]):
+            with _Hooks(back):
+                out = call()
+            before = len(launches)
+            with pytest.raises(RuntimeError, match='came back'):
+                out.backward(_randn(20, 2, 64, seed=2))
+            assert len(launches) == before
