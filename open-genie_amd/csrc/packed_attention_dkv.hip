@@ -310,6 +310,7 @@ __global__ void __launch_bounds__(256) packed_dkv_sum_kernel(const PackedArgs a)
 // measured: a step 1 us (64 keys per block), 2 us (128) or 4.2 us (256, width 128), 0.56 or 1 us per million pairs, 5 us, 6 TB/s.  The model agreed with the measured order
 // of n = 1 .. 8 on ten batches, e.g. 4 x 700 rows, 8 / 8 heads of width 64, n = 1, 2, 3: 33 / 40 / 44 us the whole backward; 16 / 4 heads, n = 3, 4, 5, 8: 57 / 55 / 56 / 64.
 static int packed_dkv_splits(int nseq, int rows_q, int rows_k, int hq, int hkv, int dim) {
+    if (rows_q == 0 || rows_k == 0) return 1;                                   // zeros: nothing to cut
     const float length = (float)rows_q / (float)(nseq > 0 ? nseq : 1);
     const float step = dim > 64 ? 4.2f * (float)dim / 128.f : packed_few(rows_q, hq, 512) ? 1.f : 2.f;
     const float chain = (length / 64.f + 1.f) * (float)(hq / hkv) * step;
@@ -327,9 +328,9 @@ static int packed_dkv_splits(int nseq, int rows_q, int rows_k, int hq, int hkv, 
     return best;
 }
 extern "C" int64_t genie_packed_attention_bwd_ws_floats(int nseq, int rows_q, int rows_k, int hq, int hkv, int dim) {
-    if (nseq < 0 || rows_q <= 0 || rows_k <= 0 || hkv <= 0 || hq <= 0 || hq % hkv != 0 || dim <= 0) return 0;
+    if (nseq < 0 || rows_q < 0 || rows_k < 0 || hkv <= 0 || hq <= 0 || hq % hkv != 0 || dim <= 0) return 0;
     const int n = packed_dkv_splits(nseq, rows_q, rows_k, hq, hkv, dim);
-    return (int64_t)hq * rows_q + 4 + (n > 1 ? (int64_t)2 * n * rows_k * hkv * dim : 0);      // delta (rounded up to 16 B), parts
+    return (int64_t)hq * rows_q + 4 + (n > 1 ? (int64_t)2 * n * rows_k * hkv * dim : 0);      // delta (rounded up to 16 B; written without keys, too), parts
 }
 
 template <int DH, int KT, int RG, int WPE, bool REST = false>

@@ -54,3 +54,24 @@ def test_gradients_after_a_round_trip_of_the_saved_tensors(lens, hook):
         with context():
             out = call(*fused.split(h, 1))
         assert torch.equal(torch.autograd.grad(out, fused, g)[0], want)
+
+
+@pytest.mark.parametrize('rows_q, rows_k', [(5, 0), (0, 16), (0, 5000), (5000, 0)])
+@pytest.mark.parametrize('hq, hkv, d', [(16, 1, 64), (8, 8, 128)])
+def test_packed_backward_entry_without_rows_on_one_side_stays_in_its_workspace(rows_q, rows_k, hq, hkv, d):
+    """The C entry with exactly the workspace it asks for: gradients are zero and nothing behind the workspace changes."""
+    from genie import _hip
+    lib, st, sk = _hip.load_library(), _hip.i64((hq * d, d)), _hip.i64((hkv * d, d))
+    q, k = _randn(rows_q + 1, hq, d, seed=1), _randn(rows_k + 1, hkv, d, seed=2)
+    dq, dk, dv = (torch.full_like(t, 3.0) for t in (q, k, k))
+    lse = torch.full((hq, rows_q + 1), float('-inf'), device='cuda')
+    need, spare = lib.genie_packed_attention_bwd_ws_floats(1, rows_q, rows_k, hq, hkv, d), 1 << 22
+    ws = torch.full((need + spare,), 7.0, device='cuda')
+    cu_q, cu_k = _cu([rows_q]), _cu([rows_k])
+    rc = lib.genie_packed_attention_bwd(*(t.data_ptr() for t in (q, k, k, q, q, q, lse, ws)), need, *(t.data_ptr() for t in (dq, dk, dv, cu_q, cu_k)), 1, rows_q, rows_k, hq, hkv, d,
+                                        st, sk, sk, st, 0.125, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, lib.genie_last_error()
+    torch.cuda.synchronize()
+    assert (ws[need:] == 7.0).all()
+    for t, rows in ((dq, rows_q), (dk, rows_k), (dv, rows_k)):
+        assert (t[:rows] == 0).all() and (t[rows:] == 3.0).all()

@@ -127,3 +127,15 @@ def test_saved_tensors_that_come_back_as_something_else_are_refused(launches):
             with pytest.raises(RuntimeError, match='came back'):
                 out.backward(_randn(20, 2, 64, seed=2))
             assert len(launches) == before
+
+
+@pytest.mark.parametrize('rows_q, rows_k', [(5, 0), (0, 16), (0, 0), (0, 5000), (5000, 0), (1, 1)])
+@pytest.mark.parametrize('hq, hkv, dim', [(16, 1, 64), (8, 8, 128)])
+def test_packed_backward_workspace_covers_calls_without_rows_on_one_side(rows_q, rows_k, hq, hkv, dim):
+    """delta is written for every query row, keys or not; and one float less than the query asks for is refused."""
+    from genie import _hip
+    lib, strides = _hip.load_library(), _hip.i64((hq * dim, dim))
+    need = lib.genie_packed_attention_bwd_ws_floats(1, rows_q, rows_k, hq, hkv, dim)
+    assert need >= hq * rows_q and need > 0
+    rc = lib.genie_packed_attention_bwd(*([16] * 8), need - 1, *([16] * 5), 1, rows_q, rows_k, hq, hkv, dim, strides, strides, strides, strides, 1.0, None)
+    assert rc == -1 and b'workspace' in lib.genie_last_error()
