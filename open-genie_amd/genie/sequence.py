@@ -103,6 +103,8 @@ def _direct(t: Tensor) -> Optional[Tuple[int, ...]]:
 
 def _rows(t: Tensor) -> Tuple[Tensor, Tuple[int, ...]]:
     """(rows, heads, d) or (batch, heads, d) ready for the kernels: the tensor itself where its layout allows, else a contiguous copy."""
+    if t.numel() == 0:                                            # (torch calls an empty tensor contiguous whatever its strides are)
+        return t, (t.shape[1] * t.shape[2], t.shape[2])
     st = _direct(t)
     if st is None or t.data_ptr() % 16:
         t = t.contiguous() if st is None else t.clone(memory_format=torch.contiguous_format)

@@ -75,3 +75,16 @@ def test_packed_backward_entry_without_rows_on_one_side_stays_in_its_workspace(r
     assert (ws[need:] == 7.0).all()
     for t, rows in ((dq, rows_q), (dk, rows_k), (dv, rows_k)):
         assert (t[:rows] == 0).all() and (t[rows:] == 3.0).all()
+
+
+def test_training_calls_without_rows_or_keys():
+    gf = _gf()
+    ld, s0 = torch.full((4,), -0.1, device='cuda'), torch.randn(1, 4, 64, 64, device='cuda')
+    for call in (lambda x: gf.packed_attention(x, x, x, _cu([0])), lambda x: gf.decay_attention(x, x, x, ld, _cu([0])),
+                 lambda x: gf.decay_attention(x, x, x, ld, _cu([0]), initial_state=s0)):
+        x = torch.zeros(0, 4, 64, dtype=torch.bfloat16, device='cuda', requires_grad=True)
+        call(x).sum().backward()
+        assert x.grad.shape == x.shape
+    q, k = _randn(5, 4, 64, seed=1).requires_grad_(True), torch.zeros(0, 4, 64, dtype=torch.bfloat16, device='cuda', requires_grad=True)
+    gf.packed_attention(q, k, k, _cu([5]), cu_seqlens_k=_cu([0])).sum().backward()
+    assert torch.equal(q.grad, torch.zeros_like(q)) and k.grad.shape == k.shape

@@ -139,3 +139,41 @@ def test_packed_backward_workspace_covers_calls_without_rows_on_one_side(rows_q,
     assert need >= hq * rows_q and need > 0
     rc = lib.genie_packed_attention_bwd(*([16] * 8), need - 1, *([16] * 5), 1, rows_q, rows_k, hq, hkv, dim, strides, strides, strides, strides, 1.0, None)
     assert rc == -1 and b'workspace' in lib.genie_last_error()
+
+
+def _empty(heads, d, kind):
+    """(0, heads, d) with the strides that an expanded gradient, a slice of a wider tensor or a row stride without 8 elements would have."""
+    if kind == 'expanded':
+        return torch.zeros((), dtype=torch.bfloat16).expand(0, heads, d)
+    if kind == 'sliced':
+        return torch.zeros(0, heads, 2 * d, dtype=torch.bfloat16)[..., ::2]
+    return torch.zeros(0, heads, d, dtype=torch.bfloat16).as_strided((0, heads, d), (3, 5, 1))
+
+
+@pytest.mark.parametrize('kind', ['expanded', 'sliced', 'odd'])
+def test_training_calls_without_rows(launches, kind):
+    """A batch without tokens: results and gradients are empty, whatever strides the empty tensors have, and nothing is launched."""
+    from genie import functional as GF
+    ld, s0 = torch.full((4,), -0.1), torch.randn(1, 4, 64, 64)
+    for call in (lambda x: GF.packed_attention(x, x, x, _cu(0)), lambda x: GF.decay_attention(x, x, x, ld, _cu(0)), lambda x: GF.decay_attention(x, x, x, ld, _cu(0), initial_state=s0)):
+        x = _empty(4, 64, kind).requires_grad_(True)
+        out = call(x)
+        assert out.shape == (0, 4, 64)
+        out.sum().backward()
+        assert x.grad.shape == x.shape
+        assert call(x.detach()).shape == x.shape
+    assert not launches
+
+
+@pytest.mark.parametrize('kind', ['expanded', 'sliced', 'odd'])
+def test_training_calls_without_keys(launches, kind):
+    from genie import functional as GF
+    q, k = _randn(5, 4, 64, seed=1).requires_grad_(True), _empty(4, 64, kind).requires_grad_(True)
+    out = GF.packed_attention(q, k, k, _cu(5), cu_seqlens_k=_cu(0))
+    assert torch.equal(out, torch.zeros_like(out))
+    out.sum().backward()
+    assert torch.equal(q.grad, torch.zeros_like(q)) and k.grad.shape == k.shape
+    out = GF.packed_attention(k, q, q, _cu(0), cu_seqlens_k=_cu(5))                 # keys, but no queries
+    q.grad = None
+    out.sum().backward()
+    assert torch.equal(q.grad, torch.zeros_like(q)) and not launches
