@@ -364,14 +364,14 @@ def cached_attention_step(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: 
     new = k_new is not None
     device, shape, nws, direct, tail = _planned(_cached_plan, (q, k_cache, v_cache, lengths, k_new, v_new), None if scale is None else float(scale))
     _no_grad_wanted(what, q, k_cache, v_cache, k_new, v_new)
+    if shape[0] == 0:
+        return q.new_empty(shape)
     kc, vc = k_cache.data_ptr(), v_cache.data_ptr()
     if (kc | vc) % 16:
         raise ValueError(f'{what}: {"k_cache" if kc % 16 else "v_cache"} must have a contiguous last axis and 16-byte aligned rows (it is updated in place and cannot be copied)')
     if new and kc == vc:
         raise ValueError(f'{what}: k_cache and v_cache are the same memory')
     out = q.new_empty(shape)
-    if shape[0] == 0:
-        return out
     ws = torch.empty(nws, dtype=torch.float32, device=device) if nws else None
     P = _hip.ptr
     sizes, cst, scale = tail

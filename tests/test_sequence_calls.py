@@ -177,3 +177,13 @@ def test_training_calls_without_keys(launches, kind):
     q.grad = None
     out.sum().backward()
     assert torch.equal(q.grad, torch.zeros_like(q)) and not launches
+
+
+def test_steps_without_sequences(launches):
+    from genie import functional as GF
+    for kind in ('expanded', 'sliced', 'odd'):
+        x = _empty(4, 64, kind)
+        assert GF.cached_attention_step(x, torch.zeros(0, 8, 4, 64, dtype=torch.bfloat16), torch.zeros(0, 8, 4, 64, dtype=torch.bfloat16),
+                                        torch.zeros(0, dtype=torch.int32), x, x).shape == (0, 4, 64)
+        assert GF.decay_attention_step(x, x, x, torch.zeros(4), torch.zeros(0, 4, 64, 64)).shape == (0, 4, 64)
+    assert not launches
