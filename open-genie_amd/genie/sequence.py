@@ -23,6 +23,7 @@ Common conventions
   * bitwise reproducible: no atomics, every sum has a fixed order.
   * capture of a backward pass into a graph: with no eager autograd graph of the same leaves alive (torch ends the process where it meets a leaf's node of another
     stream inside a capture; this holds for every differentiable operator).
+  * gradients of gradients and forward-mode differentiation (dual tensors) are refused.
   * weights (P, dS, decayed scores) are bf16 operands; up to 256 rows, and in the cached form, a second bf16 value carries what that left over.
   * a non-finite value in a token is not masked out: it may reach any row of its own sequence.
 """
@@ -33,6 +34,7 @@ from typing import Optional, Tuple, Union
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _hip
@@ -178,6 +180,12 @@ def _no_grad_wanted(what: str, *tensors: Optional[Tensor]) -> None:
         raise RuntimeError(f'{what} has no backward pass: call it under torch.no_grad(), or on tensors that do not require gradients')
 
 
+def _no_tangents(what: str, *tensors: Optional[Tensor]) -> None:
+    """Forward-mode differentiation has no formula here; a result without its tangent would be a wrong derivative of zero."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f'{what} has no forward-mode derivative (an argument is a dual tensor)')
+
+
 def _first_order(backward):
     """``once_differentiable``, whose bookkeeping (3 us of a small training call's 120) only runs where a graph of the backward pass is asked for."""
     recorded = once_differentiable(backward)
@@ -295,6 +303,7 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, cu_seqlens: Tensor, scale:
     ``cu_seqlens_k``: the keys' own packing, where a sequence has other keys than queries -- a prompt that continues a context.  The last query then sees the
     last key: query i of n sees keys ``0 .. i + n_k - n``.  A query that sees no key (``n_k < n``) returns zeros and has zero gradients."""
     scale, sizes, strides = _planned(_packed_plan, (q, k, v, cu_seqlens, cu_seqlens_k), None if scale is None else float(scale))
+    _no_tangents('packed_attention', q, k, v)
     if cu_seqlens_k is None:
         cu_seqlens_k = cu_seqlens
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
@@ -364,6 +373,7 @@ def cached_attention_step(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: 
     new = k_new is not None
     device, shape, nws, direct, tail = _planned(_cached_plan, (q, k_cache, v_cache, lengths, k_new, v_new), None if scale is None else float(scale))
     _no_grad_wanted(what, q, k_cache, v_cache, k_new, v_new)
+    _no_tangents(what, q, k_cache, v_cache, k_new, v_new)
     if shape[0] == 0:
         return q.new_empty(shape)
     kc, vc = k_cache.data_ptr(), v_cache.data_ptr()
@@ -512,6 +522,7 @@ def decay_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, cu_seqle
     last token, which ``decay_attention_step`` and a later call continue from.  States carry no gradient (truncated backpropagation)."""
     what = 'decay_attention'
     scale, direct = _planned(_decay_plan, (q, k, v, log_decay, cu_seqlens, initial_state), None if scale is None else float(scale))
+    _no_tangents(what, q, k, v, log_decay, initial_state)
     log_decay = _constant(what, 'the decays are constants (no gradient): pass log_decay.detach()', log_decay)
     if initial_state is not None:
         initial_state = _constant(what, 'no gradient flows into a state: pass initial_state.detach()', initial_state)
@@ -555,6 +566,7 @@ def decay_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, sta
     place, or into ``new_state`` (the old one then stays).  Returns (B, H, dv) bf16; no backward pass."""
     what = 'decay_attention_step'
     device, shape, direct, sizes, scale = _planned(_decay_step_plan, (q, k, v, log_decay, state, new_state), None if scale is None else float(scale))
+    _no_tangents(what, q, k, v, log_decay, state, new_state)
     log_decay = _constant(what, 'the decays are constants (no gradient): pass log_decay.detach()', log_decay)
     _no_grad_wanted(what, q, k, v, state, new_state)
     old = state.data_ptr()

@@ -187,3 +187,31 @@ def test_steps_without_sequences(launches):
                                         torch.zeros(0, dtype=torch.int32), x, x).shape == (0, 4, 64)
         assert GF.decay_attention_step(x, x, x, torch.zeros(4), torch.zeros(0, 4, 64, 64)).shape == (0, 4, 64)
     assert not launches
+
+
+def test_dual_tensors_are_refused(launches):
+    """Forward-mode differentiation: a result without its tangent would be a silent derivative of zero."""
+    from genie import functional as GF
+    import torch.autograd.forward_ad as fwad
+    x, s, ld = _randn(6, 2, 64, seed=1), torch.randn(6, 2, 64, 64), torch.full((2,), -0.1)
+    cache, n = [_randn(6, 10, 2, 64, seed=i) for i in (2, 3)], torch.zeros(6, dtype=torch.int32)
+    cu = _cu(6)
+
+    def dual(t):
+        return fwad.make_dual(t, torch.ones_like(t))
+
+    calls = [(GF.packed_attention, [x, x, x], lambda a: (*a, cu)), (GF.cached_attention_step, [x, *cache, x, x], lambda a: (*a[:3], n, *a[3:])),
+             (GF.decay_attention, [x, x, x, ld, torch.randn(1, 2, 64, 64)], lambda a: (*a[:4], cu, a[4])), (GF.decay_attention_step, [x, x, x, ld, s], lambda a: a)]
+    for call, given, order in calls:
+        for at in range(len(given)):
+            for grad in (False, True):
+                with fwad.dual_level(), torch.set_grad_enabled(grad):
+                    made = len(launches)
+                    with pytest.raises(NotImplementedError, match='forward-mode'):
+                        call(*order([dual(t) if i == at else t for i, t in enumerate(given)]))
+                    assert len(launches) == made
+        with fwad.dual_level():
+            call(*order(given))                                                   # (no dual among the arguments)
+    leaf = x.clone().requires_grad_(True)                                         # the same where a gradient is recorded as well
+    with fwad.dual_level(), pytest.raises(NotImplementedError, match='forward-mode'):
+        GF.packed_attention(dual(leaf), x, x, cu)
