@@ -15,7 +15,7 @@
 #   variants the bench on the same box with (a) the RCCL bucket all-reduces on a single-rank group, fp32 and bf16 payload, (b) the weight
 #            gradients on a side stream -- the side measurements DESIGN.md quotes next to the default line
 #                                                                          -> <tag>_bench_variants.jsonl
-#   guard    kernel-level suite under guard-page allocations, two file orders + the deliberate-overrun regression -> <tag>_guard_*.log
+#   guard    kernel-level suite under guard-page allocations, two file orders, and the harness itself -> <tag>_guard_*.log
 #   multigpu bench.py --gpus 2 (both all-reduce algorithms, bf16 payload) + the two-rank RCCL test, where two GPUs exist -> <tag>_bench_gpus2.jsonl
 #   pmc      SQ counters of the attention families and of the dominant conv layer (separate rocprofv3 passes)
 #                                                                          -> <tag>_pmc_attn.txt, <tag>_pmc_conv.txt
@@ -84,15 +84,14 @@ PY
       MB_BATCH=64 timeout 500 bash scripts/pmc_conv.sh > $OUT/${TAG}_pmc_conv.txt 2>&1 ;;
     guard)
       # kernel-level suite with every Python-side allocation behind guard pages (tests/guard.py), in TWO file orders (round 4's overrun showed
-      # in one order only), then the regression: the library with that overrun compiled back in must die under the harness
+      # in one order only), then the harness's own tests
       F1="tests/test_gpu_kernels.py tests/test_gpu_golden.py tests/test_gpu_attention.py tests/test_gpu_attention_dropout.py tests/test_gpu_maskgit.py tests/test_gpu_linear_ce.py"
       F2="tests/test_gpu_linear_ce.py tests/test_gpu_maskgit.py tests/test_gpu_golden.py tests/test_gpu_attention_dropout.py tests/test_gpu_attention.py tests/test_gpu_kernels.py"
       timeout 1500 python scripts/guard_run.py $F1 -q -m gpu -p no:cacheprovider -x 2>&1 | tail -6 > $OUT/${TAG}_guard_order1.log
       timeout 1500 python scripts/guard_run.py $F2 -q -m gpu -p no:cacheprovider -x 2>&1 | tail -6 > $OUT/${TAG}_guard_order2.log
-      make -C open-genie_amd probe -j 8 > $OUT/make_probe.log 2>&1      # incremental: rebuilt whenever the sources (or the ABI) moved since the last probe build
       timeout 900 python scripts/guard_run.py tests/test_gpu_random_geometry.py -q -m gpu -p no:cacheprovider 2>&1 | tail -4 > $OUT/${TAG}_guard_random_geometry.log
-      GENIE_GUARD_REGRESSION=1 timeout 600 python -m pytest tests/test_gpu_guard.py -q -m gpu -p no:cacheprovider 2>&1 | tail -4 > $OUT/${TAG}_guard_regression.log
-      for f in $OUT/${TAG}_guard_order1.log $OUT/${TAG}_guard_order2.log $OUT/${TAG}_guard_random_geometry.log $OUT/${TAG}_guard_regression.log; do tail -n 2 $f; done ;;
+      timeout 600 python -m pytest tests/test_gpu_guard.py -q -m gpu -p no:cacheprovider 2>&1 | tail -4 > $OUT/${TAG}_guard_harness.log
+      for f in $OUT/${TAG}_guard_order1.log $OUT/${TAG}_guard_order2.log $OUT/${TAG}_guard_random_geometry.log $OUT/${TAG}_guard_harness.log; do tail -n 2 $f; done ;;
     multigpu)
       # first contact with more than one GPU (no gpurun box has had two so far): the plain launcher branch of bench.py, both all-reduce
       # algorithms, fp32 and bf16 payload -> <tag>_bench_gpus2.jsonl with the `comm` object of each; skipped on a one-GPU box
