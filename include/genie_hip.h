@@ -540,7 +540,7 @@ int genie_cached_attention_step(const void* q, const void* k_new, const void* v_
                                 void* stream);
 /* Linear attention with a decay per head: S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T, o_t = scale q_t S_t; log_decay fp32 [heads] on the device, <= 0.
  * initial_state / final_state fp32 [nseq][heads][dk][dv], optional.  Sequences are cut into segments; states (bf16: the states in front of the segments, which the
- * backward call reads again) and ws (fp32) hold genie_decay_attention_state_elems elements each; it may be 0. */
+ * backward call reads again) and ws (fp32) hold genie_decay_attention_state_elems elements each; it may be 0.  Up to 256 rows with initial states it counts a second value for each state element: what its rounding left over. */
 int64_t genie_decay_attention_state_elems(int nseq, int rows, int heads, int dk, int dv, int has_initial);
 int genie_decay_attention_fwd(const void* q, const void* k, const void* v, const float* log_decay, const int32_t* cu, const float* initial_state, void* out,
                               float* final_state, void* states, float* ws, int64_t state_elems, int nseq, int rows, int heads, int dk, int dv,

@@ -14,7 +14,7 @@
 // (at head width 128 an fp32 matrix is as large as 128 tokens of q, k, v and o).
 // All powers have exponents >= 0 (strong decays underflow to 0, nothing overflows).
 //
-// Roundings to bf16: the scores and M as matrix operands of an output that is itself rounded to bf16.  The states themselves are fp32 and so is what goes into them:
+// Roundings to bf16: the scores and M as matrix operands of an output that is itself rounded to bf16 (up to 256 rows: as two values each, 2^-17 left).  The states themselves are fp32 and so is what goes into them:
 // the state update's decayed operand l^(n-1-s) c_s enters as a sum of three bf16 values (2^-24 left: fp32).  The backward's states, which only become
 // operands of gradients, take two (2^-16, far under the operand's own 2^-8).
 //
@@ -31,6 +31,7 @@ struct DecayRole {
     int da, dc, reverse, m_rows_a;               // m_rows_a: the stored states' rows are a's columns (else c's): the transposed use
     float* local;                                // [slot][heads][dc][da] fp32: what each segment adds
     bf16_t* states;                              // [slot][heads][dc][da] (m_rows_a: [da][dc]): state in front of each segment, or NULL
+    int64_t rest;                                // elements from a state to what its rounding left over (0: not kept)
     const float* initial;                        // [nseq][heads][da][dc]: state in front of each sequence, or NULL
     float* final_state;                          // [nseq][heads][da][dc], or NULL
 };
@@ -256,7 +257,14 @@ __global__ void __launch_bounds__(64 * NW) decay_scan_kernel(const DecayArgs g) 
             }
     }
     if (wave != 0) return;
-    if (nseg > 0) *reinterpret_cast<u32x2_t*>(dst + (nseg - 1) * step) = u32x2_t{pack_bf16x2(m[0], m[1]), pack_bf16x2(m[2], m[3])};
+    if (nseg > 0) {
+        const u32x2_t hi = {pack_bf16x2(m[0], m[1]), pack_bf16x2(m[2], m[3])};
+        *reinterpret_cast<u32x2_t*>(dst + (nseg - 1) * step) = hi;
+        if (R.rest)                                                              // (calls of one segment per sequence: m is the initial state)
+            *reinterpret_cast<u32x2_t*>(dst + (nseg - 1) * step + R.rest) =
+                u32x2_t{pack_bf16x2(m[0] - __uint_as_float(hi[0] << 16), m[1] - __uint_as_float(hi[0] & 0xffff0000u)),
+                        pack_bf16x2(m[2] - __uint_as_float(hi[1] << 16), m[3] - __uint_as_float(hi[1] & 0xffff0000u))};
+    }
     if (!R.final_state) return;
     if (nseg > 0) {
         const f32x4_t last = *reinterpret_cast<const f32x4_t*>(src + (nseg - 1) * step);
@@ -353,12 +361,13 @@ __device__ __forceinline__ void decay_out_block(const DecayArgs& g, int block, c
     };
     bf16x8_t af[G::KS];                                                          // (in front of the tiles' loads: the counted waits below count what is younger)
     packed_row_frags<DH>(af, arow, qi < s.len, R.da);
-    if (carried) {                                                               // the state: stages 0 and 1
+    auto load_state = [&](int64_t rest) {                                        // into stages 0 and 1
         const int mr = R.m_rows_a ? R.da : R.dc, mc = R.m_rows_a ? R.dc : R.da;
-        const bf16_t* m = R.states + ((int64_t)(s.start / DECAY_SEG + s.seq + seg) * g.heads + head) * mr * mc;
+        const bf16_t* m = R.states + ((int64_t)(s.start / DECAY_SEG + s.seq + seg) * g.heads + head) * mr * mc + rest;
 #pragma unroll
         for (int i = 0; i < G::DT; ++i) st.load(wave, smem + i * 32 * G::PITCH, m + i * 32 * mc, mc, mr - i * 32, mc, -1);
-    }
+    };
+    if (carried) load_state(0);
     load(0);
     if (!carried && tiles > 1) load(1);
     PackedLane<DH> at;
@@ -370,26 +379,36 @@ __device__ __forceinline__ void decay_out_block(const DecayArgs& g, int block, c
     for (int d = 0; d < G::DT; ++d) y[d] = packed_splat(0.f);
 
     if (carried) {
+        auto times_state = [&]() __attribute__((always_inline)) {                // y += a M
+            if (!R.m_rows_a) {
+#pragma unroll
+                for (int ks = 0; ks < G::KS; ++ks)
+#pragma unroll
+                    for (int d = 0; d < G::DT; ++d) y[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at.row_frag(smem + d * 32 * G::PITCH, ks), af[ks], y[d], 0, 0, 0);
+            } else {
+                // the transposing read delivers columns of a in the accumulator order, 4 h .. + 3 and 8 + 4 h .. + 3 of 16; af holds 8 h .. + 7: the lanes of a row trade halves
+#pragma unroll
+                for (int k2 = 0; k2 < G::KS; k2 += 2) {
+                    bf16x8_t ap[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const u32x4_t f = __builtin_bit_cast(u32x4_t, af[k2 + e]);
+                        const auto x = __builtin_amdgcn_permlane32_swap(f[0], f[2], false, false), z = __builtin_amdgcn_permlane32_swap(f[1], f[3], false, false);
+                        ap[e] = __builtin_bit_cast(bf16x8_t, u32x4_t{x[0], z[0], x[1], z[1]});
+                    }
+                    decay_tr_product<DH>(y, at, smem + k2 * 16 * G::PITCH, ap);
+                }
+            }
+        };
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(MINE) : "memory");
         __syncthreads();
-        if (!R.m_rows_a) {
-#pragma unroll
-            for (int ks = 0; ks < G::KS; ++ks)
-#pragma unroll
-                for (int d = 0; d < G::DT; ++d) y[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at.row_frag(smem + d * 32 * G::PITCH, ks), af[ks], y[d], 0, 0, 0);
-        } else {
-            // the transposing read delivers columns of a in the accumulator order, 4 h .. + 3 and 8 + 4 h .. + 3 of 16; af holds 8 h .. + 7: the lanes of a row trade halves
-#pragma unroll
-            for (int k2 = 0; k2 < G::KS; k2 += 2) {
-                bf16x8_t ap[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const u32x4_t f = __builtin_bit_cast(u32x4_t, af[k2 + e]);
-                    const auto x = __builtin_amdgcn_permlane32_swap(f[0], f[2], false, false), z = __builtin_amdgcn_permlane32_swap(f[1], f[3], false, false);
-                    ap[e] = __builtin_bit_cast(bf16x8_t, u32x4_t{x[0], z[0], x[1], z[1]});
-                }
-                decay_tr_product<DH>(y, at, smem + k2 * 16 * G::PITCH, ap);
-            }
+        times_state();
+        if (REST && R.rest) {                                                    // few rows: the state with what its rounding left over
+            __syncthreads();
+            load_state(R.rest);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            times_state();
         }
         const float lead = decay_pow(log2_l, qi - seg0 + 1);
 #pragma unroll
@@ -456,7 +475,7 @@ __global__ void __launch_bounds__(256, DH <= 64 ? 4 : 3) decay_out_kernel(const 
     __shared__ __attribute__((aligned(16))) char smem[decay_out_lds<DH>];
     decay_out_block<DH, false>(g, (int)blockIdx.x, smem);
 }
-// Few rows: the weights with what their rounding left over, for the reason at packed_exact() (a 32768-token prompt would pay 38 us for 33).  Where every sequence is one
+// Few rows: the weights and the state in front of a sequence with what their rounding left over, for the reason at packed_exact() (a 32768-token prompt would pay 38 us for 33).  Where every sequence is one
 // segment and starts from nothing, the final states come from the launch's last blocks: three snippets of 168 tokens together 8 us instead of 7 + 7 in two launches.
 template <int DH>
 __global__ void __launch_bounds__(256) decay_few_kernel(const DecayArgs g, int out_blocks) {
@@ -534,10 +553,12 @@ __global__ void __launch_bounds__(256) decay_step_kernel(const DecayStepArgs a) 
 // ------------------------------------------------------------------------------------------------------------------------------
 // C entry points
 // ------------------------------------------------------------------------------------------------------------------------------
-// matrix elements of a call's segment states (one bf16 operand and one fp32 sum each); none where every sequence is one segment and starts from nothing
+// matrix elements of a call's segment states (one bf16 operand and one fp32 sum each); none where every sequence is one segment and starts from nothing.  Up to a
+// segment of rows with initial states: twice as many, the second half for what the operands' rounding left over.
+static bool decay_keeps_rest(int rows, bool initial) { return initial && rows <= DECAY_SEG; }
 extern "C" int64_t genie_decay_attention_state_elems(int nseq, int rows, int heads, int dk, int dv, int has_initial) {
     if (nseq <= 0 || rows <= 0 || heads <= 0 || dk <= 0 || dv <= 0 || (rows <= DECAY_SEG && !has_initial)) return 0;
-    return (int64_t)(rows / DECAY_SEG + nseq + 1) * heads * dk * dv;
+    return (int64_t)(rows / DECAY_SEG + nseq + 1) * heads * dk * dv * (decay_keeps_rest(rows, has_initial) ? 2 : 1);
 }
 
 static int decay_check(const char* what, const DecayArgs& g) {
@@ -605,6 +626,7 @@ extern "C" int genie_decay_attention_fwd(const void* q, const void* k, const voi
     const int64_t need = genie_decay_attention_state_elems(nseq, rows, heads, dk, dv, initial_state != nullptr);
     GENIE_CHECK_ARG(state_elems >= need && (need == 0 || (states && ws)), "%s: workspace too small", what);
     if (need == 0) { r.states = nullptr; r.local = nullptr; }
+    r.rest = decay_keeps_rest(rows, initial_state) ? need / 2 : 0;
     g.roles = 1;
     return decay_run_any(g, stream);
 }
@@ -638,6 +660,7 @@ extern "C" int genie_decay_attention_bwd(const void* q, const void* k, const voi
     const int64_t need = genie_decay_attention_state_elems(nseq, rows, heads, dk, dv, 0);
     GENIE_CHECK_ARG(state_elems >= need && (need == 0 || (states && rev_states && ws)) && (!has_initial || states), "%s: workspace too small", what);
     if (need > 0) { rv.states = rk.states = (bf16_t*)rev_states; rv.local = ws; }
+    rq.rest = decay_keeps_rest(rows, has_initial) ? genie_decay_attention_state_elems(nseq, rows, heads, dk, dv, 1) / 2 : 0;
     g.roles = 3;
     return decay_run_any(g, stream);
 }

@@ -24,7 +24,8 @@ Common conventions
   * capture of a backward pass into a graph: with no eager autograd graph of the same leaves alive (torch ends the process where it meets a leaf's node of another
     stream inside a capture; this holds for every differentiable operator).
   * gradients of gradients and forward-mode differentiation (dual tensors) are refused.
-  * weights (P, dS, decayed scores) are bf16 operands; up to 256 rows, and in the cached form, a second bf16 value carries what that left over.
+  * weights (P, dS, decayed scores) and the state in front of a segment are bf16 operands; in calls of up to 256 rows (of the buffers: those behind the last sequence
+    count), and in the cached form always, a second bf16 value carries what that left over.  In longer calls a carried state enters outputs and dq as one bf16 value.
   * a non-finite value in a token is not masked out: it may reach any row of its own sequence.
 """
 from __future__ import annotations

@@ -3,6 +3,7 @@ own workspaces, versions of tensors that are updated in place, values that are n
 import pytest
 import torch
 
+import sequence_ref as R
 import util  # noqa: F401  (paths)
 
 pytestmark = pytest.mark.gpu
@@ -88,3 +89,25 @@ def test_training_calls_without_rows_or_keys():
     q, k = _randn(5, 4, 64, seed=1).requires_grad_(True), torch.zeros(0, 4, 64, dtype=torch.bfloat16, device='cuda', requires_grad=True)
     gf.packed_attention(q, k, k, _cu([5]), cu_seqlens_k=_cu([0])).sum().backward()
     assert torch.equal(q.grad, torch.zeros_like(q)) and k.grad.shape == k.shape
+
+
+@pytest.mark.parametrize('lens, spare', [([1], 0), ([2, 0, 3], 5), ([70, 130, 56], 0), ([256], 0)], ids=str)
+@pytest.mark.parametrize('dk, dv', [(32, 32), (64, 64), (96, 64), (24, 128), (128, 128)])
+def test_few_rows_carry_their_state_without_rounding_it(lens, spare, dk, dv):
+    """Up to 256 rows a state in front of a sequence enters outputs and dq with its rounding's remainder: U^2 of it is left, as of the weights."""
+    gf, rows, h, w = _gf(), sum(lens) + spare, 3, R.U ** 2
+    q, k, v, g = (_randn(rows, h, d, seed=20 + i) for i, d in enumerate((dk, dk, dv, dv)))
+    for t in (q, k, v, g):
+        t[rows - spare:] = float('nan')
+    ld = torch.tensor([-0.01, 0.0, -0.7], device='cuda')
+    s0 = torch.randn((len(lens), h, dk, dv), generator=torch.Generator(device='cuda').manual_seed(24), device='cuda') * 8
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    out, last = gf.decay_attention(q, k, v, ld, _cu(lens), initial_state=s0, return_state=True)
+    dq = torch.autograd.grad(out, q, g)[0]
+    used, tiny = sum(lens), 2.0 ** -100
+    for name, got, (val, tol) in (('out', out, R.decay_form(q.detach(), k.detach(), v.detach(), ld, lens, dk ** -0.5, state=s0, w=w)),
+                                  ('dq', dq, R.decay_form(g, v.detach(), k.detach(), ld, lens, dk ** -0.5, state=s0.transpose(2, 3), w=w))):
+        R.assert_within(got[:used], val[:used], tol[:used] + tiny, name)
+        assert (got[used:] == 0).all()
+    R.assert_within(last, *R.decay_state(k.detach(), v.detach(), ld, lens, s0), 'state')
