@@ -54,7 +54,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, W
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int d = 0; d < G::DT; ++d) dk[kt][d] = dv[kt][d] = packed_splat(0.f);
-    const float c2 = a.scale * 1.4426950408889634f, inv_scale = 1.f / a.scale;
+    // (scales under 1e-36 count as 1e-36 in the exponent, where neither leaves anything of a score: lse / scale stays an fp32 number)
+    const float es = fmaxf(a.scale, 1e-36f), c2 = es * 1.4426950408889634f, inv_scale = 1.f / es;
 
     PackedDma<DH, NW, 1, false> st;
     st.init(wave, lane, a.dim, a.q_row, a.g_row);

@@ -111,3 +111,23 @@ def test_few_rows_carry_their_state_without_rounding_it(lens, spare, dk, dv):
         R.assert_within(got[:used], val[:used], tol[:used] + tiny, name)
         assert (got[used:] == 0).all()
     R.assert_within(last, *R.decay_state(k.detach(), v.detach(), ld, lens, s0), 'state')
+
+
+@pytest.mark.parametrize('lens', [[40, 3], [300, 170]], ids=str)
+@pytest.mark.parametrize('d', [64, 128])
+@pytest.mark.parametrize('scale', [1e-44, 1e-39, 1e-37, 1e-20, 1e-3, 1.0, 3.0])
+def test_packed_gradients_at_any_scale(lens, d, scale, monkeypatch):
+    """From scales whose inverse is no fp32 number (all keys weigh the same) to ones that leave a few keys."""
+    gf, rows, hq, hkv = _gf(), sum(lens), 4, 2
+    q, k, v, g = (_randn(rows, h, d, seed=30 + i) for i, h in enumerate((hq, hkv, hkv, hq)))
+    # a score is a sum of d fp32 products: off by d 2^-24 of its magnitudes at worst, in the weight's exponent and in the log-sum-exp's
+    most = scale * torch.einsum('ihd,jhd->hij', q.float().abs(), k.float().abs().repeat_interleave(2, 1)).max().item()
+    monkeypatch.setattr(R, 'SLACK', R.SLACK + 2 * d * 2.0 ** -24 * most)
+    val, tol = R.packed_reference(q, k, v, lens, scale, g)
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    out = gf.packed_attention(q, k, v, _cu(lens), scale=scale)
+    for name, t in zip(('out', 'dq', 'dk', 'dv'), (out, *torch.autograd.grad(out, (q, k, v), g))):
+        # (results under the smallest normal number may be rounded to their multiples of 2^-133, or to zero)
+        R.assert_within(t, torch.where(val[name].abs() < 2.0 ** -126, t.double(), val[name]), tol[name] + 2.0 ** -126, name)
+        assert name in ('dq', 'dk') or (t != 0).any()
