@@ -393,6 +393,8 @@ def cached_attention_step(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: 
             (k_new, skn), (v_new, svn) = _rows(k_new), _rows(v_new)
             direct = _i64(sq), _i64(skn), _i64(svn)
     _launch('genie_cached_attention_step', device, P(q), P(k_new), P(v_new), kc, vc, P(lengths), P(out), P(ws), nws, *sizes, *direct, *cst, scale)
+    if new:
+        torch._C._increment_version((k_cache, v_cache))           # (written behind autograd's back: a graph that kept the old values must not use these)
     return out
 
 
@@ -583,4 +585,5 @@ def decay_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, sta
         (q, sq), (k, sk), (v, sv) = _rows(q), _rows(k), _rows(v)
         direct = _i64(sq), _i64(sk), _i64(sv)
     _launch('genie_decay_attention_step', device, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), old, new, out.data_ptr(), *sizes, *direct, scale)
+    torch._C._increment_version((state if new_state is None else new_state,))
     return out

@@ -215,3 +215,32 @@ def test_dual_tensors_are_refused(launches):
     leaf = x.clone().requires_grad_(True)                                         # the same where a gradient is recorded as well
     with fwad.dual_level(), pytest.raises(NotImplementedError, match='forward-mode'):
         GF.packed_attention(dual(leaf), x, x, cu)
+
+
+def test_tensors_updated_in_place_say_so(launches):
+    """Caches and states are written by the kernels: autograd sees a new version, and a graph that kept the old values refuses instead of using the new ones."""
+    from genie import functional as GF
+    x, n = _randn(6, 2, 64, seed=1), torch.zeros(6, dtype=torch.int32)
+    kc, vc, ld = _randn(6, 10, 2, 64, seed=2), _randn(6, 10, 2, 64, seed=3), torch.full((2,), -0.1)
+    state, into = torch.randn(6, 2, 64, 64), torch.zeros(6, 2, 64, 64)
+
+    def versions():
+        return [t._version for t in (x, n, kc, vc, ld, state, into)]
+
+    at = versions()
+    GF.cached_attention_step(x, kc, vc, n)                                        # nothing is written
+    assert versions() == at
+    GF.cached_attention_step(x, kc, vc, n, x, x)
+    assert [b - a for a, b in zip(at, versions())] == [0, 0, 1, 1, 0, 0, 0]
+    GF.decay_attention_step(x, x, x, ld, state)
+    assert [b - a for a, b in zip(at, versions())] == [0, 0, 1, 1, 0, 1, 0]
+    GF.decay_attention_step(x, x, x, ld, state, new_state=into)
+    assert [b - a for a, b in zip(at, versions())] == [0, 0, 1, 1, 0, 1, 1]
+    w = torch.randn(6, 2, 64, 64, requires_grad=True)
+    loss = (w * state).sum()
+    with torch.no_grad():
+        GF.decay_attention_step(x, x, x, ld, state)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        loss.backward()
+    with torch.inference_mode():
+        GF.decay_attention_step(x, x, x, ld, torch.zeros(6, 2, 64, 64))             # (tensors without versions)
