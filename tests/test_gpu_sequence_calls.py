@@ -131,3 +131,98 @@ def test_packed_gradients_at_any_scale(lens, d, scale, monkeypatch):
         # (results under the smallest normal number may be rounded to their multiples of 2^-133, or to zero)
         R.assert_within(t, torch.where(val[name].abs() < 2.0 ** -126, t.double(), val[name]), tol[name] + 2.0 ** -126, name)
         assert name in ('dq', 'dk') or (t != 0).any()
+
+
+# ------------------------------------------------------------------------------------------------------------------------------------
+# forms and bounds that tests/test_gpu_sequence.py does not reach
+# ------------------------------------------------------------------------------------------------------------------------------------
+def _state_bound(log_decay, lens, mag):
+    """Final states: the decayed operand l^e c is a sum of three bf16 values (U^3 = 2^-24 of it is left) and one fp32 product; its power carries the roundings of log2 l and of
+    their product with e (together 2^-23 of the exponent, log2 l e < |log_decay| 1.5 len) and the hardware's 2^-23; the sum over a sequence adds three products a
+    token, 2^-24 each.  A state in front of the sequence goes through one such power and one sum."""
+    lens = torch.tensor(lens, dtype=torch.float64, device=mag.device)[:, None]
+    span = (log_decay.double().clamp(min=-60).abs()[None, :] * 1.5 * lens).clamp(max=90)      # (past 2^-90 the term itself is gone)
+    return mag * (2.0 ** -24 * (3 * lens + 8 + 2 * span))[:, :, None, None]
+
+
+@pytest.mark.parametrize('lens', [[2], [3, 1, 2], [2, 5, 0, 3], [3] * 100, [1 + i % 7 for i in range(90)]], ids=lambda x: f'{len(x)}x{x[0]}')
+@pytest.mark.parametrize('dk, dv', [(64, 64), (128, 128), (32, 96), (104, 40), (8, 128)])
+@pytest.mark.parametrize('state', [False, True])
+def test_final_states_of_short_sequences_are_fp32(lens, dk, dv, state):
+    """Both forms (up to 256 rows in one launch, more in three), square and not: the states hold what fp32 holds, not what two bf16 values do."""
+    gf, h, n = _gf(), 3, sum(lens)
+    q, k, v = (_randn(n, h, d, seed=50 + i) for i, d in enumerate((dk, dk, dv)))
+    ld = torch.tensor([-0.3, -1.7, -0.01], device='cuda')
+    s0 = torch.randn((len(lens), h, dk, dv), generator=torch.Generator(device='cuda').manual_seed(54), device='cuda') if state else None
+    out, last = gf.decay_attention(q, k, v, ld, _cu(lens), initial_state=s0, return_state=True)
+    val, bound = R.decay_state(k, v, ld, lens, s0)
+    mag = bound / (R.U * R.U + 2.0 ** -18)
+    R.assert_within(last, val, _state_bound(ld, lens, mag), 'state')
+    R.assert_within(out, *R.decay_form(q, k, v, ld, lens, dk ** -0.5, state=s0), 'out')
+
+
+@pytest.mark.parametrize('heads', [(20, 1), (40, 2), (4, 4)], ids=str)
+@pytest.mark.parametrize('d', [8, 24, 40, 80, 96, 120])
+def test_cached_step_split_at_every_width(heads, d):
+    """Caches split over blocks, with and without a token to append: joins whose threads do not divide evenly, more query heads to a key head than a product has columns."""
+    gf, (hq, hkv), cap = _gf(), heads, 2600
+    lengths = [2599, 1300, 0, -1, 33]
+    b = len(lengths)
+    q, kn, vn = _randn(b, hq, d, seed=60), _randn(b, hkv, d, seed=61), _randn(b, hkv, d, seed=62)
+    kc, vc = _randn(b, cap, hkv, d, seed=63), _randn(b, cap, hkv, d, seed=64)
+    n = torch.tensor(lengths, dtype=torch.int32, device='cuda')
+    val, tol = R.step_reference(q, kc, vc, lengths, d ** -0.5)
+    R.assert_within(gf.cached_attention_step(q, kc, vc, n), val, tol, 'without a token')
+    out = gf.cached_attention_step(q, kc, vc, n, kn, vn)
+    for i, m in enumerate(lengths):
+        if m >= 0:
+            assert torch.equal(kc[i, m], kn[i]) and torch.equal(vc[i, m], vn[i])
+    val, tol = R.step_reference(q, kc, vc, [m + 1 for m in lengths], d ** -0.5)
+    R.assert_within(out, val, tol, 'with a token')
+
+
+@pytest.mark.parametrize('b, cap', [(3, 60), (3, 3000), (300, 90)])
+@pytest.mark.parametrize('d', [64, 128])
+def test_cached_step_with_values_that_are_not_finite(b, cap, d):
+    """One wide block, several parts, four waves: NaN stays in its sequence, key head and (in a value) column; a score of minus infinity is a key that is not there."""
+    gf, hq, hkv = _gf(), 4, 2
+    q, kc, vc = _randn(b, hq, d, seed=70), _randn(b, cap, hkv, d, seed=71), _randn(b, cap, hkv, d, seed=72)
+    full = torch.full((b,), cap, dtype=torch.int32, device='cuda')
+    want = gf.cached_attention_step(q, kc, vc, full)
+    rest = torch.ones_like(want, dtype=torch.bool)
+    rest[1] = False
+
+    def call(q=q, kc=kc, vc=vc, n=full):
+        return gf.cached_attention_step(q, kc, vc, n)
+
+    for at in (0, cap // 2, cap - 1):
+        bad = kc.clone()
+        bad[1, at, 0, 3] = float('nan')
+        out = call(kc=bad)
+        assert torch.isnan(out[1, :2]).all() and torch.equal(out[1, 2:], want[1, 2:]) and torch.equal(out[rest], want[rest])
+        bad = vc.clone()
+        bad[1, at, 1, 5] = float('nan')
+        out = call(vc=bad)
+        assert torch.isnan(out[1, 2:, 5]).all() and torch.equal(out[rest], want[rest]) and torch.equal(out[1, :2], want[1, :2])
+        cols = [c for c in range(d) if c != 5]
+        assert torch.equal(out[1, 2:][:, cols], want[1, 2:][:, cols])
+        bad, sign = kc.clone(), q.clone()
+        bad[1, at, 0] = 0
+        bad[1, at, 0, 0] = float('inf')
+        sign[1, 0, 0], sign[1, 1, 0] = -2.0, 2.0                                  # query head 0: a score of -inf; head 1: +inf, whose softmax is NaN
+        out = call(q=sign, kc=bad)
+        assert torch.isnan(out[1, 1]).all()
+        keep = [j for j in range(cap) if j != at]
+        val, tol = R.step_reference(sign[1:2, :1], kc[1:2, keep, :1], vc[1:2, keep, :1], [cap - 1], d ** -0.5)
+        R.assert_within(out[1:2, :1], val, tol, 'without the key')
+    bad = kc.clone()
+    bad[1] = float('nan')                                                         # nothing but NaN, in every wave and part; and as the only key
+    out = call(kc=bad)
+    assert torch.isnan(out[1]).all() and torch.equal(out[rest], want[rest])
+    one = full.clone()
+    one[1] = 1
+    assert torch.isnan(call(kc=bad, n=one)[1]).all()
+    bad = q.clone()
+    bad[1, 2] = float('nan')
+    out = call(q=bad)
+    assert torch.isnan(out[1, 2]).all() and torch.equal(out[rest], want[rest]) and torch.equal(out[1, [0, 1, 3]], want[1, [0, 1, 3]])

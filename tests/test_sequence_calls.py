@@ -244,3 +244,47 @@ def test_tensors_updated_in_place_say_so(launches):
         loss.backward()
     with torch.inference_mode():
         GF.decay_attention_step(x, x, x, ld, torch.zeros(6, 2, 64, 64))             # (tensors without versions)
+
+
+def _ballot_search(cu, rows, tile, first, slot):
+    """The 64 lanes of the longest-first search, level by level as a wave walks them -> (sequence, tile); the sequence behind the last holds the spare rows."""
+    lane, nseq = torch.arange(64), len(cu) - 1
+    clamped = [0] + [min(max(c, 0), rows) for c in cu[1:]]
+    start, after = [clamped[min(i, nseq)] for i in range(64)], [clamped[min(i + 1, nseq)] for i in range(64)]
+    n = torch.tensor([(max(0, b - a) + tile - 1) // tile for a, b in zip(start, after)])
+    lo, width, above = 0, rows // tile + 2, 0
+    while True:
+        step = (width + 62) // 63
+        c = (n[:nseq, None] - (lo + lane * step)[None, :]).clamp(min=0).sum(0)
+        if lo == 0 and slot >= int(c[0]):
+            return nseq, slot - int(c[0])
+        hits = max(1, int((c > slot).sum()))
+        assert hits == 1 or bool((c[:hits] > slot).all())                         # the ballot is a prefix
+        lo, above, width = lo + (hits - 1) * step, int(c[min(hits, 63)]), step
+        if width <= 1:
+            break
+    who = [i for i in range(64) if int(n[i]) > lo][slot - above:]
+    length = after[who[0]] - start[who[0]]
+    return who[0], (length + tile - 1) // tile - 1 - lo if first else lo
+
+
+@pytest.mark.parametrize('seed', range(12))
+@pytest.mark.parametrize('first', [False, True])
+def test_longest_first_search_covers_every_tile_once_in_order(seed, first):
+    import random
+    rng = random.Random(seed)
+    tile = rng.choice([64, 128, 256])
+    lens = [rng.choice([0, 1, tile - 1, tile, tile + 1, rng.randint(0, 40 * tile)]) for _ in range(rng.choice([1, 2, 7, 62, 63]))]
+    if seed == 0:
+        lens = [70 * tile + 3, 5, 64 * tile]                                      # more tiles than one level of the search tells apart
+    cu, spare = [0], rng.choice([0, 1, 3 * tile + 5])
+    for x in lens:
+        cu.append(cu[-1] + x)
+    rows = cu[-1] + spare
+    found = [_ballot_search(cu, rows, tile, first, slot) for slot in range(rows // tile + len(lens) + 1)]
+    real = [(s, t) for s, t in found if s < len(lens)]
+    assert sorted(real) == [(s, t) for s, n in enumerate(lens) for t in range((n + tile - 1) // tile)]
+    work = [((lens[s] + tile - 1) // tile - 1 - t) if first else t for s, t in real]
+    assert work == sorted(work, reverse=True)
+    behind = [t for s, t in found if s == len(lens)]
+    assert behind == list(range(len(behind))) and len(behind) * tile >= spare
