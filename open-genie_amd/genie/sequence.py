@@ -217,7 +217,7 @@ def _packed_forward(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Tensor,
         _launch('genie_packed_attention_fwd', q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lo, lse, cu_q.data_ptr(), cu_k.data_ptr(), *sizes, *strides, scale)
     else:
         out.zero_()
-    return out, (q, k, v, out, rest, cu_q, cu_k)
+    return out, (q, k, v, out, rest, cu_q, None if cu_k is cu_q else cu_k)
 
 
 def _packed_bwd_plan(q, k, v, out, rest, cu_q, cu_k, dout, sizes):
@@ -226,10 +226,10 @@ def _packed_bwd_plan(q, k, v, out, rest, cu_q, cu_k, dout, sizes):
     nseq, rows, rows_k, hq, hkv, d = sizes
     for t, name, dtype, shape in ((q, 'q', torch.bfloat16, (rows, hq, d)), (k, 'k', torch.bfloat16, (rows_k, hkv, d)), (v, 'v', torch.bfloat16, (rows_k, hkv, d)),
                                   (out, 'the output', torch.bfloat16, (rows, hq, d)), (rest, 'its remainder', torch.float32, (rows * hq * (d // 2 + 1),)),
-                                  (cu_q, 'cu_seqlens', torch.int32, (nseq + 1,)), (cu_k, 'cu_seqlens_k', torch.int32, (nseq + 1,))):
+                                  (cu_q, 'cu_seqlens', torch.int32, (nseq + 1,)), (cu_q if cu_k is None else cu_k, 'cu_seqlens_k', torch.int32, (nseq + 1,))):
         _came_back(what, t, name, dtype, shape, dev)
     strides = [_direct(t) for t in (q, k, v, dout)]
-    direct = None not in strides and all(t.is_contiguous() for t in (out, rest, cu_q, cu_k))
+    direct = None not in strides and all(t is None or t.is_contiguous() for t in (out, rest, cu_q, cu_k))
     return tuple(map(_i64, strides)) if direct else None, _hip.load_library().genie_packed_attention_bwd_ws_floats(*sizes)
 
 
@@ -254,6 +254,7 @@ class _PackedAttention(torch.autograd.Function):
                 (q, sq), (k, sk), (v, sv), (dout, sg) = _rows(q), _rows(k), _rows(v), _rows(dout)
                 strides = _i64(sq), _i64(sk), _i64(sv), _i64(sg)
                 out, rest, cu_q, cu_k = _dense(out), _dense(rest), _dense(cu_q), _dense(cu_k)
+            cu_k = cu_q if cu_k is None else cu_k
             lo = rest.data_ptr()
             ws = torch.empty(nws, dtype=torch.float32, device=q.device)
             _launch('genie_packed_attention_bwd', q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lo, dout.data_ptr(), lo + rows * hq * d * 2, ws.data_ptr(), nws,
