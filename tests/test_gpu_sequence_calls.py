@@ -226,3 +226,77 @@ def test_cached_step_with_values_that_are_not_finite(b, cap, d):
     bad[1, 2] = float('nan')
     out = call(q=bad)
     assert torch.isnan(out[1, 2]).all() and torch.equal(out[rest], want[rest]) and torch.equal(out[1, [0, 1, 3]], want[1, [0, 1, 3]])
+
+
+@pytest.mark.parametrize('state', [False, True])
+@pytest.mark.parametrize('d', [32, 128])
+def test_more_sequences_than_one_search_level_in_few_rows(d, state):
+    """200 sequences of 0, 1 and 2 tokens in 199 rows: forward, final states and gradients of both operators."""
+    gf, h, lens = _gf(), 2, [i % 3 for i in range(200)]
+    n, w, tiny = sum(lens), R.U ** 2, 2.0 ** -100
+    q, k, v, g = (_randn(n, h, d, seed=90 + i).requires_grad_(i < 3) for i in range(4))
+    ld = torch.tensor([-0.2, -1.0], device='cuda')
+    s0 = torch.randn((200, h, d, d), generator=torch.Generator(device='cuda').manual_seed(94), device='cuda') if state else None
+    out, last = gf.decay_attention(q, k, v, ld, _cu(lens), initial_state=s0, return_state=True)
+    grads = torch.autograd.grad(out, (q, k, v), g)
+    a, b, c = (t.detach() for t in (q, k, v))
+    st = None if s0 is None else s0.transpose(2, 3)
+    R.assert_within(last, *R.decay_state(b, c, ld, lens, s0), 'state')
+    for name, got, (val, tol) in (('out', out, R.decay_form(a, b, c, ld, lens, d ** -0.5, state=s0, w=w)), ('dq', grads[0], R.decay_form(g, c, b, ld, lens, d ** -0.5, state=st, w=w)),
+                                  ('dk', grads[1], R.decay_form(c, g, a, ld, lens, d ** -0.5, reverse=True, w=w)),
+                                  ('dv', grads[2], R.decay_form(b, a, g, ld, lens, d ** -0.5, reverse=True, w=w))):
+        R.assert_within(got, val, tol + tiny, name)
+    out = gf.packed_attention(q, k, v, _cu(lens))
+    val, tol = R.packed_reference(a, b, c, lens, d ** -0.5, g, w=w)
+    for name, got in zip(('out', 'dq', 'dk', 'dv'), (out, *torch.autograd.grad(out, (q, k, v), g))):
+        R.assert_within(got, val[name], tol[name] + tiny, name)
+
+
+@pytest.mark.parametrize('rows', [150, 3000])
+def test_wide_heads_in_a_captured_graph(rows):
+    """Heads of 128 (blocks with more than 64 KB of LDS), a state in front, forward and backward captured and replayed with other lengths; eager work between the replays."""
+    gf, d = _gf(), 128
+    q, k, v, g = (_randn(rows, h, d, seed=100 + i).requires_grad_(i < 3) for i, h in enumerate((4, 2, 2, 4)))
+    s0 = torch.randn((3, 2, d, d), generator=torch.Generator(device='cuda').manual_seed(104), device='cuda')
+    ld, cu = torch.tensor([-0.02, -0.4], device='cuda'), _cu([rows - 40, 0, 40])
+    kc, vc = _randn(3, 500, 2, d, seed=105), _randn(3, 500, 2, d, seed=106)
+    n = torch.tensor([3, 499, 70], dtype=torch.int32, device='cuda')
+
+    def everything():
+        a = gf.packed_attention(q, k, v, cu)
+        b, last = gf.decay_attention(q[:, :2], k, v, ld, cu, initial_state=s0, return_state=True)
+        with torch.no_grad():
+            step = gf.cached_attention_step(q[:3], kc, vc, n, k[:3], v[:3])
+        return [a, *torch.autograd.grad(a, (q, k, v), g), b, last, *torch.autograd.grad(b, (q, k, v), g[:, :2]), step]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        everything()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = everything()
+    for lens in ([rows - 40, 0, 40], [0, rows, 0], [5, 6, 7]):
+        cu.copy_(_cu(lens))
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [t.clone() for t in got]
+        for a, b in zip(kept, everything()):
+            assert torch.equal(a, b)
+
+
+def test_checkpointed_calls():
+    """Activation checkpointing replaces the saved tensors by recomputed ones."""
+    from torch.utils.checkpoint import checkpoint
+    gf, rows, h, d = _gf(), 300, 2, 64
+    fused, g, cu = _randn(rows, 3 * h, d, seed=110).requires_grad_(True), _randn(rows, h, d, seed=111), _cu([170, 130])
+    ld = torch.tensor([-0.02, -0.4], device='cuda')
+
+    def block(x):
+        q, k, v = (x * 0.5).split(h, 1)
+        return gf.packed_attention(q, k, v, cu) + gf.decay_attention(q, k, v, ld, cu)
+
+    want = torch.autograd.grad(block(fused), fused, g)[0]
+    assert torch.equal(torch.autograd.grad(checkpoint(block, fused, use_reentrant=False), fused, g)[0], want)
