@@ -5,8 +5,8 @@
 // Bound by reading K and V once: 4 n Hkv D bytes against 4 n Hq D operations.  The query heads that share a key head are the 16 columns of one
 // 16x16x32 product, so a cache row is read once for all of them and the vector units do no dot products; a wave walks 32-key tiles on its own --
 // loaded as whole rows, K and then V through its private LDS tile into operand layout, the next tile's loads in flight from the first product on -- and there is
-// no barrier in the key loop.  (64 sequences of up to 8191 keys, 4 key heads of width 128, 512 MB: 88 us = 5.8 TB/s;
-// with K straight into operand registers, 64 B of each of 16 rows per load, 104; without the non-temporal hint 102; parts joined in another 5.)  Where batch x key heads do not fill the chip, short caches get blocks of more waves (their parts meet in LDS), long ones are
+// no barrier in the key loop.  (64 sequences of up to 8191 keys, 4 key heads of width 128, 512 MB, cold: 93 us = 5.5 TB/s,
+// parts joined in another 5.  Call 97 us, without the non-temporal hint 108; with K straight into operand registers, 64 B of each of 16 rows per load, the kernel took 104 for 88.)  Where batch x key heads do not fill the chip, short caches get blocks of more waves (their parts meet in LDS), long ones are
 // split over blocks, and a second small kernel joins the parts (maximum, sum, unnormalised fp32 output) in a fixed order.  Lengths are read on the device: a captured graph replays with the lengths of the day.
 #include "seq_common.h"
 #include "genie_hip.h"

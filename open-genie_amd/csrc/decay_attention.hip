@@ -18,8 +18,8 @@
 // the state update's decayed operand l^(n-1-s) c_s enters as a sum of three bf16 values (2^-24 left: fp32).  The backward's states, which only become
 // operands of gradients, take two (2^-16, far under the operand's own 2^-8).
 //
-// Bound by memory and its latency.  Seven sequences of 16092 tokens, 16 heads of width 128 (66 MB a tensor): state 42 us, scan 19, outputs 68 forward and 162 for the three
-// gradients; one prompt of 32768 tokens, 8 heads of width 64 (34 MB a tensor): 17 + 8 + 32 us, about 250 MB moved at 4.4 TB/s (a large copy: 4.9).
+// Bound by memory and its latency.  Seven sequences of 16092 tokens, 16 heads of width 128 (66 MB a tensor): state 47 us, scan 18, outputs 68 forward and 156 for the three
+// gradients; one prompt of 32768 tokens, 8 heads of width 64 (34 MB a tensor): 21 + 8 + 36 us, about 250 MB moved at 3.8 TB/s (a large copy: 4.9).  All on cold inputs.
 #include "packed_common.h"
 
 #define DECAY_SEG 256
@@ -199,9 +199,9 @@ __global__ void __launch_bounds__(64 * (DH / 32), 2) decay_state_kernel(const De
 
 // States in front of the segments: M_0 = initial or 0, M_{i+1} = l^256 M_i + local_i, elementwise in fp32; each M_i is stored rounded to bf16 as the operand that it
 // becomes, the last sum is the final state.  A lane owns four elements, the block's NW waves take eight segments each: all loads of a step are in flight
-// together, the waves' sums meet in LDS, and each wave walks its own eight from there.  128 segments of 8 heads of width 64: 16 waves 8.2 us, 4 waves 9.8, one wave walking all
+// together, the waves' sums meet in LDS, and each wave walks its own eight from there.  128 segments of 8 heads of width 64: 16 waves 8.3 us, 4 waves 9.8, one wave walking all
 // of them, eight loads ahead, 18 -- a chain of store and load latencies.  Up to 32 segments a sequence four waves do it in one step: 100 MB of 63 segments of 16 heads of
-// width 128 in 21 us = 4.8 TB/s.
+// width 128 in 18 us = 5.5 TB/s (what the state kernel just wrote is partly still in the last-level cache).
 template <int NW>
 __global__ void __launch_bounds__(64 * NW) decay_scan_kernel(const DecayArgs g) {
     __shared__ __attribute__((aligned(16))) f32x4_t part[2][NW][64];
@@ -475,7 +475,8 @@ __global__ void __launch_bounds__(256, DH <= 64 ? 4 : 3) decay_out_kernel(const 
     __shared__ __attribute__((aligned(16))) char smem[decay_out_lds<DH>];
     decay_out_block<DH, false>(g, (int)blockIdx.x, smem);
 }
-// Few rows: the weights and the state in front of a sequence with what their rounding left over, for the reason at packed_exact() (a 32768-token prompt would pay 38 us for 33).  Where every sequence is one
+// Few rows: the weights and the state in front of a sequence with what their rounding left over, for the reason at packed_exact() (a 32768-token prompt would pay 38 us for 33).  The
+// state's remainder costs a second product after its own loads: 168 rows behind initial states 9.3 us for 8.4 at width 64, 12.1 for 10.6 at 128.  Where every sequence is one
 // segment and starts from nothing, the final states come from the launch's last blocks: three snippets of 168 tokens together 8 us instead of 7 + 7 in two launches.
 template <int DH>
 __global__ void __launch_bounds__(256) decay_few_kernel(const DecayArgs g, int out_blocks) {
@@ -489,7 +490,8 @@ __global__ void __launch_bounds__(256) decay_few_kernel(const DecayArgs g, int o
 // ------------------------------------------------------------------------------------------------------------------------------
 // The recurrence for one token: S' = l S + k v^T, o = scale q S'.  Bound by reading and writing the fp32 state once (8 d_k d_v bytes a head); everything else is
 // 0.4 % of that.  A thread owns four columns of every RP-th row; eight rows are in flight per thread; the rows' partial sums of o meet in LDS.  Non-temporal loads,
-// ordinary stores: 4096 states of 128 x 128 (541 MB) 81 us = 6.7 TB/s; both ordinary 103, both non-temporal 95.  Heads of
+// ordinary stores.  4096 states of 128 x 128 (541 MB), call on cold states 102 us = 5.3 TB/s: both ordinary 104, both non-temporal 96, ordinary loads and non-temporal stores 104; where the last call's
+// states are still in the last-level cache, kernel 81: both ordinary 103, both non-temporal 95.  Heads of
 // small batches are cut into column slices so that the few states spread over more CUs.
 // ------------------------------------------------------------------------------------------------------------------------------
 struct DecayStepArgs {

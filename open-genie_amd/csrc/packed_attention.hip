@@ -9,10 +9,10 @@
 // layout of the second product -- the transposed V / K / dO / Q fragments are read in that order by ds_read_b64_tr_b16, nothing is exchanged.
 // The sequences' lengths live on the device only: seq_common.h maps slots to (sequence, tile).
 //
-// Bound by the matrix cores on long sequences: 16384 rows, 8 heads of width 64, forward 297 us = 925 TFLOP/s of the products it needs; 4 x 4096 rows, 16 heads of width 128 over 4
-// key heads: forward 295 us = 930, dQ 388 us = 1060, dK / dV 570 us + 25 us for the parts' sums = 920 TFLOP/s of the products they do (bf16 library products of 8192^3 and
-// more reach 1340 here).  On short ones by the chain of a sequence's tiles (7 ragged sequences of up to 2048 rows: 27, 30 and 42 + 6 us against 21 us of products in all), and under
-// 256 rows by the launch.
+// Bound by the matrix cores on long sequences: 16384 rows, 8 heads of width 64, forward 306 us = 898 TFLOP/s of the products it needs; 4 x 4096 rows, 16 heads of width 128 over 4
+// key heads: forward 295 us = 931, dQ 386 us = 1069, dK / dV 540 us + 26 us for the parts' sums = 971 TFLOP/s of the products they do (bf16 library products of 8192^3 and
+// more reach 1340 here).  On short ones by the chain of a sequence's tiles (7 ragged sequences of up to 2048 rows: 27, 29 and 40 + 7 us against 21 us of products in all), and under
+// 256 rows by the launch.  (Medians of kernel traces in a steady run on cold inputs, scripts/sequence_kernels.py; single passes from idle clocks take up to a sixth longer.)
 #include "packed_common.h"
 
 // ------------------------------------------------------------------------------------------------------------------------------
